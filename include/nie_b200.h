@@ -407,6 +407,115 @@ int nie_linear_timeout_test(const void* x, int64_t ldx, const void* w, int64_t n
                             int32_t dtype, int32_t* err_flag, void* stream,
                             uint32_t wait_probes);
 
+/* ------------------------------------------------- 8-bit paged KV cache
+ * (No reference counterpart: the reference's cache has the activation's type.)
+ *
+ * Codes: key_cache / value_cache of the layout above in e4m3, one byte per
+ * element.  Scales: key_scales / value_scales, fp32 [num_layers, num_blocks,
+ * kv_heads], contiguous.  The value of a code is code * scale.  The scales that
+ * the appending calls write are powers of two in [2^-48, 2^48]; the readers
+ * take any scale in that range.
+ *
+ * nie_rope_write_kv8: rotates q and k (halves (a, b) of a head to
+ * (a cos - b sin, b cos + a sin), fp32, rounded once) and appends the rotated
+ * k and v.  q/k/v: rows of heads * head_dim elements at *_stride; sin/cos
+ * [num_tokens, head_dim / 2]; q_out [num_tokens, q_heads, head_dim].  Arguments
+ * otherwise as nie_rope_write_kv.
+ * nie_write_kv8: appends k and v as they are.
+ *
+ * The tokens of a call that lie in one block must be neighbours (tokens without
+ * a slot between them do not count), as nie_pack_ragged gives them; a block
+ * that occurs in two places of a call has undefined contents.  Neighbours whose
+ * slots follow one another are a run; a block's runs are taken in turn.
+ * The scale s of a run is the least power of two with max|x| <= 448 s.  Where
+ * the run continues a block (its first slot is not the block's first), s is not
+ * below the block's scale, and if it is above, the codes in front of the run
+ * are brought to s.  Non-finite values are stored as NaN and do not count for the scale;
+ * magnitudes above 448 * 2^48 saturate.  Slots below 0 are skipped; slots at or
+ * past num_blocks * block_size are skipped and raise NIE_DEV_ERR_SLOT_RANGE.
+ */
+int nie_rope_write_kv8(const void* q, int64_t q_stride, const void* k,
+                       int64_t k_stride, const void* v, int64_t v_stride,
+                       const void* sin, const void* cos, int64_t num_tokens,
+                       int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                       void* q_out, void* key_cache, void* value_cache,
+                       float* key_scales, float* value_scales, int32_t dtype,
+                       int32_t layer, int64_t num_layers, int64_t num_blocks,
+                       int32_t block_size, const int64_t* slot_mapping,
+                       int32_t* err_flag, void* stream);
+
+int nie_write_kv8(const void* keys, int64_t k_stride, const void* values,
+                  int64_t v_stride, int64_t num_tokens, void* key_cache,
+                  void* value_cache, float* key_scales, float* value_scales,
+                  int32_t dtype, int32_t layer, int64_t num_layers,
+                  int64_t num_blocks, int32_t block_size, int32_t kv_heads,
+                  int32_t head_dim, const int64_t* slot_mapping,
+                  int32_t* err_flag, void* stream);
+
+/* nie_gather_kv8: the first num_tokens tokens of a block table as values of
+ * out_dtype, [num_tokens, kv_heads, head_dim] each (code * scale in fp32,
+ * rounded once).  Tokens of a block outside the pool give zeros and raise
+ * NIE_DEV_ERR_BLOCK_RANGE. */
+int nie_gather_kv8(const void* key_cache, const void* value_cache,
+                   const float* key_scales, const float* value_scales,
+                   int32_t layer, int64_t num_layers, int64_t num_blocks,
+                   int32_t block_size, int32_t kv_heads, int32_t head_dim,
+                   const int32_t* block_table, int64_t num_tokens,
+                   void* out_keys, void* out_values, int32_t out_dtype,
+                   int32_t* err_flag, void* stream);
+
+/* nie_paged_decode_kv8 / nie_varlen_attention_kv8: nie_paged_decode /
+ * nie_varlen_attention over an 8-bit cache; q and out have `dtype` and
+ * num_q_rows rows.  Scores, softmax and sums are fp32 and the output is
+ * rounded once (the scores are not rounded to the activation's type).  A row
+ * that sees no key (seq_len 0) is zeros.  A request with a query row outside
+ * [0, num_q_rows) raises NIE_DEV_ERR_CAPACITY and is skipped; a key whose block
+ * is outside the pool raises NIE_DEV_ERR_BLOCK_RANGE.  head_dim <= 256. */
+int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* out,
+                         int64_t out_row_stride, int64_t num_q_rows,
+                         const void* key_cache, const void* value_cache,
+                         const float* key_scales, const float* value_scales,
+                         int32_t dtype, int32_t layer, int64_t num_layers,
+                         int64_t num_blocks, int32_t block_size,
+                         int32_t kv_heads, int32_t head_dim, int32_t q_heads,
+                         const int32_t* block_tables, int64_t table_stride,
+                         const int32_t* table_rows, const int32_t* seq_lens,
+                         const int64_t* q_rows, const int32_t* req_list,
+                         int32_t num_requests, float scale, int32_t* err_flag,
+                         void* stream);
+
+int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, void* out,
+                             int64_t out_row_stride, int64_t num_q_rows,
+                             const void* key_cache, const void* value_cache,
+                             const float* key_scales, const float* value_scales,
+                             int32_t dtype, int32_t layer, int64_t num_layers,
+                             int64_t num_blocks, int32_t block_size,
+                             int32_t kv_heads, int32_t head_dim,
+                             int32_t q_heads, const int32_t* block_tables,
+                             int64_t table_stride, const int32_t* table_rows,
+                             const int32_t* seq_lens,
+                             const int64_t* query_start_loc,
+                             const int32_t* req_list, int32_t num_requests,
+                             int32_t max_query_len, float scale,
+                             int32_t* err_flag, void* stream);
+
+/*
+ * nie_token_logprobs: for each row of logits (`cols` elements at row_stride)
+ *   logprobs[r]  log softmax(logits[r])[tokens[r]]
+ *   entropy[r]   -sum p log p of the row (terms with p = 0 are 0)
+ *   top_logprobs / top_ids [rows, top]  the `top` largest logits' log
+ *                probabilities and indices, largest first, ties to the lowest
+ *                index, NaN before every number
+ * in fp32.  A row that holds NaN or +inf, or only -inf, has NaN results (its
+ * top_ids still rank).  A token outside [0, cols) has logprob NaN and raises
+ * NIE_DEV_ERR_INDEX_RANGE.  0 <= top <= 32 and top <= cols.
+ */
+int nie_token_logprobs(const void* logits, int64_t rows, int64_t cols,
+                       int64_t row_stride, int32_t dtype, const int64_t* tokens,
+                       int32_t top, float* logprobs, float* entropy,
+                       float* top_logprobs, int64_t* top_ids, int32_t* err_flag,
+                       void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -26,6 +26,9 @@ SOURCES = (
     "nie_attn_prefill.cu",
     "nie_fused.cu",
     "nie_linear.cu",
+    "nie_kv8.cu",
+    "nie_kv8_attn.cu",
+    "nie_logprobs.cu",
 )
 
 ARCH_FLAGS = ("-gencode", "arch=compute_100a,code=sm_100a")

@@ -104,6 +104,39 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int32, c_void_p, c_void_p]
         + [ctypes.c_uint32],
     ),
+    "nie_rope_write_kv8": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int32, c_int32]
+        + [c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32, c_int64, c_int64, c_int32]
+        + [c_void_p, c_void_p, c_void_p],
+    ),
+    "nie_write_kv8": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32]
+        + [c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p],
+    ),
+    "nie_gather_kv8": (
+        c_int,
+        [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p]
+        + [c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_void_p],
+    ),
+    "nie_paged_decode_kv8": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32]
+        + [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]
+        + [c_void_p, c_int32, c_float, c_void_p, c_void_p],
+    ),
+    "nie_varlen_attention_kv8": (
+        c_int,
+        [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32]
+        + [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_void_p, c_void_p]
+        + [c_void_p, c_int32, c_int32, c_float, c_void_p, c_void_p],
+    ),
+    "nie_token_logprobs": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]
+        + [c_void_p, c_void_p],
+    ),
     "nie_varlen_workspace_size": (c_size_t, [c_int32, c_int32, c_int32, c_int32]),
     "nie_varlen_attention": (
         c_int,

@@ -1,0 +1,317 @@
+// Appending to and reading back the 8-bit paged cache.
+//
+//   rope_write_kv8 : q' = rope(q); k' = rope(k); k' and v go to the cache
+//                    slots in e4m3 with one scale per (block, kv head)
+//   write_kv8      : the same without the rotation (k stored as given)
+//   gather_kv8     : a table's tokens as values (code * scale)
+//
+// Rotation: (a, b) -> (a c - b s, b c + a s) on the halves of a head, in fp32
+// without fused multiply-add, rounded once: q' to the activation type, k'
+// straight to 8 bits.
+//
+// Scale of a block: tokens of one call that are neighbours, lie in one block
+// and have slots that follow one another ("a run") share s = 2^e, the least power of
+// two with max|x| <= 448 s.  A run that continues a block (its first slot is
+// not the block's first) never lowers the block's scale; where it raises it,
+// the codes before the run are brought to the new scale.  A power of two
+// costs no precision in a floating format and makes that step exact except
+// for codes that become subnormal.  Scales stay in [2^-48, 2^48]; values
+// beyond 448 * 2^48 saturate.  Non-finite values are stored as NaN and do not
+// count for the scale.
+//
+// One warp owns a (block, kv head, K or V) and takes the block's runs in turn,
+// as calls of their own would be, so no two warps write one scale or one code
+// and the result does not depend on the order of the warps.
+#include "nie_kv8.cuh"
+
+#include <algorithm>
+
+namespace nie {
+
+struct AppendArgs {
+  const void* q;  // null: no queries to rotate
+  const void* k;
+  const void* v;
+  int64_t q_stride, k_stride, v_stride;  // elements between token rows
+  const void* sin;  // null: k is stored as given
+  const void* cos;
+  int64_t tokens;
+  int hq, hkv, hd, bs;
+  void* q_out;
+  uint8_t* codes[2];   // K, V codes of the layer
+  float* scales[2];    // K, V scales of the layer
+  int64_t total_slots;
+  const int64_t* slots;
+  int32_t* err;
+};
+
+// The block of a token's slot; -1 for a token that is not stored.
+__device__ __forceinline__ int64_t block_of(const AppendArgs& a, int64_t t) {
+  const int64_t slot = a.slots[t];
+  return slot < 0 || slot >= a.total_slots ? -1 : slot / a.bs;
+}
+
+// True if token t (of block >= 0) is the first of its block's stretch: the
+// stored token before it, tokens without a slot passed over, lies elsewhere.
+__device__ __forceinline__ bool begins_block(const AppendArgs& a, int64_t t, int64_t block) {
+  for (int64_t p = t - 1; p >= 0; --p) {
+    const int64_t b = block_of(a, p);
+    if (b >= 0) return b != block;
+  }
+  return true;
+}
+
+// Number of tokens of the run that starts at t: slots that follow one another in one block.
+__device__ __forceinline__ int run_length(const AppendArgs& a, int64_t t, int64_t block) {
+  const int64_t slot = a.slots[t];
+  const int64_t most = min(a.tokens - t, (block + 1) * a.bs - slot);
+  int n = 1;
+  while (n < most && a.slots[t + n] == slot + n) ++n;
+  return n;
+}
+
+// First token of the block's next run behind token t, or -1: tokens without a slot are passed over.
+__device__ __forceinline__ int64_t next_run(const AppendArgs& a, int64_t t, int64_t block) {
+  for (; t < a.tokens; ++t) {
+    const int64_t b = block_of(a, t);
+    if (b >= 0) return b == block ? t : -1;
+  }
+  return -1;
+}
+
+// A value that has no 8-bit form becomes NaN.
+__device__ __forceinline__ float finite_or_nan(float x) {
+  return fabsf(x) <= 3.402823466e38f ? x : __int_as_float(0x7fc00000);
+}
+
+// The least power of two whose 448-fold is not below amax, in the bounds:
+// 448 = 1.75 * 2^8, so with amax = m 2^e (1 <= m < 2) it is 2^(e-8), or
+// 2^(e-7) when m > 1.75.
+__device__ __forceinline__ float scale_for(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  const int e = (int)(bits >> 23) + ((bits & 0x7fffffu) > 0x600000u ? -7 : -8);  // biased
+  if (e <= 127 - 48) return kScaleMin;
+  if (e >= 127 + 48) return kScaleMax;
+  return __uint_as_float((uint32_t)e << 23);
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+
+// New scale of a block for a run whose largest magnitude is `amax`; the codes
+// of the rows [0, off) are brought to it.  Called by a whole warp.
+__device__ __forceinline__ float settle_scale(const AppendArgs& a, int kv, int64_t block, int head, int off, float amax,
+                                              int lane) {
+  float* sp = a.scales[kv] + block * a.hkv + head;
+  float s = scale_for(amax);
+  if (off > 0) {
+    const float old = fminf(fmaxf(*sp, kScaleMin), kScaleMax);
+    if (s > old) {
+      const float ratio = old / s;
+      const int64_t row = (int64_t)a.hkv * a.hd;
+      uint8_t* base = a.codes[kv] + block * a.bs * row + (int64_t)head * a.hd;
+      for (int i = lane; i < off * a.hd; i += 32) {
+        uint8_t* c = base + (int64_t)(i / a.hd) * row + i % a.hd;
+        *c = (uint8_t)floats_to_e4m3x2(e4m3_to_float(*c) * ratio, 0.f);
+      }
+    } else {
+      s = old;
+    }
+  }
+  __syncwarp();
+  if (lane == 0) *sp = s;
+  return s;
+}
+
+// One CTA per token: its warps rotate the token's queries and, where a run
+// begins, take the run's (K / V, head) pairs in turn.  Any even head_dim, any
+// alignment; a run's values are read twice.
+template <typename T>
+__global__ void __launch_bounds__(256) append_kv8_kernel(AppendArgs a) {
+  using N = Num<T>;
+  pdl_wait();     // dependent launch: q/k/v come from the projection before
+  pdl_trigger();  // the kernel after this one may start its prologue
+  const int64_t t = blockIdx.x;
+  const int half = a.hd / 2;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const T* sn = reinterpret_cast<const T*>(a.sin);
+  const T* cs = reinterpret_cast<const T*>(a.cos);
+  if (a.q) {
+    const T* q = reinterpret_cast<const T*>(a.q) + t * a.q_stride;
+    T* out = reinterpret_cast<T*>(a.q_out) + t * a.hq * a.hd;
+    for (int p = threadIdx.x; p < a.hq * half; p += blockDim.x) {
+      const int h = p / half, i = p % half;
+      const float x1 = N::to_f(q[h * a.hd + i]), x2 = N::to_f(q[h * a.hd + i + half]);
+      const float c = N::to_f(cs[t * half + i]), s = N::to_f(sn[t * half + i]);
+      out[h * a.hd + i] = N::from_f(__fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s)));
+      out[h * a.hd + i + half] = N::from_f(__fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s)));
+    }
+  }
+  if (a.slots[t] >= a.total_slots && threadIdx.x == 0) raise_flag(a.err, NIE_DEV_ERR_SLOT_RANGE);
+  const int64_t block = block_of(a, t);
+  if (block < 0 || !begins_block(a, t, block)) return;
+  const int64_t row = (int64_t)a.hkv * a.hd;
+  for (int task = warp; task < 2 * a.hkv; task += warps) {
+    const int kv = task >= a.hkv, head = task - kv * a.hkv;
+    const bool rotate = kv == 0 && a.sin != nullptr;
+    const T* src = reinterpret_cast<const T*>(kv ? a.v : a.k);
+    const int64_t stride = kv ? a.v_stride : a.k_stride;
+    for (int64_t first = t; first >= 0;) {
+      const int n = run_length(a, first, block);
+      const int off = (int)(a.slots[first] - block * a.bs);
+      auto value = [&](int j, int d) -> float {
+        const T* x = src + (first + j) * stride + (int64_t)head * a.hd;
+        if (!rotate) return finite_or_nan(N::to_f(x[d]));
+        const int i = d < half ? d : d - half;
+        const float x1 = N::to_f(x[i]), x2 = N::to_f(x[i + half]);
+        const float c = N::to_f(cs[(first + j) * half + i]), s = N::to_f(sn[(first + j) * half + i]);
+        return finite_or_nan(d < half ? __fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s))
+                                      : __fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s)));
+      };
+      float amax = 0.f;
+      for (int i = lane; i < n * a.hd; i += 32) amax = fmaxf(amax, fabsf(value(i / a.hd, i % a.hd)));  // skips NaN
+      const float s = settle_scale(a, kv, block, head, off, warp_max(amax), lane);
+      uint8_t* dst = a.codes[kv] + (block * a.bs + off) * row + (int64_t)head * a.hd;
+      for (int i = lane; i < n * a.hd; i += 32)
+        dst[(int64_t)(i / a.hd) * row + i % a.hd] = (uint8_t)floats_to_e4m3x2(value(i / a.hd, i % a.hd) / s, 0.f);
+      __syncwarp();
+      first = next_run(a, first + n, block);
+    }
+  }
+}
+
+// Values of a table's first T tokens, one element per thread and step.
+template <typename T>
+__global__ void __launch_bounds__(256) gather_kv8_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+                                                         const float* __restrict__ ks, const float* __restrict__ vs,
+                                                         int64_t nb, int bs, int hkv, int hd,
+                                                         const int32_t* __restrict__ table, int64_t n,
+                                                         T* __restrict__ ok, T* __restrict__ ov,
+                                                         int32_t* __restrict__ err) {
+  const int64_t row = (int64_t)hkv * hd;
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n * row; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t t = i / row;
+    const int e = (int)(i % row);
+    const int64_t block = table[t / bs];
+    float k = 0.f, v = 0.f;
+    if (block < 0 || block >= nb) {
+      raise_flag(err, NIE_DEV_ERR_BLOCK_RANGE);
+    } else {
+      const int64_t at = (block * bs + t % bs) * row + e;
+      k = e4m3_to_float(kc[at]) * ks[block * hkv + e / hd];
+      v = e4m3_to_float(vc[at]) * vs[block * hkv + e / hd];
+    }
+    ok[i] = Num<T>::from_f(k);
+    ov[i] = Num<T>::from_f(v);
+  }
+}
+
+template <typename T>
+static void launch_append(const AppendArgs& a, cudaStream_t s) {
+  pdl_launch(append_kv8_kernel<T>, dim3((unsigned)a.tokens), dim3(256), s, a);
+}
+
+static int append(AppendArgs a, void* key_codes, void* value_codes, float* key_scales, float* value_scales,
+                  int32_t dtype, int32_t layer, int64_t num_layers, int64_t num_blocks, cudaStream_t s) {
+  NIE_REQUIRE(a.k && a.v && key_codes && value_codes && key_scales && value_scales && a.slots, "null pointer argument");
+  NIE_REQUIRE(a.tokens >= 0 && a.tokens < (int64_t(1) << 31), "num_tokens out of range");
+  NIE_REQUIRE(layer >= 0 && layer < num_layers, "layer %d out of range", layer);
+  NIE_REQUIRE(a.hkv > 0 && a.hd > 0 && a.bs > 0 && num_blocks > 0, "bad cache geometry");
+  NIE_REQUIRE(dtype_size(dtype) > 0, "unknown dtype %d", dtype);
+  if (a.tokens == 0) return NIE_OK;
+  a.total_slots = num_blocks * a.bs;
+  const int64_t codes = (int64_t)layer * a.total_slots * a.hkv * a.hd, scales = (int64_t)layer * num_blocks * a.hkv;
+  a.codes[0] = (uint8_t*)key_codes + codes;
+  a.codes[1] = (uint8_t*)value_codes + codes;
+  a.scales[0] = key_scales + scales;
+  a.scales[1] = value_scales + scales;
+  switch (dtype) {
+    case NIE_DTYPE_BF16: launch_append<__nv_bfloat16>(a, s); break;
+    case NIE_DTYPE_F32: launch_append<float>(a, s); break;
+    default: launch_append<__half>(a, s); break;
+  }
+  return check_launch("append_kv8_kernel");
+}
+
+}  // namespace nie
+
+using namespace nie;
+
+extern "C" int nie_rope_write_kv8(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                                  int64_t v_stride, const void* sin, const void* cos, int64_t num_tokens,
+                                  int32_t q_heads, int32_t kv_heads, int32_t head_dim, void* q_out, void* key_cache,
+                                  void* value_cache, float* key_scales, float* value_scales, int32_t dtype,
+                                  int32_t layer, int64_t num_layers, int64_t num_blocks, int32_t block_size,
+                                  const int64_t* slot_mapping, int32_t* err_flag, void* stream) {
+  NIE_REQUIRE(q && sin && cos && q_out, "null pointer argument");
+  NIE_REQUIRE(q_heads > 0, "bad geometry");
+  NIE_REQUIRE(head_dim > 0 && head_dim % 2 == 0, "head_dim must be even");
+  AppendArgs a{};
+  a.q = q, a.k = k, a.v = v;
+  a.q_stride = q_stride, a.k_stride = k_stride, a.v_stride = v_stride;
+  a.sin = sin, a.cos = cos;
+  a.tokens = num_tokens;
+  a.hq = q_heads, a.hkv = kv_heads, a.hd = head_dim, a.bs = block_size;
+  a.q_out = q_out;
+  a.slots = slot_mapping;
+  a.err = err_flag;
+  return append(a, key_cache, value_cache, key_scales, value_scales, dtype, layer, num_layers, num_blocks,
+                reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int nie_write_kv8(const void* keys, int64_t k_stride, const void* values, int64_t v_stride,
+                             int64_t num_tokens, void* key_cache, void* value_cache, float* key_scales,
+                             float* value_scales, int32_t dtype, int32_t layer, int64_t num_layers, int64_t num_blocks,
+                             int32_t block_size, int32_t kv_heads, int32_t head_dim, const int64_t* slot_mapping,
+                             int32_t* err_flag, void* stream) {
+  AppendArgs a{};
+  a.k = keys, a.v = values;
+  a.k_stride = k_stride, a.v_stride = v_stride;
+  a.tokens = num_tokens;
+  a.hkv = kv_heads, a.hd = head_dim, a.bs = block_size;
+  a.slots = slot_mapping;
+  a.err = err_flag;
+  return append(a, key_cache, value_cache, key_scales, value_scales, dtype, layer, num_layers, num_blocks,
+                reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int nie_gather_kv8(const void* key_cache, const void* value_cache, const float* key_scales,
+                              const float* value_scales, int32_t layer, int64_t num_layers, int64_t num_blocks,
+                              int32_t block_size, int32_t kv_heads, int32_t head_dim, const int32_t* block_table,
+                              int64_t num_tokens, void* out_keys, void* out_values, int32_t out_dtype,
+                              int32_t* err_flag, void* stream) {
+  NIE_REQUIRE(layer >= 0 && layer < num_layers, "layer %d out of range", layer);
+  NIE_REQUIRE(key_cache && value_cache && key_scales && value_scales && block_table && out_keys && out_values,
+              "null pointer argument");
+  NIE_REQUIRE(num_blocks > 0 && block_size > 0 && kv_heads > 0 && head_dim > 0, "bad cache geometry");
+  NIE_REQUIRE(dtype_size(out_dtype) > 0, "unknown dtype %d", out_dtype);
+  if (num_tokens <= 0) return NIE_OK;
+  const int64_t codes = (int64_t)layer * num_blocks * block_size * kv_heads * head_dim;
+  const int64_t scales = (int64_t)layer * num_blocks * kv_heads;
+  const uint8_t* kc = (const uint8_t*)key_cache + codes;
+  const uint8_t* vc = (const uint8_t*)value_cache + codes;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  const int64_t n = num_tokens * kv_heads * head_dim;
+  const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, 148 * 32);
+  switch (out_dtype) {
+    case NIE_DTYPE_BF16:
+      gather_kv8_kernel<<<grid, 256, 0, s>>>(kc, vc, key_scales + scales, value_scales + scales, num_blocks, block_size,
+                                             kv_heads, head_dim, block_table, num_tokens, (__nv_bfloat16*)out_keys,
+                                             (__nv_bfloat16*)out_values, err_flag);
+      break;
+    case NIE_DTYPE_F32:
+      gather_kv8_kernel<<<grid, 256, 0, s>>>(kc, vc, key_scales + scales, value_scales + scales, num_blocks, block_size,
+                                             kv_heads, head_dim, block_table, num_tokens, (float*)out_keys,
+                                             (float*)out_values, err_flag);
+      break;
+    default:
+      gather_kv8_kernel<<<grid, 256, 0, s>>>(kc, vc, key_scales + scales, value_scales + scales, num_blocks, block_size,
+                                             kv_heads, head_dim, block_table, num_tokens, (__half*)out_keys,
+                                             (__half*)out_values, err_flag);
+      break;
+  }
+  return check_launch("gather_kv8_kernel");
+}

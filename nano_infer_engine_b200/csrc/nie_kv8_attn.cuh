@@ -1,0 +1,56 @@
+// Declarations shared by the attention kernels over the 8-bit paged cache.
+#pragma once
+
+#include "nie_kv8.cuh"
+
+namespace nie {
+
+struct Kv8Args {
+  const void* q;
+  void* out;
+  int64_t q_stride, out_stride;  // elements between token rows
+  int64_t num_q_rows;            // rows of q and out
+  const uint8_t* kc;             // codes and scales of the layer
+  const uint8_t* vc;
+  const float* ks;
+  const float* vs;
+  int64_t nb;
+  int bs, hkv, hd, hq, group;
+  const int32_t* tables;
+  int64_t tstride;
+  const int32_t* table_rows;
+  const int32_t* seq_lens;
+  const int64_t* q_rows;  // single-token calls: a request's query row (null: its index)
+  const int64_t* qsl;     // ragged calls (non-null): a request's rows are [qsl[r], qsl[r + 1])
+  const int32_t* req_list;
+  float scale;
+  int32_t* err;
+};
+
+// Query rows of request r: [first, first + count); row j sees the keys [0, keys + j].
+struct Kv8Rows {
+  int64_t first;
+  int64_t count;
+  int64_t keys;
+};
+
+// Rows outside [0, num_q_rows) do not exist: the request is flagged and has none.
+__device__ __forceinline__ Kv8Rows kv8_rows(const Kv8Args& a, int r) {
+  Kv8Rows x;
+  const int64_t n = a.seq_lens[r];
+  if (a.qsl) {
+    x.first = a.qsl[r];
+    x.count = a.qsl[r + 1] - x.first;
+  } else {
+    x.first = a.q_rows ? a.q_rows[r] : (int64_t)r;
+    x.count = 1;
+  }
+  x.keys = n - x.count;
+  if (x.count > 0 && (x.first < 0 || x.first + x.count > a.num_q_rows)) {
+    raise_flag(a.err, NIE_DEV_ERR_CAPACITY);
+    x.count = 0;
+  }
+  return x;
+}
+
+}  // namespace nie

@@ -854,6 +854,460 @@ def argmax_rows(logits: torch.Tensor) -> torch.Tensor:
     return out
 
 
+@dataclass
+class TokenLogprobs:
+    """What :func:`token_logprobs` gives for the rows of a logits matrix."""
+
+    logprobs: torch.Tensor  # float32 [R]: log probability of the given token
+    entropy: torch.Tensor  # float32 [R]: of the row's distribution, in nats
+    top_logprobs: torch.Tensor  # float32 [R, top], largest first
+    top_ids: torch.Tensor  # int64 [R, top]; ties go to the lowest id
+
+
+LOGPROBS_MAX_TOP = 32
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) -> TokenLogprobs:
+    """Log probability of ``tokens[r]`` under ``softmax(logits[r])`` for ``[R, V]`` rows, the
+    entropy of each row and its ``top`` (0..32) likeliest tokens, in fp32.
+
+    Rows may have a stride.  Entries of -inf (forbidden tokens) have probability 0; a row that holds
+    NaN or +inf, or nothing but -inf, has NaN results.  A token outside the vocabulary has logprob
+    NaN and sets the device error flag (:func:`check_device_errors`).
+    """
+    if logits.ndim != 2 or logits.shape[1] < 1 or logits.stride(1) != 1:
+        raise ValueError("logits must be [rows, vocab] with unit inner stride")
+    rows, cols = logits.shape
+    if tokens.dtype != torch.int64 or tokens.shape != (rows,):
+        raise ValueError("tokens must be int64 with one token per row")
+    if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= min(LOGPROBS_MAX_TOP, cols):
+        raise ValueError(f"top must be an integer in [0, {min(LOGPROBS_MAX_TOP, cols)}]")
+    code = dtype_code(logits.dtype)
+    _require_cuda(logits, tokens)
+    device = _one_device(logits, tokens)
+    tokens = tokens.contiguous()
+    out = torch.empty((2, rows), dtype=torch.float32, device=device)
+    top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
+    top_ids = torch.empty((rows, top), dtype=torch.int64, device=device)
+    if rows == 0:
+        return TokenLogprobs(out[0], out[1], top_logprobs, top_ids)
+    with _on(device):
+        status = lib.nie_token_logprobs(
+            logits.data_ptr(),
+            rows,
+            cols,
+            logits.stride(0) if rows > 1 else cols,
+            code,
+            tokens.data_ptr(),
+            top,
+            out[0].data_ptr(),
+            out[1].data_ptr(),
+            top_logprobs.data_ptr(),
+            top_ids.data_ptr(),
+            error_flag(device).data_ptr(),
+            _stream(device),
+        )
+    check(status, "nie_token_logprobs")
+    _count()
+    return TokenLogprobs(out[0], out[1], top_logprobs, top_ids)
+
+
+# ------------------------------------------------------- 8-bit paged cache
+# Codes in e4m3, [layers, blocks, block_size, kv_heads, head_dim], and one fp32
+# scale per layer, block and kv head; the value of a code is code * scale.
+KV8_DTYPE = torch.float8_e4m3fn
+
+
+class _NoGuard:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_no_guard = _NoGuard()
+
+
+def _on(device: torch.device):
+    """Guard that makes ``device`` current (nothing to do when it is)."""
+    return _no_guard if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _one_device(*tensors: torch.Tensor | None) -> torch.device:
+    device = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"tensors must share a device (got {device} and {t.device})")
+    return device
+
+
+def _kv8_geometry(
+    key_cache: torch.Tensor, value_cache: torch.Tensor, key_scales: torch.Tensor, value_scales: torch.Tensor, layer: int
+) -> tuple[int, int, int, int, int]:
+    L, nb, bs, h, d = _cache_geometry(key_cache)
+    if key_cache.dtype != KV8_DTYPE or value_cache.dtype != KV8_DTYPE:
+        raise ValueError("8-bit caches must be float8_e4m3fn")
+    if value_cache.shape != key_cache.shape or not value_cache.is_contiguous():
+        raise ValueError("key and value caches must be contiguous and share a shape")
+    for s in (key_scales, value_scales):
+        if s.dtype != torch.float32 or s.shape != (L, nb, h) or not s.is_contiguous():
+            raise ValueError("scales must be contiguous float32 [num_layers, num_blocks, kv_heads]")
+    if not 0 <= layer < L:
+        raise IndexError("layer out of range")
+    return L, nb, bs, h, d
+
+
+def _check_slots(slot_mapping: torch.Tensor, tokens: int) -> None:
+    if (slot_mapping.dtype != torch.int64 or slot_mapping.ndim != 1 or slot_mapping.shape[0] < tokens
+            or not slot_mapping.is_contiguous()):
+        raise ValueError("slot_mapping must be contiguous int64 with one slot per token")
+
+
+def rope_write_kv8(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    sin: torch.Tensor,
+    cos: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer: int,
+    slot_mapping: torch.Tensor,
+    q_heads: int,
+) -> torch.Tensor:
+    """:func:`rope_write_kv` for an 8-bit cache: rotate q/k and append k/v in e4m3.
+
+    The rotation is fp32, rounded once.  The tokens of the call that lie in one block (neighbours,
+    as :func:`pack_ragged` gives them; a block may not occur in two places of a call) share per kv
+    head the least power-of-two scale that holds them; where they continue a block its scale never
+    falls, and where it grows the block's earlier codes are brought to it.  Non-finite values are
+    stored as NaN.  Returns the rotated queries as ``[T, q_heads, D]``.
+    """
+    L, nb, bs, h, d = _kv8_geometry(key_cache, value_cache, key_scales, value_scales, layer)
+    T = q.shape[0]
+    if d % 2:
+        raise ValueError("head_dim must be even")
+    for t, width in ((q, q_heads * d), (k, h * d), (v, h * d)):
+        if t.ndim != 2 or t.shape != (T, width) or t.stride(1) != 1 or t.dtype != q.dtype:
+            raise ValueError("q/k/v must be [T, heads*head_dim] of one dtype with unit inner stride")
+    for t in (sin, cos):
+        if t.shape != (T, d // 2) or not t.is_contiguous() or t.dtype != q.dtype:
+            raise ValueError("sin/cos must be contiguous [T, head_dim/2] of q's dtype")
+    _check_slots(slot_mapping, T)
+    code = dtype_code(q.dtype)
+    _require_cuda(q, k, v, sin, cos, key_cache, value_cache, key_scales, value_scales, slot_mapping)
+    device = _one_device(q, k, v, sin, cos, key_cache, value_cache, key_scales, value_scales, slot_mapping)
+    q_out = torch.empty((T, q_heads, d), dtype=q.dtype, device=device)
+    if T == 0:
+        return q_out
+    with _on(device):
+        status = lib.nie_rope_write_kv8(
+            q.data_ptr(),
+            q.stride(0),
+            k.data_ptr(),
+            k.stride(0),
+            v.data_ptr(),
+            v.stride(0),
+            sin.data_ptr(),
+            cos.data_ptr(),
+            T,
+            q_heads,
+            h,
+            d,
+            q_out.data_ptr(),
+            key_cache.data_ptr(),
+            value_cache.data_ptr(),
+            key_scales.data_ptr(),
+            value_scales.data_ptr(),
+            code,
+            layer,
+            L,
+            nb,
+            bs,
+            slot_mapping.data_ptr(),
+            error_flag(device).data_ptr(),
+            _stream(device),
+        )
+    check(status, "nie_rope_write_kv8")
+    _count()
+    return q_out
+
+
+def write_kv8(
+    keys: torch.Tensor,
+    values: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer: int,
+    slot_mapping: torch.Tensor,
+) -> None:
+    """Append ``keys/values [T, H, D]`` to an 8-bit cache (:func:`rope_write_kv8` without the rotation)."""
+    L, nb, bs, h, d = _kv8_geometry(key_cache, value_cache, key_scales, value_scales, layer)
+    if keys.shape != values.shape or keys.ndim != 3 or keys.shape[1:] != (h, d) or keys.dtype != values.dtype:
+        raise ValueError("keys/values must be [T, kv_heads, head_dim] of one dtype matching the cache")
+    T = keys.shape[0]
+    _check_slots(slot_mapping, T)
+    code = dtype_code(keys.dtype)
+    _require_cuda(keys, values, key_cache, value_cache, key_scales, value_scales, slot_mapping)
+    device = _one_device(keys, values, key_cache, value_cache, key_scales, value_scales, slot_mapping)
+    keys = keys.contiguous()
+    values = values.contiguous()
+    if T == 0:
+        return
+    with _on(device):
+        status = lib.nie_write_kv8(
+            keys.data_ptr(),
+            h * d,
+            values.data_ptr(),
+            h * d,
+            T,
+            key_cache.data_ptr(),
+            value_cache.data_ptr(),
+            key_scales.data_ptr(),
+            value_scales.data_ptr(),
+            code,
+            layer,
+            L,
+            nb,
+            bs,
+            h,
+            d,
+            slot_mapping.data_ptr(),
+            error_flag(device).data_ptr(),
+            _stream(device),
+        )
+    check(status, "nie_write_kv8")
+    _count()
+
+
+def gather_kv8(
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer: int,
+    block_table: torch.Tensor,
+    num_tokens: int,
+    *,
+    dtype: torch.dtype = torch.bfloat16,
+) -> tuple[torch.Tensor, torch.Tensor]:
+    """The first ``num_tokens`` K/V rows of a block table as values (``code * scale``) of ``dtype``."""
+    L, nb, bs, h, d = _kv8_geometry(key_cache, value_cache, key_scales, value_scales, layer)
+    if block_table.dtype != torch.int32 or block_table.ndim != 1 or not block_table.is_contiguous():
+        raise ValueError("block_table must be a contiguous 1-D int32 tensor")
+    if not 0 <= num_tokens <= block_table.numel() * bs:
+        raise ValueError("num_tokens must be covered by the block table")
+    code = dtype_code(dtype)
+    _require_cuda(key_cache, value_cache, key_scales, value_scales, block_table)
+    device = _one_device(key_cache, value_cache, key_scales, value_scales, block_table)
+    out_k = torch.empty((num_tokens, h, d), dtype=dtype, device=device)
+    out_v = torch.empty_like(out_k)
+    if num_tokens == 0:
+        return out_k, out_v
+    with _on(device):
+        status = lib.nie_gather_kv8(
+            key_cache.data_ptr(),
+            value_cache.data_ptr(),
+            key_scales.data_ptr(),
+            value_scales.data_ptr(),
+            layer,
+            L,
+            nb,
+            bs,
+            h,
+            d,
+            block_table.data_ptr(),
+            num_tokens,
+            out_k.data_ptr(),
+            out_v.data_ptr(),
+            code,
+            error_flag(device).data_ptr(),
+            _stream(device),
+        )
+    check(status, "nie_gather_kv8")
+    _count()
+    return out_k, out_v
+
+
+def _check_kv8_query(
+    query: torch.Tensor, out: torch.Tensor | None, h: int, d: int, block_tables: torch.Tensor, seq_lens: torch.Tensor,
+    table_rows: torch.Tensor | None, req_list: torch.Tensor | None, num_requests: int | None,
+) -> int:
+    """Checks that the two attention calls share; returns the number of requests."""
+    if query.ndim != 3 or query.shape[2] != d or query.stride(2) != 1 or query.stride(1) != d:
+        raise ValueError("query must be [rows, q_heads, head_dim] with contiguous rows")
+    if query.shape[1] < 1 or query.shape[1] % h:
+        raise ValueError("q_heads must be a multiple of kv_heads")
+    if out is not None and (out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1
+                            or out.stride(1) != d):
+        raise ValueError("out must have the query's shape and dtype with contiguous rows")
+    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.stride(1) != 1:
+        raise ValueError("block_tables must be int32 [rows, stride] with contiguous rows")
+    for name, t in (("seq_lens", seq_lens), ("table_rows", table_rows), ("req_list", req_list)):
+        if t is not None and (t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous()):
+            raise ValueError(f"{name} must be contiguous 1-D int32")
+    requests = seq_lens.numel()
+    if table_rows is None and block_tables.shape[0] < requests:
+        raise ValueError("block_tables must have a row per request")
+    if table_rows is not None and table_rows.numel() < requests:
+        raise ValueError("table_rows must have an entry per request")
+    listed = requests if req_list is None else req_list.numel()
+    R = listed if num_requests is None else int(num_requests)
+    if not 0 <= R <= listed:
+        raise ValueError("num_requests must be covered by req_list (or seq_lens)")
+    return R
+
+
+def paged_decode_kv8(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer: int,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    *,
+    out: torch.Tensor | None = None,
+    table_rows: torch.Tensor | None = None,
+    q_rows: torch.Tensor | None = None,
+    req_list: torch.Tensor | None = None,
+    num_requests: int | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """:func:`paged_decode` over an 8-bit cache: fp32 scores, softmax and sums, the output rounded once.
+
+    A request of length 0 gives zeros; rows of ``out`` that no request has are left as they were.
+    """
+    L, nb, bs, h, d = _kv8_geometry(key_cache, value_cache, key_scales, value_scales, layer)
+    R = _check_kv8_query(query, out, h, d, block_tables, seq_lens, table_rows, req_list, num_requests)
+    if q_rows is not None and (q_rows.dtype != torch.int64 or q_rows.ndim != 1 or not q_rows.is_contiguous()
+                               or q_rows.numel() < seq_lens.numel()):
+        raise ValueError("q_rows must be contiguous int64 with an entry per request")
+    code = dtype_code(query.dtype)
+    _require_cuda(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, out, table_rows, q_rows,
+                  req_list)
+    device = _one_device(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, out, table_rows,
+                         q_rows, req_list)
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=device)
+    if R == 0:
+        return out
+    with _on(device):
+        status = lib.nie_paged_decode_kv8(
+            query.data_ptr(),
+            query.stride(0),
+            out.data_ptr(),
+            out.stride(0),
+            query.shape[0],
+            key_cache.data_ptr(),
+            value_cache.data_ptr(),
+            key_scales.data_ptr(),
+            value_scales.data_ptr(),
+            code,
+            layer,
+            L,
+            nb,
+            bs,
+            h,
+            d,
+            query.shape[1],
+            block_tables.data_ptr(),
+            block_tables.stride(0),
+            _ptr(table_rows),
+            seq_lens.data_ptr(),
+            _ptr(q_rows),
+            _ptr(req_list),
+            R,
+            float(d**-0.5 if scale is None else scale),
+            error_flag(device).data_ptr(),
+            _stream(device),
+        )
+    check(status, "nie_paged_decode_kv8")
+    _count()
+    return out
+
+
+def varlen_attention_kv8(
+    query: torch.Tensor,
+    key_cache: torch.Tensor,
+    value_cache: torch.Tensor,
+    key_scales: torch.Tensor,
+    value_scales: torch.Tensor,
+    layer: int,
+    block_tables: torch.Tensor,
+    seq_lens: torch.Tensor,
+    query_start_loc: torch.Tensor,
+    max_query_len: int,
+    *,
+    out: torch.Tensor | None = None,
+    table_rows: torch.Tensor | None = None,
+    req_list: torch.Tensor | None = None,
+    num_requests: int | None = None,
+    scale: float | None = None,
+) -> torch.Tensor:
+    """:func:`varlen_attention` over an 8-bit cache: fp32 scores, softmax and sums, the output rounded once.
+
+    ``max_query_len`` sizes the launch; it need not be exact.  A row that sees no key gives zeros; rows
+    of ``out`` that no request has are left as they were.
+    """
+    L, nb, bs, h, d = _kv8_geometry(key_cache, value_cache, key_scales, value_scales, layer)
+    R = _check_kv8_query(query, out, h, d, block_tables, seq_lens, table_rows, req_list, num_requests)
+    if (query_start_loc.dtype != torch.int64 or query_start_loc.ndim != 1 or not query_start_loc.is_contiguous()
+            or query_start_loc.numel() < seq_lens.numel() + 1):
+        raise ValueError("query_start_loc must be contiguous int64 with one boundary more than requests")
+    if int(max_query_len) < 1:
+        raise ValueError("max_query_len must be positive")
+    code = dtype_code(query.dtype)
+    _require_cuda(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, query_start_loc, out,
+                  table_rows, req_list)
+    device = _one_device(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, query_start_loc,
+                         out, table_rows, req_list)
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=device)
+    if R == 0:
+        return out
+    with _on(device):
+        status = lib.nie_varlen_attention_kv8(
+            query.data_ptr(),
+            query.stride(0),
+            out.data_ptr(),
+            out.stride(0),
+            query.shape[0],
+            key_cache.data_ptr(),
+            value_cache.data_ptr(),
+            key_scales.data_ptr(),
+            value_scales.data_ptr(),
+            code,
+            layer,
+            L,
+            nb,
+            bs,
+            h,
+            d,
+            query.shape[1],
+            block_tables.data_ptr(),
+            block_tables.stride(0),
+            _ptr(table_rows),
+            seq_lens.data_ptr(),
+            query_start_loc.data_ptr(),
+            _ptr(req_list),
+            R,
+            int(max_query_len),
+            float(d**-0.5 if scale is None else scale),
+            error_flag(device).data_ptr(),
+            _stream(device),
+        )
+    check(status, "nie_varlen_attention_kv8")
+    _count()
+    return out
+
+
 # ------------------------------------------------------ layer-loop extension
 _LAYER_LOOP_PATH = Path(__file__).resolve().parent / "_nie_torch_ext.so"
 _layer_loop: object = None
