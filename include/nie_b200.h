@@ -470,7 +470,17 @@ int nie_gather_kv8(const void* key_cache, const void* value_cache,
  * rounded once (the scores are not rounded to the activation's type).  A row
  * that sees no key (seq_len 0) is zeros.  A request with a query row outside
  * [0, num_q_rows) raises NIE_DEV_ERR_CAPACITY and is skipped; a key whose block
- * is outside the pool raises NIE_DEV_ERR_BLOCK_RANGE.  head_dim <= 256. */
+ * is outside the pool raises NIE_DEV_ERR_BLOCK_RANGE.  seq_lens, table_rows and
+ * q_rows have num_seqs entries, block_tables num_table_rows rows; a request of
+ * req_list or a row of table_rows outside them is flagged and skipped likewise.
+ * head_dim <= 256.  The decode workspace (nie_paged_decode_kv8_workspace_size
+ * bytes, 256-byte aligned) holds partial sums of one call; calls that share it
+ * must not overlap on the GPU.  overlap != 0: the kernel may start before the
+ * previous kernel on the stream ends, as nie_paged_decode_overlapped, with its
+ * precondition. */
+size_t nie_paged_decode_kv8_workspace_size(int device, int32_t num_requests,
+                                           int32_t q_heads, int32_t head_dim);
+
 int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* out,
                          int64_t out_row_stride, int64_t num_q_rows,
                          const void* key_cache, const void* value_cache,
@@ -479,10 +489,12 @@ int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* out,
                          int64_t num_blocks, int32_t block_size,
                          int32_t kv_heads, int32_t head_dim, int32_t q_heads,
                          const int32_t* block_tables, int64_t table_stride,
-                         const int32_t* table_rows, const int32_t* seq_lens,
+                         int64_t num_table_rows, const int32_t* table_rows,
+                         const int32_t* seq_lens, int32_t num_seqs,
                          const int64_t* q_rows, const int32_t* req_list,
-                         int32_t num_requests, float scale, int32_t* err_flag,
-                         void* stream);
+                         int32_t num_requests, float scale, void* workspace,
+                         size_t workspace_bytes, int32_t overlap,
+                         int32_t* err_flag, void* stream);
 
 int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, void* out,
                              int64_t out_row_stride, int64_t num_q_rows,
@@ -492,9 +504,9 @@ int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, void* out,
                              int64_t num_blocks, int32_t block_size,
                              int32_t kv_heads, int32_t head_dim,
                              int32_t q_heads, const int32_t* block_tables,
-                             int64_t table_stride, const int32_t* table_rows,
-                             const int32_t* seq_lens,
-                             const int64_t* query_start_loc,
+                             int64_t table_stride, int64_t num_table_rows,
+                             const int32_t* table_rows, const int32_t* seq_lens,
+                             int32_t num_seqs, const int64_t* query_start_loc,
                              const int32_t* req_list, int32_t num_requests,
                              int32_t max_query_len, float scale,
                              int32_t* err_flag, void* stream);

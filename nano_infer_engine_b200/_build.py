@@ -28,6 +28,7 @@ SOURCES = (
     "nie_linear.cu",
     "nie_kv8.cu",
     "nie_kv8_attn.cu",
+    "nie_kv8_decode.cu",
     "nie_logprobs.cu",
 )
 

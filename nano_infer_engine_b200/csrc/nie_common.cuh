@@ -29,7 +29,8 @@ enum SmemSlot {
   kSmemPrefill = 2,
   kSmemLinear = 3,
   kSmemLinear64 = 4,
-  kSmemSlots = 6
+  kSmemKv8Decode = 5,   // 8 instances
+  kSmemSlots = 13
 };
 int opt_in_smem(int slot, const void* kernel, size_t bytes);
 

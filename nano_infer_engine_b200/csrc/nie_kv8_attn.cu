@@ -1,5 +1,6 @@
-// Attention over the 8-bit paged cache, any activation type / block size /
-// head group, head_dim <= 256:
+// Entry points of the attention over the 8-bit paged cache, and the kernel of
+// the shapes that no other takes: any activation type / block size / head group,
+// head_dim <= 256:
 //   S = scale * q . (kc ks[block]),  P = softmax over the visible keys,
 //   out = sum P (vc vs[block]),      everything in fp32, rounded once.
 // One CTA per (request, query row, query head); its four warps walk the keys
@@ -20,8 +21,12 @@ __global__ void __launch_bounds__(kG8Warps * 32) kv8_generic_kernel(Kv8Args a) {
   constexpr int kPer = kG8MaxHd / 32;
   const int h = blockIdx.z, kvh = h / a.group;
   const int r = a.req_list ? a.req_list[blockIdx.x] : (int)blockIdx.x;
+  const int trow = r < 0 || r >= a.num_seqs ? -1 : a.table_rows ? a.table_rows[r] : r;
+  if (trow < 0 || trow >= a.num_table_rows) {
+    raise_flag(a.err, NIE_DEV_ERR_CAPACITY);
+    return;
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int trow = a.table_rows ? a.table_rows[r] : r;
   const int32_t* table = a.tables + (int64_t)trow * a.tstride;
   const int64_t row_elems = (int64_t)a.hkv * a.hd;
   const Kv8Rows rows = kv8_rows(a, r);
@@ -112,6 +117,7 @@ static int check_args(const Kv8Args& a, int32_t dtype, int32_t layer, int64_t nu
   NIE_REQUIRE(a.hq % a.hkv == 0, "q_heads must be divisible by kv_heads");
   NIE_REQUIRE(num_requests >= 0, "num_requests must be non-negative");
   NIE_REQUIRE(a.tstride > 0, "table_stride must be positive");
+  NIE_REQUIRE(a.num_q_rows >= 0 && a.num_table_rows >= 0 && a.num_seqs >= 0, "row counts must be non-negative");
   return NIE_OK;
 }
 
@@ -133,21 +139,39 @@ extern "C" int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* o
                                     const float* key_scales, const float* value_scales, int32_t dtype, int32_t layer,
                                     int64_t num_layers, int64_t num_blocks, int32_t block_size, int32_t kv_heads,
                                     int32_t head_dim, int32_t q_heads, const int32_t* block_tables,
-                                    int64_t table_stride, const int32_t* table_rows, const int32_t* seq_lens,
-                                    const int64_t* q_rows, const int32_t* req_list, int32_t num_requests, float scale,
-                                    int32_t* err_flag, void* stream) {
+                                    int64_t table_stride, int64_t num_table_rows, const int32_t* table_rows,
+                                    const int32_t* seq_lens, int32_t num_seqs, const int64_t* q_rows,
+                                    const int32_t* req_list, int32_t num_requests, float scale,
+                                    void* workspace, size_t workspace_bytes, int32_t overlap, int32_t* err_flag,
+                                    void* stream) {
   Kv8Args a{};
   a.q = q, a.out = out, a.q_stride = q_row_stride, a.out_stride = out_row_stride, a.num_q_rows = num_q_rows;
   a.kc = (const uint8_t*)key_cache, a.vc = (const uint8_t*)value_cache, a.ks = key_scales, a.vs = value_scales;
   a.nb = num_blocks, a.bs = block_size, a.hkv = kv_heads, a.hd = head_dim, a.hq = q_heads;
-  a.tables = block_tables, a.tstride = table_stride, a.table_rows = table_rows;
-  a.seq_lens = seq_lens, a.q_rows = q_rows, a.req_list = req_list;
+  a.tables = block_tables, a.tstride = table_stride, a.num_table_rows = num_table_rows, a.table_rows = table_rows;
+  a.seq_lens = seq_lens, a.num_seqs = num_seqs, a.q_rows = q_rows, a.req_list = req_list;
   a.scale = scale, a.err = err_flag;
   const int rc = check_args(a, dtype, layer, num_layers, num_requests);
   if (rc != NIE_OK) return rc;
   if (num_requests == 0) return NIE_OK;
   to_layer(a, layer);
-  return launch_kv8_generic(dtype, a, num_requests, 1, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (kv8_decode_takes(dtype, a)) {
+    const int sms = sm_count(stream_device(s));
+    NIE_REQUIRE(sms > 0, "cannot query the SM count");
+    NIE_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
+                    workspace_bytes >= kv8_decode_workspace(sms, num_requests, q_heads, head_dim),
+                "workspace too small or not 256-byte aligned");
+    return launch_kv8_decode(dtype, a, num_requests, sms, workspace, overlap != 0, s);
+  }
+  return launch_kv8_generic(dtype, a, num_requests, 1, s);
+}
+
+extern "C" size_t nie_paged_decode_kv8_workspace_size(int device, int32_t num_requests, int32_t q_heads,
+                                                      int32_t head_dim) {
+  const int sms = sm_count(device);
+  if (sms <= 0 || num_requests <= 0 || q_heads <= 0 || head_dim <= 0) return 0;
+  return kv8_decode_workspace(sms, num_requests, q_heads, head_dim);
 }
 
 extern "C" int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
@@ -155,16 +179,17 @@ extern "C" int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, voi
                                         const float* key_scales, const float* value_scales, int32_t dtype,
                                         int32_t layer, int64_t num_layers, int64_t num_blocks, int32_t block_size,
                                         int32_t kv_heads, int32_t head_dim, int32_t q_heads,
-                                        const int32_t* block_tables, int64_t table_stride, const int32_t* table_rows,
-                                        const int32_t* seq_lens, const int64_t* query_start_loc,
+                                        const int32_t* block_tables, int64_t table_stride, int64_t num_table_rows,
+                                        const int32_t* table_rows, const int32_t* seq_lens, int32_t num_seqs,
+                                        const int64_t* query_start_loc,
                                         const int32_t* req_list, int32_t num_requests, int32_t max_query_len,
                                         float scale, int32_t* err_flag, void* stream) {
   Kv8Args a{};
   a.q = q, a.out = out, a.q_stride = q_row_stride, a.out_stride = out_row_stride, a.num_q_rows = num_q_rows;
   a.kc = (const uint8_t*)key_cache, a.vc = (const uint8_t*)value_cache, a.ks = key_scales, a.vs = value_scales;
   a.nb = num_blocks, a.bs = block_size, a.hkv = kv_heads, a.hd = head_dim, a.hq = q_heads;
-  a.tables = block_tables, a.tstride = table_stride, a.table_rows = table_rows;
-  a.seq_lens = seq_lens, a.qsl = query_start_loc, a.req_list = req_list;
+  a.tables = block_tables, a.tstride = table_stride, a.num_table_rows = num_table_rows, a.table_rows = table_rows;
+  a.seq_lens = seq_lens, a.num_seqs = num_seqs, a.qsl = query_start_loc, a.req_list = req_list;
   a.scale = scale, a.err = err_flag;
   const int rc = check_args(a, dtype, layer, num_layers, num_requests);
   if (rc != NIE_OK) return rc;

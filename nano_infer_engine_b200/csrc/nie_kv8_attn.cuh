@@ -10,6 +10,8 @@ struct Kv8Args {
   void* out;
   int64_t q_stride, out_stride;  // elements between token rows
   int64_t num_q_rows;            // rows of q and out
+  int64_t num_table_rows;        // rows of tables
+  int num_seqs;                  // entries of seq_lens, q_rows and table_rows
   const uint8_t* kc;             // codes and scales of the layer
   const uint8_t* vc;
   const float* ks;
@@ -52,5 +54,12 @@ __device__ __forceinline__ Kv8Rows kv8_rows(const Kv8Args& a, int r) {
   }
   return x;
 }
+
+// The kernel of single tokens (nie_kv8_decode.cu), where kv8_decode_takes() says
+// so; workspace of kv8_decode_workspace() bytes, 256-byte aligned.
+bool kv8_decode_takes(int dtype, const Kv8Args& a);
+size_t kv8_decode_workspace(int sms, int num_requests, int q_heads, int head_dim);
+int launch_kv8_decode(int dtype, const Kv8Args& a, int num_requests, int sms, void* workspace, bool overlap,
+                      cudaStream_t s);
 
 }  // namespace nie

@@ -1179,10 +1179,12 @@ def paged_decode_kv8(
     req_list: torch.Tensor | None = None,
     num_requests: int | None = None,
     scale: float | None = None,
+    overlap: bool = False,
 ) -> torch.Tensor:
     """:func:`paged_decode` over an 8-bit cache: fp32 scores, softmax and sums, the output rounded once.
 
     A request of length 0 gives zeros; rows of ``out`` that no request has are left as they were.
+    ``overlap``: as in :func:`paged_decode`.
     """
     L, nb, bs, h, d = _kv8_geometry(key_cache, value_cache, key_scales, value_scales, layer)
     R = _check_kv8_query(query, out, h, d, block_tables, seq_lens, table_rows, req_list, num_requests)
@@ -1198,6 +1200,9 @@ def paged_decode_kv8(
         out = torch.empty(query.shape, dtype=query.dtype, device=device)
     if R == 0:
         return out
+    # of this call alone: calls on other streams and captured graphs have their own
+    need = lib.nie_paged_decode_kv8_workspace_size(device.index, R, query.shape[1], d)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
     with _on(device):
         status = lib.nie_paged_decode_kv8(
             query.data_ptr(),
@@ -1219,17 +1224,22 @@ def paged_decode_kv8(
             query.shape[1],
             block_tables.data_ptr(),
             block_tables.stride(0),
+            block_tables.shape[0],
             _ptr(table_rows),
             seq_lens.data_ptr(),
+            seq_lens.numel(),
             _ptr(q_rows),
             _ptr(req_list),
             R,
             float(d**-0.5 if scale is None else scale),
+            ws.data_ptr(),
+            need,
+            int(overlap),
             error_flag(device).data_ptr(),
             _stream(device),
         )
     check(status, "nie_paged_decode_kv8")
-    _count()
+    _count(kv8_decode_launch_count(query.dtype, bs, d, R))
     return out
 
 
@@ -1293,8 +1303,10 @@ def varlen_attention_kv8(
             query.shape[1],
             block_tables.data_ptr(),
             block_tables.stride(0),
+            block_tables.shape[0],
             _ptr(table_rows),
             seq_lens.data_ptr(),
+            seq_lens.numel(),
             query_start_loc.data_ptr(),
             _ptr(req_list),
             R,
@@ -1335,3 +1347,9 @@ def decode_launch_count(dtype: torch.dtype, block_size: int, kv_heads: int, head
     """Kernels one :func:`paged_decode` call launches (split-K kernel + combine, or the generic one)."""
     fast = dtype == torch.bfloat16 and head_dim == 64 and block_size == 16 and q_heads // kv_heads <= 16 and kv_heads <= 16
     return 2 if fast else 1
+
+
+def kv8_decode_launch_count(dtype: torch.dtype, block_size: int, head_dim: int, num_requests: int) -> int:
+    """Kernels one :func:`paged_decode_kv8` call launches (two per 512 requests, or the generic one)."""
+    fast = dtype != torch.float32 and head_dim in (64, 128) and block_size % 16 == 0
+    return 2 * -(-num_requests // 512) if fast else 1
