@@ -473,13 +473,14 @@ int nie_gather_kv8(const void* key_cache, const void* value_cache,
  * is outside the pool raises NIE_DEV_ERR_BLOCK_RANGE.  seq_lens, table_rows and
  * q_rows have num_seqs entries, block_tables num_table_rows rows; a request of
  * req_list or a row of table_rows outside them is flagged and skipped likewise.
- * head_dim <= 256.  The decode workspace (nie_paged_decode_kv8_workspace_size
- * bytes, 256-byte aligned) holds partial sums of one call; calls that share it
- * must not overlap on the GPU.  overlap != 0: the kernel may start before the
+ * head_dim <= 256.  The workspace (nie_paged_decode_kv8_workspace_size,
+ * nie_varlen_kv8_workspace_size bytes, 256-byte aligned) holds partial sums of
+ * one call; calls that share it must not overlap on the GPU.  overlap != 0: the kernel may start before the
  * previous kernel on the stream ends, as nie_paged_decode_overlapped, with its
  * precondition. */
 size_t nie_paged_decode_kv8_workspace_size(int device, int32_t num_requests,
                                            int32_t q_heads, int32_t head_dim);
+size_t nie_varlen_kv8_workspace_size(int device, int32_t head_dim);
 
 int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* out,
                          int64_t out_row_stride, int64_t num_q_rows,
@@ -509,6 +510,7 @@ int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, void* out,
                              int32_t num_seqs, const int64_t* query_start_loc,
                              const int32_t* req_list, int32_t num_requests,
                              int32_t max_query_len, float scale,
+                             void* workspace, size_t workspace_bytes,
                              int32_t* err_flag, void* stream);
 
 /*

@@ -29,6 +29,7 @@ SOURCES = (
     "nie_kv8.cu",
     "nie_kv8_attn.cu",
     "nie_kv8_decode.cu",
+    "nie_kv8_prefill.cu",
     "nie_logprobs.cu",
 )
 

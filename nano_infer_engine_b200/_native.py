@@ -131,8 +131,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32]
         + [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32]
-        + [c_void_p, c_void_p, c_int32, c_int32, c_float, c_void_p, c_void_p],
+        + [c_void_p, c_void_p, c_int32, c_int32, c_float, c_void_p, c_size_t, c_void_p, c_void_p],
     ),
+    "nie_varlen_kv8_workspace_size": (c_size_t, [c_int, c_int32]),
     "nie_token_logprobs": (
         c_int,
         [c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]

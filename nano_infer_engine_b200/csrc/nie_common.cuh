@@ -30,7 +30,8 @@ enum SmemSlot {
   kSmemLinear = 3,
   kSmemLinear64 = 4,
   kSmemKv8Decode = 5,   // 8 instances
-  kSmemSlots = 13
+  kSmemKv8Prefill = 13,  // 4 instances
+  kSmemSlots = 17
 };
 int opt_in_smem(int slot, const void* kernel, size_t bytes);
 

@@ -183,7 +183,8 @@ extern "C" int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, voi
                                         const int32_t* table_rows, const int32_t* seq_lens, int32_t num_seqs,
                                         const int64_t* query_start_loc,
                                         const int32_t* req_list, int32_t num_requests, int32_t max_query_len,
-                                        float scale, int32_t* err_flag, void* stream) {
+                                        float scale, void* workspace, size_t workspace_bytes, int32_t* err_flag,
+                                        void* stream) {
   Kv8Args a{};
   a.q = q, a.out = out, a.q_stride = q_row_stride, a.out_stride = out_row_stride, a.num_q_rows = num_q_rows;
   a.kc = (const uint8_t*)key_cache, a.vc = (const uint8_t*)value_cache, a.ks = key_scales, a.vs = value_scales;
@@ -196,5 +197,19 @@ extern "C" int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, voi
   NIE_REQUIRE(query_start_loc, "null pointer argument");
   if (num_requests == 0) return NIE_OK;
   to_layer(a, layer);
-  return launch_kv8_generic(dtype, a, num_requests, max_query_len, reinterpret_cast<cudaStream_t>(stream));
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  if (kv8_prefill_takes(dtype, a)) {
+    const int sms = sm_count(stream_device(s));
+    NIE_REQUIRE(sms > 0, "cannot query the SM count");
+    NIE_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
+                    workspace_bytes >= kv8_prefill_workspace(sms, head_dim),
+                "workspace too small or not 256-byte aligned");
+    return launch_kv8_prefill(dtype, a, num_requests, sms, workspace, s);
+  }
+  return launch_kv8_generic(dtype, a, num_requests, max_query_len, s);
+}
+
+extern "C" size_t nie_varlen_kv8_workspace_size(int device, int32_t head_dim) {
+  const int sms = sm_count(device);
+  return sms <= 0 || head_dim <= 0 ? 0 : kv8_prefill_workspace(sms, head_dim);
 }

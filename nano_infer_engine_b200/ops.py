@@ -1239,7 +1239,7 @@ def paged_decode_kv8(
             _stream(device),
         )
     check(status, "nie_paged_decode_kv8")
-    _count(kv8_decode_launch_count(query.dtype, bs, d, R))
+    _count(kv8_launch_count(query.dtype, bs, d, R))
     return out
 
 
@@ -1282,6 +1282,9 @@ def varlen_attention_kv8(
         out = torch.empty(query.shape, dtype=query.dtype, device=device)
     if R == 0:
         return out
+    # of this call alone: calls on other streams and captured graphs have their own
+    need = lib.nie_varlen_kv8_workspace_size(device.index, d)
+    ws = torch.empty(need, dtype=torch.uint8, device=device)
     with _on(device):
         status = lib.nie_varlen_attention_kv8(
             query.data_ptr(),
@@ -1312,11 +1315,13 @@ def varlen_attention_kv8(
             R,
             int(max_query_len),
             float(d**-0.5 if scale is None else scale),
+            ws.data_ptr(),
+            need,
             error_flag(device).data_ptr(),
             _stream(device),
         )
     check(status, "nie_varlen_attention_kv8")
-    _count()
+    _count(kv8_launch_count(query.dtype, bs, d, R))
     return out
 
 
@@ -1349,7 +1354,7 @@ def decode_launch_count(dtype: torch.dtype, block_size: int, kv_heads: int, head
     return 2 if fast else 1
 
 
-def kv8_decode_launch_count(dtype: torch.dtype, block_size: int, head_dim: int, num_requests: int) -> int:
-    """Kernels one :func:`paged_decode_kv8` call launches (two per 512 requests, or the generic one)."""
+def kv8_launch_count(dtype: torch.dtype, block_size: int, head_dim: int, num_requests: int) -> int:
+    """Kernels one :func:`paged_decode_kv8` or :func:`varlen_attention_kv8` call launches (two per 512 requests, or the generic one)."""
     fast = dtype != torch.float32 and head_dim in (64, 128) and block_size % 16 == 0
     return 2 * -(-num_requests // 512) if fast else 1
