@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(kG8Warps * 32) kv8_generic_kernel(Kv8Args a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int32_t* table = a.tables + (int64_t)trow * a.tstride;
   const int64_t row_elems = (int64_t)a.hkv * a.hd;
-  const Kv8Rows rows = kv8_rows(a, r);
+  const Kv8Rows rows = kv8_rows(a, r, a.err);
   __shared__ float sm_m[kG8Warps], sm_l[kG8Warps], sm_o[kG8Warps][kG8MaxHd];
 
   for (int64_t j = blockIdx.y; j < rows.count; j += gridDim.y) {

@@ -37,7 +37,7 @@ struct Kv8Rows {
 };
 
 // Rows outside [0, num_q_rows) do not exist: the request is flagged and has none.
-__device__ __forceinline__ Kv8Rows kv8_rows(const Kv8Args& a, int r) {
+__device__ __forceinline__ Kv8Rows kv8_rows(const Kv8Args& a, int r, int32_t* err) {
   Kv8Rows x;
   const int64_t n = a.seq_lens[r];
   if (a.qsl) {
@@ -49,7 +49,7 @@ __device__ __forceinline__ Kv8Rows kv8_rows(const Kv8Args& a, int r) {
   }
   x.keys = n - x.count;
   if (x.count > 0 && (x.first < 0 || x.first + x.count > a.num_q_rows)) {
-    raise_flag(a.err, NIE_DEV_ERR_CAPACITY);
+    raise_flag(err, NIE_DEV_ERR_CAPACITY);
     x.count = 0;
   }
   return x;

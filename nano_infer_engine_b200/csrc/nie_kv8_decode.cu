@@ -99,7 +99,8 @@ __device__ __forceinline__ int row_token(int i) { return (i & 8) + ((i & 7) >> 1
 __device__ __forceinline__ float merge_weight(float m, float M) { return m == -INFINITY ? 0.f : fast_exp2(m - M); }
 
 template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) kv8_decode_kernel(const Kv8Args a, const D8Plan p) {
+__global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) kv8_decode_kernel(const __grid_constant__ Kv8Args a,
+                                                                           const __grid_constant__ D8Plan p) {
   constexpr int TOK = 2048 / HD, SUBS = TOK / 16, CPR = HD / 16;  // tokens, sub-blocks, 16-byte chunks per row
   constexpr int ITEMS = 32 / SUBS;                                // tiles whose rows a warp looks up at once
   constexpr int MS = HD + 4;                                      // floats between rows of the merge buffer
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
     int n = 0, tr = 0, qr = -1;
     if (r >= 0 && r < a.num_seqs) {
       tr = a.table_rows ? a.table_rows[r] : r;
-      const Kv8Rows rows = kv8_rows(a, r);
+      const Kv8Rows rows = kv8_rows(a, r, a.err);
       if (rows.count > 0 && tr >= 0 && tr < a.num_table_rows) {
         n = max(a.seq_lens[r], 0);
         qr = (int)rows.first;
@@ -485,7 +486,8 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
 // (request, query head); sixteenths of it take every sixteenth partial, all of
 // a thread's loads go out together.  Requests without keys get zeros.
 template <int HD, typename T>
-__global__ void __launch_bounds__(HD * 4) kv8_decode_merge_kernel(const Kv8Args a, const D8Plan p) {
+__global__ void __launch_bounds__(HD * 4) kv8_decode_merge_kernel(const __grid_constant__ Kv8Args a,
+                                                                           const __grid_constant__ D8Plan p) {
   constexpr int GROUPS = 16, LANES = HD / 4;
   __shared__ float4 so[GROUPS][LANES];
   __shared__ float sm_m[GROUPS], sm_l[GROUPS];

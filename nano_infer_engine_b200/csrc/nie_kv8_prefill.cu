@@ -17,22 +17,22 @@
 // a border leaves (max, sum, unnormalised output) of each part for a merging
 // kernel; which parts and in which order follows from the lengths alone.
 //
-// Roles (13 warps, all walking the same segments and key tiles):
-//   warps 0-3, 4-7  softmax of tile A, B: a thread owns a row
-//   warps 8-11      loaders: q to f16 (bf16 rows scaled by a power of two so that
-//                   8 bits fit f16's 11 whatever the row's size), codes to f16
-//                   (exact), into 128-byte swizzled shared memory; codes come
-//                   two tiles ahead by cp.async into a thread's own bytes
-//   warp 12         issues S = Q K^T, then O += P V (P from TMEM), A and B in turn:
-//                   one tile's MMAs run under the other's softmax
+// Roles (16 warps):
+//   warps 0-3, 4-7  softmax of half A, B: a thread owns a row.  It takes the row's
+//                   scores of a tile into registers at once, so that the next
+//                   tile's S runs under this tile's exponentials
+//   warps 8-11      codes to 16 bits (exact: K in the queries' type, V in f16) into
+//                   128-byte swizzled shared memory; they come two tiles ahead by cp.async into a thread's own bytes
+//   warp 12         one thread issues S = Q K^T and O += P V (P from TMEM)
+//   warps 13-15     queries to shared memory, a segment ahead where it has room for two
 //
 // Softmax with scales as in the single-token kernel: y = S c + log2 vs per block
 // of 16 keys, p = 2^(y - m) in f16 for the product (its error of 2^-12 is below
 // the output's step), O = sum p vcode, l = sum p / vs from the unrounded p.  m
 // is raised (and O and l rescaled) only when exceeded by more than 2^8.
 //
-// TMEM columns: S of A 0-127, of B 128-255 (P takes its place), O of A from 256,
-// of B from 384.  Waits are bounded; one that runs out raises
+// TMEM columns: head_dim 64: S 0-255, O 256-383, P 384-511; head_dim 128: S 0-127,
+// P 128-191, O 256-511 (A's part first).  Waits are bounded; one that runs out raises
 // NIE_DEV_ERR_TIMEOUT and ends the CTA.
 #include <algorithm>
 #include <type_traits>
@@ -42,14 +42,16 @@
 namespace nie {
 
 constexpr int kF8Rows = 256;
-constexpr int kF8Threads = 13 * 32;
+constexpr int kF8Threads = 16 * 32;
+// Registers per thread after the split: 256 softmax threads, 256 others; together what 512 threads have at launch.
+constexpr int kF8SoftmaxRegs = 184, kF8OtherRegs = 72;
+static_assert(256 * (kF8SoftmaxRegs + kF8OtherRegs) <= 65536, "more registers than the launch has");
 constexpr int kF8Stages = 3;       // f16 key tiles in shared memory
 constexpr int kF8MaxReq = 512;     // requests of one launch
 constexpr int kF8SegCost = 2;      // a segment's fixed part, in key tiles
 constexpr uint32_t kF8Wait = 1u << 22;
 constexpr float kF8Log2e = 1.4426950408889634f;
 constexpr float kF8Lazy = 8.f;
-constexpr uint32_t kF8OCol = 256;
 
 // What the merging kernel needs about the segment that begins in a CTA's
 // stretch and goes on behind it (parts: CTAs after it that hold some of it).
@@ -74,18 +76,23 @@ struct F8Cfg {
   static constexpr int StageBytes = 2 * TileBytes;
   static constexpr int CodeBytes = 2 * BN * HD;           // codes of a tile
   static constexpr int Subs = BN / 16;
+  // TMEM columns; a half's S, O and P are BN, HD and BN / 2 wide
+  static constexpr uint32_t SCol = 0, OCol = 256, PCol = HD == 64 ? 384 : 128;
 };
+
+// A key tile of a segment: its first in this CTA, its last, with rows in half B; the end of the stretch.
+enum F8Flag { kF8First = 1, kF8Last = 2, kF8Two = 4, kF8End = 8 };
 
 struct F8Bars {
   uint64_t q_full[2], q_empty[2];
   uint64_t kv_full[kF8Stages], kv_empty[kF8Stages];
-  uint64_t s_full[2], p_full[2], o_full[2], o_free[2];
+  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];
   uint64_t done;
   uint32_t tmem_base;
   int abort;
   int start_req, start_tile, start_head;
   int64_t start_pos;
-  float q_undo[2][kF8Rows];              // what undoes a row's scaling
+  int flags[kF8Stages];                  // of a stage's tile: kF8First, ...
   float4 info[kF8Stages][8];             // of 16 keys: score factor, log2 vs, 1 / vs
   int64_t cum[kF8MaxReq + 1];            // cost before each request
 };
@@ -98,6 +105,25 @@ __device__ __forceinline__ bool f8_wait(F8Bars* b, uint64_t* bar, uint32_t parit
   *reinterpret_cast<volatile int*>(&b->abort) = 1;
   raise_flag(err, NIE_DEV_ERR_TIMEOUT);
   return false;
+}
+
+// The same for warps that run ahead: they sleep between probes, since every probe
+// goes through the queue that the exponentials of the softmax warps use.
+__device__ __forceinline__ bool f8_wait_idle(F8Bars* b, uint64_t* bar, uint32_t parity, int32_t* err) {
+  for (uint32_t i = 0; i < kF8Wait; ++i) {
+    if (mbar_try_wait(bar, parity)) return true;
+    __nanosleep(100);
+    if ((i & 1023u) == 1023u && *reinterpret_cast<volatile int*>(&b->abort)) return false;
+  }
+  *reinterpret_cast<volatile int*>(&b->abort) = 1;
+  raise_flag(err, NIE_DEV_ERR_TIMEOUT);
+  return false;
+}
+
+__device__ __forceinline__ float f8_max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
 }
 
 __device__ __forceinline__ void f8_fma2(float& d0, float& d1, float a0, float a1, float b, float c) {
@@ -120,85 +146,78 @@ __device__ __forceinline__ void f8_cp16(uint32_t dst, const void* src, int bytes
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// kind::f16 with f16 A and B, f32 D.
-constexpr uint32_t f8_idesc(int m, int n, bool b_mn_major) {
-  return (1u << 4) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+// kind::f16 with f16 (or bf16) A and B, f32 D.
+constexpr uint32_t f8_idesc(int m, int n, bool b_mn_major, bool bf16) {
+  return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
 }
 
 // A request of the call; none of its fields depend on the kv head.
 struct F8Req {
-  int64_t first;  // first query row
-  int64_t rows;   // query tokens * heads of a group
-  int64_t ctx;    // keys before its first token (negative: the first tokens see none)
-  int n;          // keys
+  int first;  // first query row
+  int rows;   // query tokens * heads of a group
+  int ctx;    // keys before its first token (negative: the first tokens see none)
+  int n;      // keys
   int trow;
-  int tiles;      // 256-row tiles
+  int tiles;  // 256-row tiles
 };
 
-__device__ __forceinline__ F8Req f8_request(const Kv8Args& a, int i, bool flag) {
+__device__ __forceinline__ F8Req f8_request(const Kv8Args& a, int i, int32_t* err) {
   F8Req x{};
   const int r = a.req_list ? a.req_list[i] : i;
   const int tr = r < 0 || r >= a.num_seqs ? -1 : a.table_rows ? a.table_rows[r] : r;
   if (tr < 0 || tr >= a.num_table_rows) {
-    if (flag) raise_flag(a.err, NIE_DEV_ERR_CAPACITY);
+    raise_flag(err, NIE_DEV_ERR_CAPACITY);
     return x;
   }
-  Kv8Args q = a;
-  if (!flag) q.err = nullptr;
-  const Kv8Rows rows = kv8_rows(q, r);
+  const Kv8Rows rows = kv8_rows(a, r, err);
   if (rows.count <= 0) return x;
-  x.first = rows.first;
-  x.rows = rows.count * a.group;
-  x.ctx = rows.keys;
+  x.first = (int)rows.first;
+  x.rows = (int)rows.count * a.group;
+  x.ctx = (int)rows.keys;
   x.n = max(a.seq_lens[r], 0);
   x.trow = tr;
-  x.tiles = (int)((x.rows + kF8Rows - 1) / kF8Rows);
+  x.tiles = (x.rows + kF8Rows - 1) / kF8Rows;
   return x;
 }
 
 // Keys that the last token of a tile sees, and the tiles of BN keys they fill (at
 // least one: rows that see no key still get their zeros from a masked tile).
 __device__ __forceinline__ int f8_keys(const F8Req& x, int group, int tile) {
-  const int64_t last = (min(x.rows, (int64_t)(tile + 1) * kF8Rows) - 1) / group;
-  return (int)max((int64_t)0, x.ctx + last + 1);
+  return max(0, x.ctx + (min(x.rows, (tile + 1) * kF8Rows) - 1) / group + 1);
 }
 template <int BN>
 __device__ __forceinline__ int f8_key_tiles(int keys) {
   return max(1, (keys + BN - 1) / BN);
 }
 
-// Walks the segments of a CTA's stretch [lo, hi): requests, tiles, kv heads.
+// Walks the segments of a CTA's stretch: requests, tiles, kv heads.  Positions
+// are costs from the stretch's beginning; it ends at `hi`.
 template <int BN>
 struct F8Walk {
-  const Kv8Args* a;
-  int num_req;
-  int64_t lo, hi, start;  // start: cost position of the segment's first key tile
+  int hi, start;  // start: position of the segment's first key tile (may be negative)
   int i, tile, h, keys, n;
   F8Req x;
 
-  __device__ void load() {
-    keys = f8_keys(x, a->group, tile);
+  __device__ __forceinline__ void load(const Kv8Args& a) {
+    keys = f8_keys(x, a.group, tile);
     n = f8_key_tiles<BN>(keys);
   }
-  __device__ void init(const Kv8Args* args, int R, const F8Bars* b, int64_t l, int64_t h_) {
-    a = args;
-    num_req = R;
-    lo = l;
-    hi = h_;
+  __device__ __forceinline__ void init(const Kv8Args& a, const F8Bars* b, int64_t lo, int64_t end) {
+    hi = (int)(end - lo);
     i = b->start_req;
     tile = b->start_tile;
     h = b->start_head;
-    x = f8_request(*a, i, false);
-    load();
-    start = b->start_pos + kF8SegCost;
+    x = f8_request(a, i, nullptr);
+    load(a);
+    start = (int)(b->start_pos - lo) + kF8SegCost;
   }
-  __device__ bool valid() const { return start < hi; }
-  __device__ int t_lo() const { return (int)(max(lo, start) - start); }
-  __device__ int t_hi() const { return (int)(min(hi, start + n) - start); }
-  __device__ int rows() const { return (int)min((int64_t)kF8Rows, x.rows - (int64_t)tile * kF8Rows); }
-  __device__ void next() {
+  __device__ __forceinline__ bool valid() const { return start < hi; }
+  __device__ __forceinline__ int t_lo() const { return max(0, -start); }
+  __device__ __forceinline__ int t_hi() const { return min(hi - start, n); }
+  __device__ __forceinline__ int rows() const { return min(kF8Rows, x.rows - tile * kF8Rows); }
+  __device__ __forceinline__ void next(const Kv8Args& a, int num_req) {
     start += n;
-    if (++h == a->hkv) {
+    if (++h == a.hkv) {
       h = 0;
       if (++tile >= x.tiles) {
         tile = 0;
@@ -207,17 +226,50 @@ struct F8Walk {
             start = hi;
             return;
           }
-          x = f8_request(*a, i, false);
+          x = f8_request(a, i, nullptr);
         } while (x.tiles == 0);
       }
-      load();
+      load(a);
     }
     start += kF8SegCost;
   }
 };
 
+// D[tmem] (+)= A[smem] * B[smem] and A[tmem] * B[smem], kind::f16.
+__device__ __forceinline__ void f8_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
+      "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void f8_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a),
+      "l"(b), "r"(idesc), "r"((uint32_t)add)
+      : "memory");
+}
+
+// 32 lanes x 16 consecutive 32-bit columns.
+__device__ __forceinline__ void f8_tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
+
+template <int REGS>
+__device__ __forceinline__ void f8_more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+template <int REGS>
+__device__ __forceinline__ void f8_fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
+}
+
 template <int HD, typename T>
-__global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const Kv8Args a, const F8Plan p) {
+__global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid_constant__ Kv8Args a,
+                                                                    const __grid_constant__ F8Plan p) {
   using C = F8Cfg<HD>;
   constexpr int BN = C::BN;
   extern __shared__ uint8_t f8_raw[];
@@ -233,7 +285,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const Kv8Arg
   pdl_trigger();
   // ---- cost of each request (a warp each), then of all before it
   for (int i = warp; i < R; i += kF8Threads / 32) {
-    const F8Req x = f8_request(a, i, blockIdx.x == 0 && lane == 0);
+    const F8Req x = f8_request(a, i, blockIdx.x == 0 && lane == 0 ? a.err : nullptr);
     int64_t cost = 0;
     for (int tile = lane; tile < x.tiles; tile += 32) cost += f8_key_tiles<BN>(f8_keys(x, a.group, tile)) + kF8SegCost;
 #pragma unroll
@@ -243,12 +295,13 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const Kv8Arg
   if (threadIdx.x == 0) {
     b->cum[0] = 0;
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&b->q_full[i], 128);
-      mbar_init(&b->q_empty[i], 1 + 8);
+      mbar_init(&b->q_full[i], 96);
+      mbar_init(&b->q_empty[i], 1);
       mbar_init(&b->s_full[i], 1);
-      mbar_init(&b->p_full[i], 128);
-      mbar_init(&b->o_full[i], 1);
-      mbar_init(&b->o_free[i], 128);
+      mbar_init(&b->s_free[i], 4);
+      mbar_init(&b->p_full[i], 4);
+      mbar_init(&b->pv_done[i], 1);
+      mbar_init(&b->o_free[i], 4);
     }
     for (int s = 0; s < kF8Stages; ++s) {
       mbar_init(&b->kv_full[s], 128);
@@ -287,7 +340,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const Kv8Arg
       const int mid = (l + r) >> 1;
       if (b->cum[mid] <= lo) l = mid; else r = mid;
     }
-    const F8Req x = f8_request(a, l, false);
+    const F8Req x = f8_request(a, l, nullptr);
     int64_t pos = b->cum[l];
     for (int t0 = 0; t0 < x.tiles; t0 += 32) {
       const int64_t c = t0 + lane < x.tiles ? f8_key_tiles<BN>(f8_keys(x, a.group, t0 + lane)) + kF8SegCost : 0;
@@ -317,132 +370,78 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const Kv8Arg
   tc_fence_after();
   const uint32_t tbase = b->tmem_base;
   F8Walk<BN> seg;
-  seg.init(&a, R, b, lo, hi);
+  seg.init(a, b, lo, hi);
 
   if (warp >= 8 && warp < 12) {
+    f8_fewer_registers<kF8OtherRegs>();
     // ------------------------------------------------------------ loaders
     const int tid = threadIdx.x - 256;
     const int64_t row_bytes = (int64_t)a.hkv * HD;
     const float coef = fabsf(a.scale) * kF8Log2e;
-    const bool negate = a.scale < 0.f;
+    const uint32_t flip = a.scale < 0.f ? 0x80808080u : 0u;  // a negative scale's sign goes to the keys
     // tiles come two ahead: `ahead` walks in front of `seg`
     F8Walk<BN> ahead = seg;
     int a_kt = ahead.valid() ? ahead.t_lo() : 0;
-    while (ahead.valid() && a_kt >= ahead.t_hi()) {
-      ahead.next();
-      a_kt = ahead.valid() ? ahead.t_lo() : 0;
-    }
-    float pend_ks[2] = {0.f, 0.f}, pend_vs[2] = {1.f, 1.f};
-    bool pend_ok[2] = {false, false};
-    auto block_of = [&](const F8Walk<BN>& w, int key) -> int64_t {
-      if (key >= w.keys || key >= w.x.n) return -1;
-      const int lb = key / a.bs;
-      const int64_t block = lb < a.tstride ? (int64_t)a.tables[(int64_t)w.x.trow * a.tstride + lb] : -1;
-      if (block < 0 || block >= a.nb) {
-        raise_flag(a.err, NIE_DEV_ERR_BLOCK_RANGE);
-        return -1;
-      }
-      return block;
-    };
-    auto fetch = [&](int slot) {
+    // Lane s of each warp looks up the block of the tile's s-th 16 keys, a tile
+    // before its codes are fetched; all rows of a warp's copy j lie in 16 keys.
+    int entry = -1, offset = 0, count = 0;  // count: keys of the 16 that are there
+    auto look_up = [&]() {
+      count = 0;
       if (ahead.valid()) {
-        const int key0 = a_kt * BN;
+        const int key = a_kt * BN + 16 * lane;
+        if (lane < C::Subs) count = min(16, min(ahead.keys, ahead.x.n) - key);
+        const int lb = key / a.bs;
+        offset = key - lb * a.bs;
+        entry = count > 0 && lb < a.tstride ? a.tables[(int64_t)ahead.x.trow * a.tstride + lb] : -1;
+      }
+    };
+    // scales of the next tile and of the one after it (warp 8, lane s: the s-th 16 keys)
+    float ks0 = 0.f, vs0 = 1.f, ks1 = 0.f, vs1 = 1.f;
+    bool ok0 = false, ok1 = false;
+    auto fetch = [&](int slot, float& p_ks, float& p_vs, bool& p_ok) {
+      if (ahead.valid()) {
         const uint32_t base = smem_u32(scode + slot * C::CodeBytes) + tid * 16;
-        int64_t block[BN / 32];
-#pragma unroll
-        for (int j = 0; j < BN / 32; ++j) block[j] = block_of(ahead, key0 + (tid >> 2) + 32 * j);
-        const int64_t sb = tid < C::Subs ? block_of(ahead, key0 + 16 * tid) : -1;
-        float ks = 0.f, vs = 1.f;
-        if (sb >= 0) {
-          ks = a.ks[sb * a.hkv + ahead.h];
-          vs = a.vs[sb * a.hkv + ahead.h];
+        const bool found = count > 0 && entry >= 0 && entry < a.nb;
+        if (count > 0 && !found) raise_flag(a.err, NIE_DEV_ERR_BLOCK_RANGE);
+        const int at = entry * a.bs + offset, here = found ? count : 0;
+        if (tid < C::Subs) {
+          p_ok = found;
+          if (found) {
+            p_ks = a.ks[(int64_t)entry * a.hkv + ahead.h];
+            p_vs = a.vs[(int64_t)entry * a.hkv + ahead.h];
+          }
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int row = (tid >> 2) + 32 * (j % (BN / 32)), half = j / (BN / 32);
-          const int64_t blk = block[j % (BN / 32)];
-          const int64_t off = blk < 0 ? 0
-                                      : (blk * a.bs + (key0 + row) % a.bs) * row_bytes + (int64_t)ahead.h * HD + half * 64 +
-                                            (tid & 3) * 16;
-          f8_cp16(base + j * 2048, a.kc + off, blk < 0 ? 0 : 16);
-          f8_cp16(base + (4 + j) * 2048, a.vc + off, blk < 0 ? 0 : 16);
+          const int half = j / (BN / 32);
+          const int s = 2 * (j % (BN / 32)) + (tid >> 6), row = (tid >> 2) & 15;
+          const int from = __shfl_sync(0xffffffffu, at, s);
+          const bool there = row < __shfl_sync(0xffffffffu, here, s);
+          const int64_t off =
+              there ? (int64_t)(from + row) * row_bytes + (int64_t)ahead.h * HD + half * 64 + (tid & 3) * 16 : 0;
+          f8_cp16(base + j * 2048, a.kc + off, there ? 16 : 0);
+          f8_cp16(base + (4 + j) * 2048, a.vc + off, there ? 16 : 0);
         }
-        pend_ks[slot] = fminf(fmaxf(ks, 0.f), kScaleMax);
-        pend_vs[slot] = fminf(fmaxf(vs, kScaleMin), kScaleMax);
-        pend_ok[slot] = sb >= 0;
         if (++a_kt >= ahead.t_hi()) {
-          do {
-            ahead.next();
-            a_kt = ahead.valid() ? ahead.t_lo() : 0;
-          } while (ahead.valid() && a_kt >= ahead.t_hi());
+          ahead.next(a, R);
+          a_kt = 0;
         }
+        look_up();
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    fetch(0);
-    fetch(1);
+    look_up();
+    fetch(0, ks0, vs0, ok0);
+    fetch(1, ks1, vs1, ok1);
     bool ok = true;
-    int64_t g = 0;
-    for (int k = 0; ok && seg.valid(); seg.next(), ++k) {
-      // the tile's queries
-      const int qb = k % C::QBufs;
-      if (k >= C::QBufs && !f8_wait(b, &b->q_empty[qb], (uint32_t)((k / C::QBufs) - 1) & 1u, a.err)) break;
-      constexpr int LPR = HD / 8;  // lanes of a row, 8 elements each
+    int st = 0, slot = 0;
+    uint32_t par = 1;  // parity of the stage's last release; the first round finds the stages free
+    for (; ok && seg.valid(); seg.next(a, R)) {
       const int rows = seg.rows();
-      const int c = tid % LPR;
-      uint8_t* qdst = sq + qb * C::QBytes;
-      for (int r0 = 0; r0 < kF8Rows; r0 += 4 * (128 / LPR)) {
-        uint4 raw[4];
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int row = r0 + u * (128 / LPR) + tid / LPR;
-          raw[u] = make_uint4(0u, 0u, 0u, 0u);
-          if (row < rows) {
-            const int64_t fr = (int64_t)seg.tile * kF8Rows + row;
-            raw[u] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (seg.x.first + fr / a.group) * a.q_stride +
-                                                     (int64_t)(seg.h * a.group + fr % a.group) * HD + c * 8);
-          }
-        }
-#pragma unroll
-        for (int u = 0; u < 4; ++u) {
-          const int row = r0 + u * (128 / LPR) + tid / LPR;
-          uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-          float undo = 1.f;
-          if constexpr (std::is_same<T, __half>::value) {
-            if (negate) {
-#pragma unroll
-              for (int e = 0; e < 4; ++e) w[e] ^= 0x80008000u;
-            }
-          } else {
-            float mx = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(w[e] << 16)), fabsf(__uint_as_float(w[e] & 0xffff0000u))));
-#pragma unroll
-            for (int o = 1; o < LPR; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            // largest element to [2^14, 2^15)
-            const int e2 = min(max((int)(__float_as_uint(mx) >> 23) - 127, -100), 127);
-            float up = __uint_as_float((uint32_t)(127 + 14 - e2) << 23);
-            undo = __uint_as_float((uint32_t)max(127 + e2 - 14, 1) << 23);
-            if (negate) up = -up;
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = f8_pack(__uint_as_float(w[e] << 16) * up, __uint_as_float(w[e] & 0xffff0000u) * up);
-          }
-          if (c == 0) b->q_undo[qb][row] = undo;
-          uint8_t* dst = qdst + (row >> 7) * (128 * HD * 2) + (c >> 3) * (128 * 128) + (row & 127) * 128 +
-                         (((c & 7) ^ (row & 7)) << 4);
-          *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-        }
-      }
-      fence_proxy_async_smem();
-      mbar_arrive(&b->q_full[qb]);
-      // its key tiles
       const int thi = seg.t_hi();
-      for (int kt = seg.t_lo(); kt < thi; ++kt, ++g) {
-        const int st = (int)(g % kF8Stages), slot = (int)(g & 1);
+      for (int kt = seg.t_lo(); kt < thi; ++kt) {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
-        if (g >= kF8Stages && !f8_wait(b, &b->kv_empty[st], (uint32_t)((g / kF8Stages) - 1) & 1u, a.err)) {
+        if (!f8_wait_idle(b, &b->kv_empty[st], par, a.err)) {
           ok = false;
           break;
         }
@@ -453,12 +452,19 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const Kv8Arg
           const int jj = j & 3;
           const int row = (tid >> 2) + 32 * (jj % (BN / 32)), half = jj / (BN / 32);
           const uint4 x = *reinterpret_cast<const uint4*>(src + j * 2048);
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-          uint32_t h[8];
+          uint32_t w[4] = {x.x, x.y, x.z, x.w}, h[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
+            if (j < 4) w[e] ^= flip;
             h[2 * e] = e4m3x2_to_f16x2((uint16_t)(w[e] & 0xffffu));
             h[2 * e + 1] = e4m3x2_to_f16x2((uint16_t)(w[e] >> 16));
+          }
+          if (j < 4 && !std::is_same<T, __half>::value) {  // keys meet bf16 queries: 4 bits fit either type
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              const float2 f = f16x2_to_float2(h[e]);
+              h[e] = pack_bf16x2(f.x, f.y);
+            }
           }
           uint8_t* at = dst + (j >> 2) * C::TileBytes + half * (BN * 128) + row * 128;
           const int ch = 2 * (tid & 3);
@@ -466,243 +472,292 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const Kv8Arg
           *reinterpret_cast<uint4*>(at + (((ch + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
         }
         if (tid < C::Subs)  // keys without a block have no weight
-          b->info[st][tid] = pend_ok[slot] ? make_float4(pend_ks[slot] * coef, __log2f(pend_vs[slot]), 1.f / pend_vs[slot], 0.f)
-                                           : make_float4(0.f, -INFINITY, 0.f, 0.f);
+          {
+          const float vs = fminf(fmaxf(vs0, kScaleMin), kScaleMax);
+          b->info[st][tid] = ok0 ? make_float4(fminf(fmaxf(ks0, 0.f), kScaleMax) * coef, __log2f(vs), 1.f / vs, 0.f)
+                                 : make_float4(0.f, -INFINITY, 0.f, 0.f);
+        }
+        if (tid == 0)
+          b->flags[st] = (kt == seg.t_lo() ? kF8First : 0) | (kt + 1 == thi ? kF8Last : 0) | (rows > 128 ? kF8Two : 0);
         fence_proxy_async_smem();
         mbar_arrive(&b->kv_full[st]);
-        fetch(slot);
+        ks0 = ks1, vs0 = vs1, ok0 = ok1;
+        fetch(slot, ks1, vs1, ok1);
+        slot ^= 1;
+        if (++st == kF8Stages) {
+          st = 0;
+          par ^= 1u;
+        }
+      }
+    }
+    {  // the end, in place of a tile
+      if (ok && f8_wait_idle(b, &b->kv_empty[st], par, a.err)) {
+        if (tid == 0) b->flags[st] = kF8End;
+        mbar_arrive(&b->kv_full[st]);
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == 12) {
+  } else if (warp >= 12) {
+    f8_fewer_registers<kF8OtherRegs>();
     // --------------------------------------------------------- MMA issuer
-    constexpr uint32_t id_s = f8_idesc(128, BN, false), id_o = f8_idesc(128, HD, true);
-    // `nx` is the key tile whose scores are issued next, `cur` the one before it, whose P V follow
-    struct Item {
-      bool live = false, first = false, last = false, two = false;
-      int k = 0, st = 0;
-    } cur, nx;
-    int k = 0, kt = 0;
-    int64_t g = 0;
-    bool fresh = true;
-    int used[2] = {0, 0};       // scores issued per tile half
-    int segs[2] = {0, 0};       // segments that wrote the half's output
-    auto advance = [&]() {      // the next key tile of the stretch into nx
-      nx.live = false;
-      while (seg.valid()) {
-        if (fresh) {
-          kt = seg.t_lo();
-          fresh = false;
+    // One thread.  What it has to know of a key tile stands beside the tile.
+    if (warp == 12 && lane == 0) {
+      const uint64_t q_desc = smem_desc_sw128(smem_u32(sq), 16, 1024), k_desc = smem_desc_sw128(smem_u32(skv), 16, 1024);
+      const uint64_t v_desc = smem_desc_sw128(smem_u32(skv + C::TileBytes), BN * 128, 1024);
+      constexpr uint32_t id_s = f8_idesc(128, BN, false, !std::is_same<T, __half>::value);
+      constexpr uint32_t id_o = f8_idesc(128, HD, true, false);
+      int nx = 0, cur = 0;          // flags of the tile whose scores come next, and of the one before it
+      int nx_st = 0, cur_st = 0;    // their stages
+      uint32_t kv_par = 0;          // phase parity of nx_st
+      int k = -1;                   // segment of nx
+      int issued[2] = {0, 0};       // scores and products of each half
+      int used[2] = {0, 0};
+      int segs[2] = {0, 0};         // segments that wrote its output
+      bool ok = true;
+      auto take = [&]() {  // the flags of the tile in stage nx_st
+        ok = f8_wait(b, &b->kv_full[nx_st], kv_par, a.err);
+        nx = ok ? *reinterpret_cast<volatile int*>(&b->flags[nx_st]) : kF8End;
+        if (ok && (nx & kF8First)) {
+          ++k;
+          ok = f8_wait(b, &b->q_full[k % C::QBufs], (uint32_t)(k / C::QBufs) & 1u, a.err);
         }
-        if (kt < seg.t_hi()) {
-          nx.live = true;
-          nx.first = kt == seg.t_lo();
-          nx.last = kt + 1 == seg.t_hi();
-          nx.two = seg.rows() > 128;
-          nx.k = k;
-          nx.st = (int)(g % kF8Stages);
-          ++kt;
-          return;
-        }
-        seg.next();
-        fresh = true;
-        ++k;
-      }
-    };
-    bool ok = true;
-    auto scores = [&](int x) -> bool {  // S of half x for nx
-      if (x == 0) {
-        if (nx.first && !f8_wait(b, &b->q_full[nx.k % C::QBufs], (uint32_t)(nx.k / C::QBufs) & 1u, a.err)) return false;
-        if (!f8_wait(b, &b->kv_full[nx.st], (uint32_t)(g / kF8Stages) & 1u, a.err)) return false;
-      }
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t q = smem_u32(sq + (nx.k % C::QBufs) * C::QBytes + x * (128 * HD * 2));
-        const uint32_t kk0 = smem_u32(skv + nx.st * C::StageBytes);
+        tc_fence_after();
+      };
+      auto scores = [&](auto half) {  // S of a half for nx
+        constexpr int x = decltype(half)::value;
+        // the softmax warps have taken the scores before these
+        if (issued[x] > 0) ok = f8_wait(b, &b->s_free[x], (uint32_t)(issued[x] - 1) & 1u, a.err);
+        if (!ok) return;
+        ++issued[x];
+        tc_fence_after();
+        // descriptors count addresses in 16 bytes: steps along a row or to the next 64 dims are added to them
+        const uint64_t q = q_desc + (uint32_t)((k % C::QBufs) * (C::QBytes / 16) + x * (128 * HD * 2 / 16));
+        const uint64_t kd = k_desc + (uint32_t)(nx_st * (C::StageBytes / 16));
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
-          tc_mma_ss(tbase + x * 128, smem_desc_sw128(q + (kk >> 2) * (128 * 128) + (kk & 3) * 32, 16, 1024),
-                    smem_desc_sw128(kk0 + (kk >> 2) * (BN * 128) + (kk & 3) * 32, 16, 1024), id_s, kk > 0 ? 1u : 0u);
+          f8_mma_ss(tbase + C::SCol + x * BN, q + ((kk >> 2) * (128 * 128 / 16) + (kk & 3) * 2),
+                    kd + ((kk >> 2) * (BN * 128 / 16) + (kk & 3) * 2), id_s, kk > 0);
         tc_commit(&b->s_full[x]);
         // the queries are free once the segment's last scores are done
-        if (nx.last && (x == 1 || !nx.two)) tc_commit(&b->q_empty[nx.k % C::QBufs]);
-      }
-      __syncwarp();
-      return true;
-    };
-    auto product = [&](int x) -> bool {  // O of half x += P V for cur
-      if (!f8_wait(b, &b->p_full[x], (uint32_t)(used[x] & 1), a.err)) return false;
-      ++used[x];
-      if (cur.first) {
-        // the softmax warps have read the half's output of the segment before
-        if (segs[x] > 0 && !f8_wait(b, &b->o_free[x], (uint32_t)(segs[x] - 1) & 1u, a.err)) return false;
-        ++segs[x];
-      }
-      tc_fence_after();
-      if (lane == 0) {
-        const uint32_t v = smem_u32(skv + cur.st * C::StageBytes + C::TileBytes);
+        if ((nx & kF8Last) && (x == 1 || !(nx & kF8Two))) tc_commit(&b->q_empty[k % C::QBufs]);
+      };
+      auto product = [&](auto half) {  // O of a half += P V for cur
+        constexpr int x = decltype(half)::value;
+        ok = f8_wait(b, &b->p_full[x], (uint32_t)(used[x] & 1), a.err);
+        ++used[x];
+        if (ok && (cur & kF8First)) {
+          // the softmax warps have read the half's output of the segment before
+          if (segs[x] > 0) ok = f8_wait(b, &b->o_free[x], (uint32_t)(segs[x] - 1) & 1u, a.err);
+          ++segs[x];
+        }
+        if (!ok) return;
+        tc_fence_after();
+        const uint64_t vd = v_desc + (uint32_t)(cur_st * (C::StageBytes / 16));
 #pragma unroll
-        for (int kk = 0; kk < BN / 16; ++kk) {
-          // P of keys 64.. lies at the end of the S columns, see the softmax
-          const uint32_t pcol = tbase + x * 128 + (kk < 4 ? kk * 8 : 96 + (kk - 4) * 8);
-          tc_mma_ts(tbase + kF8OCol + x * 128, pcol, smem_desc_sw128(v + kk * 2048, BN * 128, 1024), id_o,
-                    (!cur.first || kk > 0) ? 1u : 0u);
+        for (int kk = 0; kk < BN / 16; ++kk)
+          f8_mma_ts(tbase + C::OCol + x * HD, tbase + C::PCol + x * (BN / 2) + kk * 8, vd + kk * (2048 / 16), id_o,
+                    kk > 0 || !(cur & kF8First));
+        tc_commit(&b->pv_done[x]);
+        if (x == 1 || !(cur & kF8Two)) tc_commit(&b->kv_empty[cur_st]);
+      };
+      constexpr std::integral_constant<int, 0> A{};
+      constexpr std::integral_constant<int, 1> B{};
+      take();
+      if (ok && !(nx & kF8End)) {
+        scores(A);
+        if (ok && (nx & kF8Two)) scores(B);
+        while (ok) {
+          cur = nx;
+          cur_st = nx_st;
+          if (++nx_st == kF8Stages) {
+            nx_st = 0;
+            kv_par ^= 1u;
+          }
+          take();
+          const bool more = ok && !(nx & kF8End);
+          if (ok && more) scores(A);
+          if (ok && more && (nx & kF8Two)) scores(B);
+          if (ok) product(A);
+          if (ok && (cur & kF8Two)) product(B);
+          if (!more) break;
         }
-        if (x == 1 || !cur.two) tc_commit(&b->kv_empty[cur.st]);
-        if (cur.last) tc_commit(&b->o_full[x]);
       }
-      __syncwarp();
-      return true;
-    };
-    advance();
-    if (nx.live) {
-      ok = scores(0) && (!nx.two || scores(1));
-      cur = nx;
-      ++g;
-      if (ok) advance();
-      while (ok && cur.live) {
-        ok = product(0);
-        if (ok && nx.live) ok = scores(0);
-        if (ok && cur.two) ok = product(1);
-        if (ok && nx.live && nx.two) ok = scores(1);
-        if (!ok) break;
-        cur = nx;
-        if (nx.live) {
-          ++g;
-          advance();
+      tc_commit(&b->done);
+      mbar_wait_bounded(&b->done, 0, kF8Wait);
+    }
+    __syncwarp();
+    // ------------------------------------------------------------ queries
+    if (warp > 12) {
+      constexpr int LPR = HD / 8, RP = 32 / LPR;     // lanes of a row, rows of a warp's copy
+      const int c = lane % LPR;
+      const int dt = 3 * RP / a.group, dh = 3 * RP % a.group;  // tokens and heads from one of a lane's rows to its next
+      for (int k = 0; seg.valid(); seg.next(a, R), ++k) {
+        const int qb = k % C::QBufs;
+        if (k >= C::QBufs && !f8_wait_idle(b, &b->q_empty[qb], (uint32_t)((k / C::QBufs) - 1) & 1u, a.err)) break;
+        const int rows = seg.rows();
+        const uint32_t dst = smem_u32(sq + qb * C::QBytes) + (c >> 3) * (128 * 128);
+        int row = (warp - 13) * RP + lane / LPR;
+        int tok = (seg.tile * kF8Rows + row) / a.group, head = (seg.tile * kF8Rows + row) % a.group;
+        const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)seg.x.first * a.q_stride + (int64_t)seg.h * a.group * HD + c * 8;
+        for (; row < kF8Rows; row += 3 * RP) {  // rows that are not there become zeros
+          const bool there = row < rows;
+          f8_cp16(dst + (row >> 7) * (128 * HD * 2) + (row & 127) * 128 + (((c & 7) ^ (row & 7)) << 4),
+                  there ? q + (int64_t)tok * a.q_stride + head * HD : q, there ? 16 : 0);
+          tok += dt;
+          head += dh;
+          if (head >= a.group) {
+            head -= a.group;
+            ++tok;
+          }
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        fence_proxy_async_smem();
+        mbar_arrive(&b->q_full[qb]);
       }
     }
-    if (lane == 0) tc_commit(&b->done);
-    __syncwarp();
-    mbar_wait_bounded(&b->done, 0, kF8Wait);
   } else {
+    f8_more_registers<kF8SoftmaxRegs>();
     // ------------------------------------------------------ softmax warps
     const int x = warp >> 2;                       // half
     const int t = (warp & 3) * 32 + lane;          // row of the half, TMEM lane
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tbase + lane_off + x * 128, o_addr = tbase + lane_off + kF8OCol + x * 128;
+    const uint32_t s_addr = tbase + lane_off + C::SCol + x * BN, o_addr = tbase + lane_off + C::OCol + x * HD;
+    const uint32_t p_addr = tbase + lane_off + C::PCol + x * (BN / 2);
     bool ok = true;
-    int64_t g = 0;
-    int used = 0, segs = 0;
-    for (int k = 0; ok && seg.valid(); seg.next(), ++k) {
-      const int qb = k % C::QBufs;
-      if (!f8_wait(b, &b->q_full[qb], (uint32_t)(k / C::QBufs) & 1u, a.err)) break;
+    int st = 0;             // stage of the key tile
+    uint32_t kv_par = 0;    // and its phase parity
+    int used = 0;
+    for (; ok && seg.valid(); seg.next(a, R)) {
       const int rows = seg.rows();
-      const float undo = b->q_undo[qb][x * 128 + t];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&b->q_empty[qb]);
       const int tlo = seg.t_lo(), thi = seg.t_hi();
       if (x == 1 && rows <= 128) {  // the half has no rows
-        g += thi - tlo;
+        for (int kt = tlo; kt < thi; ++kt)
+          if (++st == kF8Stages) {
+            st = 0;
+            kv_par ^= 1u;
+          }
         continue;
       }
       const bool active = x * 128 + (warp & 3) * 32 < rows;  // this warp has rows
-      const int64_t fr = (int64_t)seg.tile * kF8Rows + x * 128 + t;
-      const int64_t qpos = seg.x.ctx + fr / a.group;         // position of the row's token
-      const int64_t first_pos = seg.x.ctx + (fr - lane) / a.group;  // of the warp's first row
+      const int fr = seg.tile * kF8Rows + x * 128 + t;
+      const int qpos = seg.x.ctx + fr / a.group;              // position of the row's token
+      const int first_pos = seg.x.ctx + (fr - lane) / a.group;  // of the warp's first row
       float m_ref = -INFINITY, l = 0.f;
-      for (int kt = tlo; kt < thi; ++kt, ++g, ++used) {
-        const int st = (int)(g % kF8Stages);
-        if (!f8_wait(b, &b->s_full[x], (uint32_t)(used & 1), a.err) ||
-            !f8_wait(b, &b->kv_full[st], (uint32_t)(g / kF8Stages) & 1u, a.err)) {
+      // one key tile of the row, its scores in v; MASK: some row of the warp does not see all of it
+      uint32_t v[BN];
+      auto softmax_tile = [&](int kt, auto masked) {
+        constexpr bool MASK = decltype(masked)::value;
+        const float4* info = b->info[st];
+        const int seen = min(BN, max(0, qpos - kt * BN + 1));  // keys of the tile that the row sees
+        if constexpr (MASK) {
+#pragma unroll
+          for (int e = 0; e < BN; ++e)
+            if (e >= seen) v[e] = 0xff800000u;
+        }
+        // largest y: per 16 keys the largest score, since their factor is not negative
+        float mx = -INFINITY;
+#pragma unroll
+        for (int u = 0; u < C::Subs; ++u) {
+          const float* s = reinterpret_cast<const float*>(&v[16 * u]);
+          const float s0 = f8_max3(f8_max3(s[0], s[1], s[2]), f8_max3(s[3], s[4], s[5]), f8_max3(s[6], s[7], s[8]));
+          const float s1 = f8_max3(f8_max3(s[9], s[10], s[11]), f8_max3(s[12], s[13], s[14]), s[15]);
+          const float4 f = info[u];
+          mx = fmaxf(mx, fmaf(fmaxf(s0, s1), f.x, f.y));
+        }
+        const bool raise = mx > m_ref + kF8Lazy;
+        // the product of the tile before is done: P and O may be written
+        if (used > 0 && !f8_wait(b, &b->pv_done[x], (uint32_t)(used - 1) & 1u, a.err)) return false;
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, raise)) {
+          const float keep = raise ? (m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - mx)) : 1.f;
+          if (raise) {
+            l *= keep;
+            m_ref = mx;
+          }
+          if (kt > tlo) {
+            uint32_t o[16];
+#pragma unroll
+            for (int c = 0; c < HD / 16; ++c) {
+              f8_tmem_ld16(o_addr + 16 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+              tmem_st16(o_addr + 16 * c, o);
+            }
+          }
+        }
+        const float ref = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll
+        for (int w = 0; w < C::Subs / 2; ++w) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int u = 2 * w + h;
+            const float4 f = info[u];
+            const float fc = f.x, fb = f.y - ref;
+            float r0 = 0.f, r1 = 0.f;
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              float y0, y1;
+              f8_fma2(y0, y1, __uint_as_float(v[16 * u + e]), __uint_as_float(v[16 * u + e + 1]), fc, fb);
+              if constexpr (MASK) {  // a factor of 0 made NaN of the masked score
+                if (16 * u + e >= seen) y0 = -INFINITY;
+                if (16 * u + e + 1 >= seen) y1 = -INFINITY;
+              }
+              const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
+              f8_add2(r0, r1, p0, p1);
+              pk[8 * h + e / 2] = f8_pack(p0, p1);
+            }
+            l = fmaf(r0 + r1, f.z, l);
+          }
+          tmem_st16(p_addr + 16 * w, pk);
+        }
+        tmem_wait_st();
+        return true;
+      };
+      for (int kt = tlo; kt < thi; ++kt, ++used) {
+        if (!f8_wait(b, &b->s_full[x], (uint32_t)(used & 1), a.err)) {
           ok = false;
           break;
         }
         tc_fence_after();
         if (active) {
-          const float4* info = b->info[st];
-          const int64_t key0 = (int64_t)kt * BN;
-          const bool mask = key0 + BN - 1 > first_pos;
-          const int seen = (int)min((int64_t)BN, max((int64_t)0, qpos - key0 + 1));  // keys of the tile that the row sees
-          uint32_t v[64];
-          float mx = -INFINITY;
-          // largest y: per 16 keys the largest score, since their factor is not negative
 #pragma unroll
-          for (int h = 0; h < BN / 64; ++h) {
-            tmem_ld32(s_addr + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-            tmem_ld32(s_addr + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-            tmem_wait_ld();
-            if (mask) {
-#pragma unroll
-              for (int e = 0; e < 64; ++e)
-                if (64 * h + e >= seen) v[e] = 0xff800000u;
-            }
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              float s = __uint_as_float(v[16 * u]);
-#pragma unroll
-              for (int e = 1; e < 16; ++e) s = fmaxf(s, __uint_as_float(v[16 * u + e]));
-              const float4 f = info[4 * h + u];
-              mx = fmaxf(mx, fmaf(s, f.x * undo, f.y));
-            }
-          }
-          const bool raise = mx > m_ref + kF8Lazy;
-          if (__any_sync(0xffffffffu, raise)) {
-            const float keep = raise ? (m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - mx)) : 1.f;
-            if (raise) {
-              l *= keep;
-              m_ref = mx;
-            }
-            if (kt > tlo) {
-              // O holds the products up to the last tile: these scores were issued after them, so their
-              // arrival says that the products are done
-              uint32_t o[32];
-#pragma unroll
-              for (int c = 0; c < HD / 32; ++c) {
-                tmem_ld32(o_addr + 32 * c, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-                tmem_st32(o_addr + 32 * c, o);
-              }
-            }
-          }
-          const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-          // the half of the keys that is still in registers first: its P goes to the columns that it came from
-#pragma unroll
-          for (int h = BN / 64 - 1; h >= 0; --h) {
-            if (h < BN / 64 - 1) {
-              tmem_ld32(s_addr + 64 * h, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-              tmem_ld32(s_addr + 64 * h + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-              tmem_wait_ld();
-            }
-            uint32_t pk[32];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              const float4 f = info[4 * h + u];
-              const float fc = f.x * undo, fb = f.y - ref;
-              float r0 = 0.f, r1 = 0.f;
-#pragma unroll
-              for (int e = 0; e < 16; e += 2) {
-                float y0, y1;
-                f8_fma2(y0, y1, __uint_as_float(v[16 * u + e]), __uint_as_float(v[16 * u + e + 1]), fc, fb);
-                if (mask) {
-                  if (64 * h + 16 * u + e >= seen) y0 = -INFINITY;
-                  if (64 * h + 16 * u + e + 1 >= seen) y1 = -INFINITY;
-                }
-                const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
-                f8_add2(r0, r1, p0, p1);
-                pk[8 * u + e / 2] = f8_pack(p0, p1);
-              }
-              l = fmaf(r0 + r1, f.z, l);
-            }
-            tmem_st32(s_addr + 96 * h, pk);
-          }
-          tmem_wait_st();
+          for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
+          // long since there (the scores came from it): makes the loaders' factors visible
+          ok = f8_wait(b, &b->kv_full[st], kv_par, a.err);
+          tmem_wait_ld();
         }
         tc_fence_before();
-        mbar_arrive(&b->p_full[x]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b->s_free[x]);
+        if (active) {
+          if (kt * BN + BN - 1 > first_pos) ok = softmax_tile(kt, std::true_type{}) && ok;
+          else ok = softmax_tile(kt, std::false_type{}) && ok;
+        } else if (used > 0) {
+          // a warp without rows keeps step: it must not arrive twice in one phase of p_full
+          ok = f8_wait(b, &b->pv_done[x], (uint32_t)(used - 1) & 1u, a.err);
+        }
+        if (!__all_sync(0xffffffffu, ok)) {
+          ok = false;
+          break;
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&b->p_full[x]);
+        if (++st == kF8Stages) {
+          st = 0;
+          kv_par ^= 1u;
+        }
       }
       if (!ok) break;
-      if (!f8_wait(b, &b->o_full[x], (uint32_t)(segs & 1), a.err)) break;
-      ++segs;
+      if (!f8_wait(b, &b->pv_done[x], (uint32_t)(used - 1) & 1u, a.err)) break;
       tc_fence_after();
       const bool whole = tlo == 0 && thi == seg.n;
       const int row = x * 128 + t;
       float* ps = p.partials + (int64_t)(2 * blockIdx.x + (tlo == 0)) * (HD + 2) * kF8Rows + row;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      T* op = reinterpret_cast<T*>(a.out) + (seg.x.first + fr / a.group) * a.out_stride +
+      T* op = reinterpret_cast<T*>(a.out) + (int64_t)(seg.x.first + fr / a.group) * a.out_stride +
               (int64_t)(seg.h * a.group + fr % a.group) * HD;
       if (active) {
 #pragma unroll
@@ -731,10 +786,11 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const Kv8Arg
         }
       }
       tc_fence_before();
-      mbar_arrive(&b->o_free[x]);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b->o_free[x]);
       if (tlo == 0 && thi < seg.n && threadIdx.x == 0)
         p.cuts[blockIdx.x] = F8Cut{(int64_t)seg.tile * kF8Rows, seg.x.first, rows, seg.h,
-                                   (int)((seg.start + seg.n - 1) / W - blockIdx.x), 0};
+                                   (int)((lo + seg.start + seg.n - 1) / W - blockIdx.x), 0};
     }
   }
   tc_fence_before();
@@ -748,7 +804,8 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const Kv8Arg
 // Segments cut by borders: CTA (c, y) merges 32 rows of the one that begins in
 // the first kernel's CTA c, its parts in order.  A thread: one row, every 8th dim.
 template <int HD, typename T>
-__global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const Kv8Args a, const F8Plan p) {
+__global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const __grid_constant__ Kv8Args a,
+                                                                 const __grid_constant__ F8Plan p) {
   pdl_wait();
   const F8Cut cut = p.cuts[blockIdx.x];
   const int row = blockIdx.y * 32 + (threadIdx.x & 31), d0 = threadIdx.x >> 5;
@@ -786,7 +843,7 @@ bool kv8_prefill_takes(int dtype, const Kv8Args& a) {
   auto aligned = [](const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
   return (dtype == NIE_DTYPE_BF16 || dtype == NIE_DTYPE_F16) && (a.hd == 64 || a.hd == 128) && a.bs % 16 == 0 &&
          aligned(a.kc, 16) && aligned(a.vc, 16) && aligned(a.q, 16) && aligned(a.out, 16) && a.q_stride % 8 == 0 &&
-         a.out_stride % 8 == 0;
+         a.out_stride % 8 == 0 && a.nb * a.bs < (int64_t(1) << 31) && a.num_q_rows * a.group < (int64_t(1) << 31);
 }
 
 template <int HD, typename T>
