@@ -13,26 +13,29 @@
 // head against all keys that its last token sees.
 //
 // Split.  All segments lie end to end, each weighted as its key tiles plus a
-// fixed part; every CTA (one per SM) takes an equal stretch.  A segment cut by
-// a border leaves (max, sum, unnormalised output) of each part for a merging
-// kernel; which parts and in which order follows from the lengths alone.
+// fixed part; every CTA takes an equal stretch.  A segment cut by a border leaves
+// (max, sum, unnormalised output) of each part for a merging kernel; which parts
+// and in which order follows from the lengths alone.
 //
-// Roles (16 warps):
-//   warps 0-3, 4-7  softmax of half A, B: a thread owns a row.  It takes the row's
-//                   scores of a tile into registers at once, so that the next
-//                   tile's S runs under this tile's exponentials
-//   warps 8-11      codes to 16 bits (exact: K in the queries' type, V in f16) into
-//                   128-byte swizzled shared memory; they come two tiles ahead by cp.async into a thread's own bytes
-//   warp 12         one thread issues S = Q K^T and O += P V (P from TMEM)
-//   warps 13-15     queries to shared memory, a segment ahead where it has room for two
+// Latency is what such a chain costs (S, its softmax, P V, the next S of the same
+// rows, each waiting for the one before), so several chains share an SM: the two
+// halves of a tile, and at head_dim 64 two CTAs.
+//
+// Roles:
+//   warps 0-3, 4-7  softmax of half A, B: a thread owns a row
+//   warp 8          one thread issues S = Q K^T and O += P V (P from TMEM), A and B in turn
+//   warp 9          queries to shared memory
+//   the others      codes to 16 bits (exact: K in the queries' type, V in f16) into
+//                   128-byte swizzled shared memory; they come two tiles ahead
+//                   by cp.async into a thread's own bytes
 //
 // Softmax with scales as in the single-token kernel: y = S c + log2 vs per block
 // of 16 keys, p = 2^(y - m) in f16 for the product (its error of 2^-12 is below
 // the output's step), O = sum p vcode, l = sum p / vs from the unrounded p.  m
 // is raised (and O and l rescaled) only when exceeded by more than 2^8.
 //
-// TMEM columns: head_dim 64: S 0-255, O 256-383, P 384-511; head_dim 128: S 0-127,
-// P 128-191, O 256-511 (A's part first).  Waits are bounded; one that runs out raises
+// TMEM columns: S of A 0-63, of B 64-127 (P takes the place of the scores it came
+// from), then O of A and B.  Waits are bounded; one that runs out raises
 // NIE_DEV_ERR_TIMEOUT and ends the CTA.
 #include <algorithm>
 #include <type_traits>
@@ -42,13 +45,9 @@
 namespace nie {
 
 constexpr int kF8Rows = 256;
-constexpr int kF8Threads = 16 * 32;
-// Registers per thread after the split: 256 softmax threads, 256 others; together what 512 threads have at launch.
-constexpr int kF8SoftmaxRegs = 184, kF8OtherRegs = 72;
-static_assert(256 * (kF8SoftmaxRegs + kF8OtherRegs) <= 65536, "more registers than the launch has");
-constexpr int kF8Stages = 3;       // f16 key tiles in shared memory
-constexpr int kF8MaxReq = 512;     // requests of one launch
-constexpr int kF8SegCost = 2;      // a segment's fixed part, in key tiles
+constexpr int kF8Stages = 3;       // 16-bit key tiles in shared memory
+constexpr int kF8MaxReq = 256;     // requests of one launch
+constexpr int kF8SegCost = 5;      // a segment's fixed part, in key tiles
 constexpr uint32_t kF8Wait = 1u << 22;
 constexpr float kF8Log2e = 1.4426950408889634f;
 constexpr float kF8Lazy = 8.f;
@@ -69,24 +68,26 @@ struct F8Plan {
 
 template <int HD>
 struct F8Cfg {
-  static constexpr int BN = HD == 64 ? 128 : 64;          // keys of a tile
-  static constexpr int QBufs = HD == 64 ? 2 : 1;
+  static constexpr int BN = 64;                           // keys of a tile
+  static constexpr int Subs = BN / 16;
+  static constexpr int Ctas = HD == 64 ? 2 : 1;           // per SM
+  static constexpr int Loaders = HD == 64 ? 64 : 128;     // threads
+  static constexpr int Threads = 10 * 32 + Loaders;
   static constexpr int QBytes = kF8Rows * HD * 2;
-  static constexpr int TileBytes = BN * HD * 2;           // K or V of a tile in f16
+  static constexpr int TileBytes = BN * HD * 2;           // K or V of a tile in 16 bits
   static constexpr int StageBytes = 2 * TileBytes;
   static constexpr int CodeBytes = 2 * BN * HD;           // codes of a tile
-  static constexpr int Subs = BN / 16;
-  // TMEM columns; a half's S, O and P are BN, HD and BN / 2 wide
-  static constexpr uint32_t SCol = 0, OCol = 256, PCol = HD == 64 ? 384 : 128;
+  static constexpr uint32_t Cols = HD == 64 ? 256 : 512;  // TMEM columns
+  static constexpr uint32_t OCol = HD == 64 ? 128 : 256;
 };
 
 // A key tile of a segment: its first in this CTA, its last, with rows in half B; the end of the stretch.
 enum F8Flag { kF8First = 1, kF8Last = 2, kF8Two = 4, kF8End = 8 };
 
 struct F8Bars {
-  uint64_t q_full[2], q_empty[2];
+  uint64_t q_full, q_empty;
   uint64_t kv_full[kF8Stages], kv_empty[kF8Stages];
-  uint64_t s_full[2], s_free[2], p_full[2], pv_done[2], o_free[2];
+  uint64_t s_full[2], p_full[2], o_full[2], o_free[2];
   uint64_t done;
   uint32_t tmem_base;
   int abort;
@@ -161,7 +162,7 @@ struct F8Req {
   int tiles;  // 256-row tiles
 };
 
-__device__ __forceinline__ F8Req f8_request(const Kv8Args& a, int i, int32_t* err) {
+__device__ __noinline__ F8Req f8_request(const Kv8Args& a, int i, int32_t* err) {
   F8Req x{};
   const int r = a.req_list ? a.req_list[i] : i;
   const int tr = r < 0 || r >= a.num_seqs ? -1 : a.table_rows ? a.table_rows[r] : r;
@@ -249,33 +250,15 @@ __device__ __forceinline__ void f8_mma_ts(uint32_t d, uint32_t a, uint64_t b, ui
       : "memory");
 }
 
-// 32 lanes x 16 consecutive 32-bit columns.
-__device__ __forceinline__ void f8_tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr));
-}
-
-template <int REGS>
-__device__ __forceinline__ void f8_more_registers() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(REGS));
-}
-template <int REGS>
-__device__ __forceinline__ void f8_fewer_registers() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(REGS));
-}
-
 template <int HD, typename T>
-__global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid_constant__ Kv8Args a,
-                                                                    const __grid_constant__ F8Plan p) {
+__global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
+    kv8_prefill_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ F8Plan p) {
   using C = F8Cfg<HD>;
   constexpr int BN = C::BN;
   extern __shared__ uint8_t f8_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(f8_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = sm;
-  uint8_t* skv = sq + C::QBufs * C::QBytes;
+  uint8_t* skv = sq + C::QBytes;
   uint8_t* scode = skv + kF8Stages * C::StageBytes;
   F8Bars* b = reinterpret_cast<F8Bars*>(scode + 2 * C::CodeBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -284,7 +267,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
   pdl_wait();
   pdl_trigger();
   // ---- cost of each request (a warp each), then of all before it
-  for (int i = warp; i < R; i += kF8Threads / 32) {
+  for (int i = warp; i < R; i += C::Threads / 32) {
     const F8Req x = f8_request(a, i, blockIdx.x == 0 && lane == 0 ? a.err : nullptr);
     int64_t cost = 0;
     for (int tile = lane; tile < x.tiles; tile += 32) cost += f8_key_tiles<BN>(f8_keys(x, a.group, tile)) + kF8SegCost;
@@ -294,17 +277,16 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
   }
   if (threadIdx.x == 0) {
     b->cum[0] = 0;
+    mbar_init(&b->q_full, 32);
+    mbar_init(&b->q_empty, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&b->q_full[i], 96);
-      mbar_init(&b->q_empty[i], 1);
       mbar_init(&b->s_full[i], 1);
-      mbar_init(&b->s_free[i], 4);
       mbar_init(&b->p_full[i], 4);
-      mbar_init(&b->pv_done[i], 1);
+      mbar_init(&b->o_full[i], 1);
       mbar_init(&b->o_free[i], 4);
     }
     for (int s = 0; s < kF8Stages; ++s) {
-      mbar_init(&b->kv_full[s], 128);
+      mbar_init(&b->kv_full[s], C::Loaders);
       mbar_init(&b->kv_empty[s], 1);
     }
     mbar_init(&b->done, 1);
@@ -361,8 +343,8 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
       if (lo < pos) break;
     }
   }
-  if (warp == 12) {
-    tmem_alloc(&b->tmem_base, 512);
+  if (warp == 8) {
+    tmem_alloc(&b->tmem_base, C::Cols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -372,10 +354,10 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
   F8Walk<BN> seg;
   seg.init(a, b, lo, hi);
 
-  if (warp >= 8 && warp < 12) {
-    f8_fewer_registers<kF8OtherRegs>();
+  if (warp >= 10) {
     // ------------------------------------------------------------ loaders
-    const int tid = threadIdx.x - 256;
+    const int tid = threadIdx.x - 320;
+    constexpr int Pass = C::Loaders / 4, Passes = BN / Pass;  // rows of a copy, copies for 64 dims of all rows
     const int64_t row_bytes = (int64_t)a.hkv * HD;
     const float coef = fabsf(a.scale) * kF8Log2e;
     const uint32_t flip = a.scale < 0.f ? 0x80808080u : 0u;  // a negative scale's sign goes to the keys
@@ -395,7 +377,7 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
         entry = count > 0 && lb < a.tstride ? a.tables[(int64_t)ahead.x.trow * a.tstride + lb] : -1;
       }
     };
-    // scales of the next tile and of the one after it (warp 8, lane s: the s-th 16 keys)
+    // scales of the next tile and of the one after it (first warp, lane s: the s-th 16 keys)
     float ks0 = 0.f, vs0 = 1.f, ks1 = 0.f, vs1 = 1.f;
     bool ok0 = false, ok1 = false;
     auto fetch = [&](int slot, float& p_ks, float& p_vs, bool& p_ok) {
@@ -413,14 +395,14 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int half = j / (BN / 32);
-          const int s = 2 * (j % (BN / 32)) + (tid >> 6), row = (tid >> 2) & 15;
+          const int half = j / Passes;
+          const int s = ((tid >> 2) + Pass * (j % Passes)) >> 4, row = (tid >> 2) & 15;  // all of a warp's rows lie in 16 keys
           const int from = __shfl_sync(0xffffffffu, at, s);
           const bool there = row < __shfl_sync(0xffffffffu, here, s);
           const int64_t off =
               there ? (int64_t)(from + row) * row_bytes + (int64_t)ahead.h * HD + half * 64 + (tid & 3) * 16 : 0;
-          f8_cp16(base + j * 2048, a.kc + off, there ? 16 : 0);
-          f8_cp16(base + (4 + j) * 2048, a.vc + off, there ? 16 : 0);
+          f8_cp16(base + j * (C::Loaders * 16), a.kc + off, there ? 16 : 0);
+          f8_cp16(base + (4 + j) * (C::Loaders * 16), a.vc + off, there ? 16 : 0);
         }
         if (++a_kt >= ahead.t_hi()) {
           ahead.next(a, R);
@@ -450,8 +432,8 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           const int jj = j & 3;
-          const int row = (tid >> 2) + 32 * (jj % (BN / 32)), half = jj / (BN / 32);
-          const uint4 x = *reinterpret_cast<const uint4*>(src + j * 2048);
+          const int row = (tid >> 2) + Pass * (jj % Passes), half = jj / Passes;
+          const uint4 x = *reinterpret_cast<const uint4*>(src + j * (C::Loaders * 16));
           uint32_t w[4] = {x.x, x.y, x.z, x.w}, h[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -497,49 +479,41 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp >= 12) {
-    f8_fewer_registers<kF8OtherRegs>();
+  } else if (warp == 8) {
     // --------------------------------------------------------- MMA issuer
     // One thread.  What it has to know of a key tile stands beside the tile.
-    if (warp == 12 && lane == 0) {
+    if (lane == 0) {
       const uint64_t q_desc = smem_desc_sw128(smem_u32(sq), 16, 1024), k_desc = smem_desc_sw128(smem_u32(skv), 16, 1024);
       const uint64_t v_desc = smem_desc_sw128(smem_u32(skv + C::TileBytes), BN * 128, 1024);
       constexpr uint32_t id_s = f8_idesc(128, BN, false, !std::is_same<T, __half>::value);
       constexpr uint32_t id_o = f8_idesc(128, HD, true, false);
       int nx = 0, cur = 0;          // flags of the tile whose scores come next, and of the one before it
       int nx_st = 0, cur_st = 0;    // their stages
-      uint32_t kv_par = 0;          // phase parity of nx_st
-      int k = -1;                   // segment of nx
-      int issued[2] = {0, 0};       // scores and products of each half
-      int used[2] = {0, 0};
+      uint32_t kv_par = 0, q_par = 0;  // phase parities of nx_st and of the queries
+      int used[2] = {0, 0};         // products of each half
       int segs[2] = {0, 0};         // segments that wrote its output
       bool ok = true;
       auto take = [&]() {  // the flags of the tile in stage nx_st
         ok = f8_wait(b, &b->kv_full[nx_st], kv_par, a.err);
         nx = ok ? *reinterpret_cast<volatile int*>(&b->flags[nx_st]) : kF8End;
         if (ok && (nx & kF8First)) {
-          ++k;
-          ok = f8_wait(b, &b->q_full[k % C::QBufs], (uint32_t)(k / C::QBufs) & 1u, a.err);
+          ok = f8_wait(b, &b->q_full, q_par, a.err);
+          q_par ^= 1u;
         }
         tc_fence_after();
       };
       auto scores = [&](auto half) {  // S of a half for nx
         constexpr int x = decltype(half)::value;
-        // the softmax warps have taken the scores before these
-        if (issued[x] > 0) ok = f8_wait(b, &b->s_free[x], (uint32_t)(issued[x] - 1) & 1u, a.err);
-        if (!ok) return;
-        ++issued[x];
-        tc_fence_after();
         // descriptors count addresses in 16 bytes: steps along a row or to the next 64 dims are added to them
-        const uint64_t q = q_desc + (uint32_t)((k % C::QBufs) * (C::QBytes / 16) + x * (128 * HD * 2 / 16));
+        const uint64_t q = q_desc + (uint32_t)(x * (128 * HD * 2 / 16));
         const uint64_t kd = k_desc + (uint32_t)(nx_st * (C::StageBytes / 16));
 #pragma unroll
         for (int kk = 0; kk < HD / 16; ++kk)
-          f8_mma_ss(tbase + C::SCol + x * BN, q + ((kk >> 2) * (128 * 128 / 16) + (kk & 3) * 2),
+          f8_mma_ss(tbase + x * BN, q + ((kk >> 2) * (128 * 128 / 16) + (kk & 3) * 2),
                     kd + ((kk >> 2) * (BN * 128 / 16) + (kk & 3) * 2), id_s, kk > 0);
         tc_commit(&b->s_full[x]);
         // the queries are free once the segment's last scores are done
-        if ((nx & kF8Last) && (x == 1 || !(nx & kF8Two))) tc_commit(&b->q_empty[k % C::QBufs]);
+        if ((nx & kF8Last) && (x == 1 || !(nx & kF8Two))) tc_commit(&b->q_empty);
       };
       auto product = [&](auto half) {  // O of a half += P V for cur
         constexpr int x = decltype(half)::value;
@@ -555,17 +529,16 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
         const uint64_t vd = v_desc + (uint32_t)(cur_st * (C::StageBytes / 16));
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          f8_mma_ts(tbase + C::OCol + x * HD, tbase + C::PCol + x * (BN / 2) + kk * 8, vd + kk * (2048 / 16), id_o,
-                    kk > 0 || !(cur & kF8First));
-        tc_commit(&b->pv_done[x]);
+          f8_mma_ts(tbase + C::OCol + x * HD, tbase + x * BN + kk * 8, vd + kk * (2048 / 16), id_o, kk > 0 || !(cur & kF8First));
         if (x == 1 || !(cur & kF8Two)) tc_commit(&b->kv_empty[cur_st]);
+        if (cur & kF8Last) tc_commit(&b->o_full[x]);
       };
       constexpr std::integral_constant<int, 0> A{};
       constexpr std::integral_constant<int, 1> B{};
       take();
       if (ok && !(nx & kF8End)) {
         scores(A);
-        if (ok && (nx & kF8Two)) scores(B);
+        if (nx & kF8Two) scores(B);
         while (ok) {
           cur = nx;
           cur_st = nx_st;
@@ -573,12 +546,12 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
             nx_st = 0;
             kv_par ^= 1u;
           }
-          take();
+          product(A);
+          if (ok) take();
           const bool more = ok && !(nx & kF8End);
-          if (ok && more) scores(A);
-          if (ok && more && (nx & kF8Two)) scores(B);
-          if (ok) product(A);
+          if (more) scores(A);  // over the P that the product issued before reads: MMAs run in order
           if (ok && (cur & kF8Two)) product(B);
+          if (ok && more && (nx & kF8Two)) scores(B);
           if (!more) break;
         }
       }
@@ -586,47 +559,45 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
       mbar_wait_bounded(&b->done, 0, kF8Wait);
     }
     __syncwarp();
+  } else if (warp == 9) {
     // ------------------------------------------------------------ queries
-    if (warp > 12) {
-      constexpr int LPR = HD / 8, RP = 32 / LPR;     // lanes of a row, rows of a warp's copy
-      const int c = lane % LPR;
-      const int dt = 3 * RP / a.group, dh = 3 * RP % a.group;  // tokens and heads from one of a lane's rows to its next
-      for (int k = 0; seg.valid(); seg.next(a, R), ++k) {
-        const int qb = k % C::QBufs;
-        if (k >= C::QBufs && !f8_wait_idle(b, &b->q_empty[qb], (uint32_t)((k / C::QBufs) - 1) & 1u, a.err)) break;
-        const int rows = seg.rows();
-        const uint32_t dst = smem_u32(sq + qb * C::QBytes) + (c >> 3) * (128 * 128);
-        int row = (warp - 13) * RP + lane / LPR;
-        int tok = (seg.tile * kF8Rows + row) / a.group, head = (seg.tile * kF8Rows + row) % a.group;
-        const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)seg.x.first * a.q_stride + (int64_t)seg.h * a.group * HD + c * 8;
-        for (; row < kF8Rows; row += 3 * RP) {  // rows that are not there become zeros
-          const bool there = row < rows;
-          f8_cp16(dst + (row >> 7) * (128 * HD * 2) + (row & 127) * 128 + (((c & 7) ^ (row & 7)) << 4),
-                  there ? q + (int64_t)tok * a.q_stride + head * HD : q, there ? 16 : 0);
-          tok += dt;
-          head += dh;
-          if (head >= a.group) {
-            head -= a.group;
-            ++tok;
-          }
+    constexpr int LPR = HD / 8, RP = 32 / LPR;     // lanes of a row, rows of a copy
+    const int c = lane % LPR;
+    const int dt = RP / a.group, dh = RP % a.group;  // tokens and heads from one of a lane's rows to its next
+    for (int k = 0; seg.valid(); seg.next(a, R), ++k) {
+      if (!f8_wait_idle(b, &b->q_empty, (uint32_t)(k + 1) & 1u, a.err)) break;
+      const int rows = seg.rows();
+      const uint32_t dst = smem_u32(sq) + (c >> 3) * (128 * 128);
+      int row = lane / LPR;
+      int tok = (seg.tile * kF8Rows + row) / a.group, head = (seg.tile * kF8Rows + row) % a.group;
+      const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)seg.x.first * a.q_stride + (int64_t)seg.h * a.group * HD + c * 8;
+      const int last = rows > 128 ? kF8Rows : 128;  // half B without rows is not used
+#pragma unroll 4
+      for (; row < last; row += RP) {  // rows that are not there become zeros
+        const bool there = row < rows;
+        f8_cp16(dst + (row >> 7) * (128 * HD * 2) + (row & 127) * 128 + (((c & 7) ^ (row & 7)) << 4),
+                there ? q + (int64_t)tok * a.q_stride + head * HD : q, there ? 16 : 0);
+        tok += dt;
+        head += dh;
+        if (head >= a.group) {
+          head -= a.group;
+          ++tok;
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_proxy_async_smem();
-        mbar_arrive(&b->q_full[qb]);
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async_smem();
+      mbar_arrive(&b->q_full);
     }
   } else {
-    f8_more_registers<kF8SoftmaxRegs>();
     // ------------------------------------------------------ softmax warps
     const int x = warp >> 2;                       // half
     const int t = (warp & 3) * 32 + lane;          // row of the half, TMEM lane
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tbase + lane_off + C::SCol + x * BN, o_addr = tbase + lane_off + C::OCol + x * HD;
-    const uint32_t p_addr = tbase + lane_off + C::PCol + x * (BN / 2);
+    const uint32_t s_addr = tbase + lane_off + x * BN, o_addr = tbase + lane_off + C::OCol + x * HD;
     bool ok = true;
     int st = 0;             // stage of the key tile
     uint32_t kv_par = 0;    // and its phase parity
-    int used = 0;
+    int used = 0, segs = 0;
     for (; ok && seg.valid(); seg.next(a, R)) {
       const int rows = seg.rows();
       const int tlo = seg.t_lo(), thi = seg.t_hi();
@@ -643,77 +614,79 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
       const int qpos = seg.x.ctx + fr / a.group;              // position of the row's token
       const int first_pos = seg.x.ctx + (fr - lane) / a.group;  // of the warp's first row
       float m_ref = -INFINITY, l = 0.f;
-      // one key tile of the row, its scores in v; MASK: some row of the warp does not see all of it
-      uint32_t v[BN];
+      // One key tile of the row; MASK: some row of the warp does not see all of it.  Loops of 32 keys that
+      // stay loops: unrolled, the roles' code together outgrows the instruction caches.
       auto softmax_tile = [&](int kt, auto masked) {
         constexpr bool MASK = decltype(masked)::value;
         const float4* info = b->info[st];
         const int seen = min(BN, max(0, qpos - kt * BN + 1));  // keys of the tile that the row sees
-        if constexpr (MASK) {
-#pragma unroll
-          for (int e = 0; e < BN; ++e)
-            if (e >= seen) v[e] = 0xff800000u;
-        }
+        uint32_t v[32];
         // largest y: per 16 keys the largest score, since their factor is not negative
         float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; ++c) {
+          tmem_ld32(s_addr + 32 * c, v);
+          const float4 f0 = info[2 * c], f1 = info[2 * c + 1];
+          tmem_wait_ld();
+          if constexpr (MASK) {
 #pragma unroll
-        for (int u = 0; u < C::Subs; ++u) {
-          const float* s = reinterpret_cast<const float*>(&v[16 * u]);
-          const float s0 = f8_max3(f8_max3(s[0], s[1], s[2]), f8_max3(s[3], s[4], s[5]), f8_max3(s[6], s[7], s[8]));
-          const float s1 = f8_max3(f8_max3(s[9], s[10], s[11]), f8_max3(s[12], s[13], s[14]), s[15]);
-          const float4 f = info[u];
-          mx = fmaxf(mx, fmaf(fmaxf(s0, s1), f.x, f.y));
+            for (int e = 0; e < 32; ++e)
+              if (32 * c + e >= seen) v[e] = 0xff800000u;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float* s = reinterpret_cast<const float*>(&v[16 * h]);
+            const float s0 = f8_max3(f8_max3(s[0], s[1], s[2]), f8_max3(s[3], s[4], s[5]), f8_max3(s[6], s[7], s[8]));
+            const float s1 = f8_max3(f8_max3(s[9], s[10], s[11]), f8_max3(s[12], s[13], s[14]), s[15]);
+            mx = fmaxf(mx, fmaf(fmaxf(s0, s1), h ? f1.x : f0.x, h ? f1.y : f0.y));
+          }
         }
         const bool raise = mx > m_ref + kF8Lazy;
-        // the product of the tile before is done: P and O may be written
-        if (used > 0 && !f8_wait(b, &b->pv_done[x], (uint32_t)(used - 1) & 1u, a.err)) return false;
-        tc_fence_after();
         if (__any_sync(0xffffffffu, raise)) {
           const float keep = raise ? (m_ref == -INFINITY ? 0.f : fast_exp2(m_ref - mx)) : 1.f;
           if (raise) {
             l *= keep;
             m_ref = mx;
           }
-          if (kt > tlo) {
-            uint32_t o[16];
-#pragma unroll
-            for (int c = 0; c < HD / 16; ++c) {
-              f8_tmem_ld16(o_addr + 16 * c, o);
+          if (kt > tlo) {  // O is complete up to the last tile: these scores were issued after its product
+#pragma unroll 1
+            for (int c = 0; c < HD / 32; ++c) {
+              tmem_ld32(o_addr + 32 * c, v);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-              tmem_st16(o_addr + 16 * c, o);
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
+              tmem_st32(o_addr + 32 * c, v);
             }
           }
         }
         const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-#pragma unroll
-        for (int w = 0; w < C::Subs / 2; ++w) {
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; ++c) {
+          tmem_ld32(s_addr + 32 * c, v);
+          const float4 f0 = info[2 * c], f1 = info[2 * c + 1];
+          tmem_wait_ld();
           uint32_t pk[16];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int u = 2 * w + h;
-            const float4 f = info[u];
-            const float fc = f.x, fb = f.y - ref;
+            const float fc = h ? f1.x : f0.x, fb = (h ? f1.y : f0.y) - ref;
             float r0 = 0.f, r1 = 0.f;
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
+            for (int e = 16 * h; e < 16 * h + 16; e += 2) {
               float y0, y1;
-              f8_fma2(y0, y1, __uint_as_float(v[16 * u + e]), __uint_as_float(v[16 * u + e + 1]), fc, fb);
-              if constexpr (MASK) {  // a factor of 0 made NaN of the masked score
-                if (16 * u + e >= seen) y0 = -INFINITY;
-                if (16 * u + e + 1 >= seen) y1 = -INFINITY;
+              f8_fma2(y0, y1, __uint_as_float(v[e]), __uint_as_float(v[e + 1]), fc, fb);
+              if constexpr (MASK) {
+                if (32 * c + e >= seen) y0 = -INFINITY;
+                if (32 * c + e + 1 >= seen) y1 = -INFINITY;
               }
               const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
               f8_add2(r0, r1, p0, p1);
-              pk[8 * h + e / 2] = f8_pack(p0, p1);
+              pk[e / 2] = f8_pack(p0, p1);
             }
-            l = fmaf(r0 + r1, f.z, l);
+            l = fmaf(r0 + r1, h ? f1.z : f0.z, l);
           }
-          tmem_st16(p_addr + 16 * w, pk);
+          tmem_st16(s_addr + 16 * c, pk);  // over scores that were taken
         }
         tmem_wait_st();
-        return true;
       };
       for (int kt = tlo; kt < thi; ++kt, ++used) {
         if (!f8_wait(b, &b->s_full[x], (uint32_t)(used & 1), a.err)) {
@@ -722,25 +695,14 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
         }
         tc_fence_after();
         if (active) {
-#pragma unroll
-          for (int c = 0; c < BN / 32; ++c) tmem_ld32(s_addr + 32 * c, *reinterpret_cast<uint32_t(*)[32]>(&v[32 * c]));
           // long since there (the scores came from it): makes the loaders' factors visible
           ok = f8_wait(b, &b->kv_full[st], kv_par, a.err);
-          tmem_wait_ld();
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&b->s_free[x]);
-        if (active) {
-          if (kt * BN + BN - 1 > first_pos) ok = softmax_tile(kt, std::true_type{}) && ok;
-          else ok = softmax_tile(kt, std::false_type{}) && ok;
-        } else if (used > 0) {
-          // a warp without rows keeps step: it must not arrive twice in one phase of p_full
-          ok = f8_wait(b, &b->pv_done[x], (uint32_t)(used - 1) & 1u, a.err);
-        }
-        if (!__all_sync(0xffffffffu, ok)) {
-          ok = false;
-          break;
+          if (!__all_sync(0xffffffffu, ok)) {
+            ok = false;
+            break;
+          }
+          if (kt * BN + BN - 1 > first_pos) softmax_tile(kt, std::true_type{});
+          else softmax_tile(kt, std::false_type{});
         }
         tc_fence_before();
         __syncwarp();
@@ -751,7 +713,8 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
         }
       }
       if (!ok) break;
-      if (!f8_wait(b, &b->pv_done[x], (uint32_t)(used - 1) & 1u, a.err)) break;
+      if (!f8_wait(b, &b->o_full[x], (uint32_t)(segs & 1), a.err)) break;
+      ++segs;
       tc_fence_after();
       const bool whole = tlo == 0 && thi == seg.n;
       const int row = x * 128 + t;
@@ -795,9 +758,9 @@ __global__ void __launch_bounds__(kF8Threads, 1) kv8_prefill_kernel(const __grid
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == 8) {
     tc_fence_after();
-    tmem_dealloc(tbase, 512);
+    tmem_dealloc(tbase, C::Cols);
   }
 }
 
@@ -833,10 +796,12 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const __grid_con
   for (int d = 0; d < HD / 8; ++d) op[d0 + 8 * d] = Num<T>::from_f(O[d] * inv);
 }
 
-static size_t f8_cut_bytes(int sms) { return ((size_t)sms * sizeof(F8Cut) + 255) & ~size_t(255); }
+static int f8_ctas(int sms, int head_dim) { return sms * (head_dim == 64 ? F8Cfg<64>::Ctas : F8Cfg<128>::Ctas); }
+static size_t f8_cut_bytes(int ctas) { return ((size_t)ctas * sizeof(F8Cut) + 255) & ~size_t(255); }
 
 size_t kv8_prefill_workspace(int sms, int head_dim) {
-  return f8_cut_bytes(sms) + (size_t)2 * sms * (head_dim + 2) * kF8Rows * sizeof(float);
+  const int ctas = f8_ctas(sms, head_dim);
+  return f8_cut_bytes(ctas) + (size_t)2 * ctas * (head_dim + 2) * kF8Rows * sizeof(float);
 }
 
 bool kv8_prefill_takes(int dtype, const Kv8Args& a) {
@@ -849,14 +814,14 @@ bool kv8_prefill_takes(int dtype, const Kv8Args& a) {
 template <int HD, typename T>
 static int launch_prefill(const Kv8Args& a, const F8Plan& p, int sms, cudaStream_t s) {
   using C = F8Cfg<HD>;
-  const size_t smem = 1024 + (size_t)C::QBufs * C::QBytes + (size_t)kF8Stages * C::StageBytes + 2 * C::CodeBytes + sizeof(F8Bars);
+  const size_t smem = 1024 + C::QBytes + (size_t)kF8Stages * C::StageBytes + 2 * C::CodeBytes + sizeof(F8Bars);
   auto* kernel = kv8_prefill_kernel<HD, T>;
   const int rc = opt_in_smem(kSmemKv8Prefill + (HD == 128) * 2 + std::is_same<T, __half>::value, (const void*)kernel, smem);
   if (rc != NIE_OK) return rc;
-  kernel<<<sms, kF8Threads, smem, s>>>(a, p);
+  kernel<<<sms * C::Ctas, C::Threads, smem, s>>>(a, p);
   const int st = check_launch("kv8_prefill_kernel");
   if (st != NIE_OK) return st;
-  pdl_launch(kv8_prefill_merge_kernel<HD, T>, dim3((unsigned)sms, kF8Rows / 32), dim3(256), s, a, p);
+  pdl_launch(kv8_prefill_merge_kernel<HD, T>, dim3((unsigned)(sms * C::Ctas), kF8Rows / 32), dim3(256), s, a, p);
   return check_launch("kv8_prefill_merge_kernel");
 }
 
@@ -878,7 +843,7 @@ int launch_kv8_prefill(int dtype, const Kv8Args& args, int num_requests, int sms
       }
     }
     p.cuts = (F8Cut*)workspace;
-    p.partials = (float*)((char*)workspace + f8_cut_bytes(sms));
+    p.partials = (float*)((char*)workspace + f8_cut_bytes(f8_ctas(sms, a.hd)));
     int rc;
     if (a.hd == 64) rc = dtype == NIE_DTYPE_F16 ? launch_prefill<64, __half>(a, p, sms, s) : launch_prefill<64, __nv_bfloat16>(a, p, sms, s);
     else rc = dtype == NIE_DTYPE_F16 ? launch_prefill<128, __half>(a, p, sms, s) : launch_prefill<128, __nv_bfloat16>(a, p, sms, s);
