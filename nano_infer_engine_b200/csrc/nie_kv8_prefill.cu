@@ -17,15 +17,16 @@
 // (max, sum, unnormalised output) of each part for a merging kernel; which parts
 // and in which order follows from the lengths alone.
 //
-// Latency is what such a chain costs (S, its softmax, P V, the next S of the same
-// rows, each waiting for the one before), so several chains share an SM: the two
-// halves of a tile, and at head_dim 64 two CTAs.
+// Latency is what the chain of a row costs (S, its softmax, P V, each waiting for
+// the one before): a half has two S buffers, so that the next tile's S is there
+// when a softmax ends, and P V runs under the next softmax.
 //
 // Roles:
-//   warps 0-3, 4-7  softmax of half A, B: a thread owns a row
-//   warp 8          one thread issues S = Q K^T and O += P V (P from TMEM), A and B in turn
-//   warp 9          queries to shared memory
-//   the others      codes to 16 bits (exact: K in the queries' type, V in f16) into
+//   warps 0-3, 4-7  softmax of half A, B: a thread owns a row, and brings its row of
+//                   the next segment's queries to shared memory under the last tile
+//   warps 8, 9      one thread each issues S = Q K^T and O += P V (P from TMEM) of half
+//                   A, B (an issuing thread is slow, some ten instructions to an MMA)
+//   warps 10-13     codes to 16 bits (exact: K in the queries' type, V in f16) into
 //                   128-byte swizzled shared memory; they come two tiles ahead
 //                   by cp.async into a thread's own bytes
 //
@@ -34,9 +35,9 @@
 // the output's step), O = sum p vcode, l = sum p / vs from the unrounded p.  m
 // is raised (and O and l rescaled) only when exceeded by more than 2^8.
 //
-// TMEM columns: S of A 0-63, of B 64-127 (P takes the place of the scores it came
-// from), then O of A and B.  Waits are bounded; one that runs out raises
-// NIE_DEV_ERR_TIMEOUT and ends the CTA.
+// TMEM columns: two S buffers of A 0-127, of B 128-255 (P takes the place of the
+// scores it came from), then O of A and B.  Waits are bounded; one that runs out
+// raises NIE_DEV_ERR_TIMEOUT and ends the CTA.
 #include <algorithm>
 #include <type_traits>
 
@@ -45,8 +46,9 @@
 namespace nie {
 
 constexpr int kF8Rows = 256;
-constexpr int kF8Stages = 3;       // 16-bit key tiles in shared memory
 constexpr int kF8MaxReq = 256;     // requests of one launch
+constexpr int kF8MaxStages = 5;
+constexpr uint32_t kF8OCol = 256;
 constexpr int kF8SegCost = 5;      // a segment's fixed part, in key tiles
 constexpr uint32_t kF8Wait = 1u << 22;
 constexpr float kF8Log2e = 1.4426950408889634f;
@@ -70,31 +72,31 @@ template <int HD>
 struct F8Cfg {
   static constexpr int BN = 64;                           // keys of a tile
   static constexpr int Subs = BN / 16;
-  static constexpr int Ctas = HD == 64 ? 2 : 1;           // per SM
-  static constexpr int Loaders = HD == 64 ? 64 : 128;     // threads
+  static constexpr int Stages = HD == 64 ? 5 : 3;         // 16-bit key tiles in shared memory
+  static constexpr int Loaders = 128;                     // threads
   static constexpr int Threads = 10 * 32 + Loaders;
   static constexpr int QBytes = kF8Rows * HD * 2;
   static constexpr int TileBytes = BN * HD * 2;           // K or V of a tile in 16 bits
   static constexpr int StageBytes = 2 * TileBytes;
   static constexpr int CodeBytes = 2 * BN * HD;           // codes of a tile
-  static constexpr uint32_t Cols = HD == 64 ? 256 : 512;  // TMEM columns
-  static constexpr uint32_t OCol = HD == 64 ? 128 : 256;
 };
 
 // A key tile of a segment: its first in this CTA, its last, with rows in half B; the end of the stretch.
 enum F8Flag { kF8First = 1, kF8Last = 2, kF8Two = 4, kF8End = 8 };
 
 struct F8Bars {
-  uint64_t q_full, q_empty;
-  uint64_t kv_full[kF8Stages], kv_empty[kF8Stages];
-  uint64_t s_full[2], p_full[2], o_full[2], o_free[2];
+  uint64_t q_full[2];
+  uint64_t kv_full[kF8MaxStages], kv_empty[kF8MaxStages];
+  uint64_t s_full[2][2], p_full[2][2];   // of a half's S buffers
+  uint64_t o_done[2];                    // a half's product is done
+  uint64_t o_full[2], o_free[2];         // a segment's last one; its output has been read
   uint64_t done;
   uint32_t tmem_base;
   int abort;
   int start_req, start_tile, start_head;
   int64_t start_pos;
-  int flags[kF8Stages];                  // of a stage's tile: kF8First, ...
-  float4 info[kF8Stages][8];             // of 16 keys: score factor, log2 vs, 1 / vs
+  int flags[kF8MaxStages];                  // of a stage's tile: kF8First, ...
+  float4 info[kF8MaxStages][4];             // of 16 keys: score factor, log2 vs, 1 / vs
   int64_t cum[kF8MaxReq + 1];            // cost before each request
 };
 
@@ -236,22 +238,35 @@ struct F8Walk {
   }
 };
 
-// D[tmem] (+)= A[smem] * B[smem] and A[tmem] * B[smem], kind::f16.
-__device__ __forceinline__ void f8_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+// D[tmem] (+)= A[smem] * B[smem] and A[tmem] * B[smem], kind::f16.  Only the low words
+// of the operands' descriptors differ: 128-byte swizzle, 1024 bytes between groups of 8 rows.
+constexpr uint32_t kF8DescHi = (1024 >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void f8_mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a),
-      "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n.reg .pred p;\n.reg .b64 da, db;\nmov.b64 da, {%1, %5};\nmov.b64 db, {%2, %5};\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "n"(kF8DescHi)
       : "memory");
 }
-__device__ __forceinline__ void f8_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+__device__ __forceinline__ void f8_mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\ntcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a),
-      "l"(b), "r"(idesc), "r"((uint32_t)add)
+      "{\n.reg .pred p;\n.reg .b64 db;\nmov.b64 db, {%2, %5};\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "n"(kF8DescHi)
       : "memory");
 }
+// 32 lanes x 16 consecutive 32-bit columns.
+__device__ __forceinline__ void f8_tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ uint32_t f8_desc(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | ((lbo >> 4) << 16); }
 
 template <int HD, typename T>
-__global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
+__global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
     kv8_prefill_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ F8Plan p) {
   using C = F8Cfg<HD>;
   constexpr int BN = C::BN;
@@ -259,7 +274,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(f8_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = sm;
   uint8_t* skv = sq + C::QBytes;
-  uint8_t* scode = skv + kF8Stages * C::StageBytes;
+  uint8_t* scode = skv + C::Stages * C::StageBytes;
   F8Bars* b = reinterpret_cast<F8Bars*>(scode + 2 * C::CodeBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int R = p.num_req;
@@ -277,19 +292,21 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
   }
   if (threadIdx.x == 0) {
     b->cum[0] = 0;
-    mbar_init(&b->q_full, 32);
-    mbar_init(&b->q_empty, 1);
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&b->s_full[i], 1);
-      mbar_init(&b->p_full[i], 4);
+      mbar_init(&b->q_full[i], 4);
+      for (int u = 0; u < 2; ++u) {
+        mbar_init(&b->s_full[i][u], 1);
+        mbar_init(&b->p_full[i][u], 4);
+      }
+      mbar_init(&b->o_done[i], 1);
       mbar_init(&b->o_full[i], 1);
       mbar_init(&b->o_free[i], 4);
     }
-    for (int s = 0; s < kF8Stages; ++s) {
+    for (int s = 0; s < C::Stages; ++s) {
       mbar_init(&b->kv_full[s], C::Loaders);
-      mbar_init(&b->kv_empty[s], 1);
+      mbar_init(&b->kv_empty[s], 2);
     }
-    mbar_init(&b->done, 1);
+    mbar_init(&b->done, 2);
     b->abort = 0;
     fence_mbar_init();
   }
@@ -344,7 +361,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
     }
   }
   if (warp == 8) {
-    tmem_alloc(&b->tmem_base, C::Cols);
+    tmem_alloc(&b->tmem_base, 512);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -358,6 +375,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
     // ------------------------------------------------------------ loaders
     const int tid = threadIdx.x - 320;
     constexpr int Pass = C::Loaders / 4, Passes = BN / Pass;  // rows of a copy, copies for 64 dims of all rows
+    constexpr int Copies = Passes * HD / 64;                  // of K, and of V
     const int64_t row_bytes = (int64_t)a.hkv * HD;
     const float coef = fabsf(a.scale) * kF8Log2e;
     const uint32_t flip = a.scale < 0.f ? 0x80808080u : 0u;  // a negative scale's sign goes to the keys
@@ -394,7 +412,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
           }
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int j = 0; j < Copies; ++j) {
           const int half = j / Passes;
           const int s = ((tid >> 2) + Pass * (j % Passes)) >> 4, row = (tid >> 2) & 15;  // all of a warp's rows lie in 16 keys
           const int from = __shfl_sync(0xffffffffu, at, s);
@@ -402,7 +420,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
           const int64_t off =
               there ? (int64_t)(from + row) * row_bytes + (int64_t)ahead.h * HD + half * 64 + (tid & 3) * 16 : 0;
           f8_cp16(base + j * (C::Loaders * 16), a.kc + off, there ? 16 : 0);
-          f8_cp16(base + (4 + j) * (C::Loaders * 16), a.vc + off, there ? 16 : 0);
+          f8_cp16(base + (Copies + j) * (C::Loaders * 16), a.vc + off, there ? 16 : 0);
         }
         if (++a_kt >= ahead.t_hi()) {
           ahead.next(a, R);
@@ -430,25 +448,25 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
         uint8_t* dst = skv + st * C::StageBytes;
         const uint8_t* src = scode + slot * C::CodeBytes + tid * 16;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int jj = j & 3;
+        for (int j = 0; j < 2 * Copies; ++j) {
+          const int jj = j % Copies;
           const int row = (tid >> 2) + Pass * (jj % Passes), half = jj / Passes;
           const uint4 x = *reinterpret_cast<const uint4*>(src + j * (C::Loaders * 16));
           uint32_t w[4] = {x.x, x.y, x.z, x.w}, h[8];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            if (j < 4) w[e] ^= flip;
+            if (j < Copies) w[e] ^= flip;
             h[2 * e] = e4m3x2_to_f16x2((uint16_t)(w[e] & 0xffffu));
             h[2 * e + 1] = e4m3x2_to_f16x2((uint16_t)(w[e] >> 16));
           }
-          if (j < 4 && !std::is_same<T, __half>::value) {  // keys meet bf16 queries: 4 bits fit either type
+          if (j < Copies && !std::is_same<T, __half>::value) {  // keys meet bf16 queries: 4 bits fit either type
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
               const float2 f = f16x2_to_float2(h[e]);
               h[e] = pack_bf16x2(f.x, f.y);
             }
           }
-          uint8_t* at = dst + (j >> 2) * C::TileBytes + half * (BN * 128) + row * 128;
+          uint8_t* at = dst + j / Copies * C::TileBytes + half * (BN * 128) + row * 128;
           const int ch = 2 * (tid & 3);
           *reinterpret_cast<uint4*>(at + ((ch ^ (row & 7)) << 4)) = make_uint4(h[0], h[1], h[2], h[3]);
           *reinterpret_cast<uint4*>(at + (((ch + 1) ^ (row & 7)) << 4)) = make_uint4(h[4], h[5], h[6], h[7]);
@@ -466,7 +484,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
         ks0 = ks1, vs0 = vs1, ok0 = ok1;
         fetch(slot, ks1, vs1, ok1);
         slot ^= 1;
-        if (++st == kF8Stages) {
+        if (++st == C::Stages) {
           st = 0;
           par ^= 1u;
         }
@@ -479,167 +497,172 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp == 8) {
-    // --------------------------------------------------------- MMA issuer
-    // One thread.  What it has to know of a key tile stands beside the tile.
+  } else if (warp >= 8) {
+    // -------------------------------------------------------- MMA issuers
+    // One thread for each half.  What it has to know of a key tile stands beside the tile.
     if (lane == 0) {
-      const uint64_t q_desc = smem_desc_sw128(smem_u32(sq), 16, 1024), k_desc = smem_desc_sw128(smem_u32(skv), 16, 1024);
-      const uint64_t v_desc = smem_desc_sw128(smem_u32(skv + C::TileBytes), BN * 128, 1024);
+      const int x = warp - 8;
+      const uint32_t q_desc = f8_desc(smem_u32(sq) + x * (128 * HD * 2), 16);
+      const uint32_t k_desc = f8_desc(smem_u32(skv), 16), v_desc = f8_desc(smem_u32(skv + C::TileBytes), BN * 128);
+      const uint32_t s_col = tbase + x * 128, o_col = tbase + kF8OCol + x * HD;
       constexpr uint32_t id_s = f8_idesc(128, BN, false, !std::is_same<T, __half>::value);
       constexpr uint32_t id_o = f8_idesc(128, HD, true, false);
-      int nx = 0, cur = 0;          // flags of the tile whose scores come next, and of the one before it
-      int nx_st = 0, cur_st = 0;    // their stages
-      uint32_t kv_par = 0, q_par = 0;  // phase parities of nx_st and of the queries
-      int used[2] = {0, 0};         // products of each half
-      int segs[2] = {0, 0};         // segments that wrote its output
+      int flags = 0, st = 0;     // of the tile whose scores come next
+      uint32_t par = 0;          // phase parity of its stage
+      int tiles = 0, done = 0;   // of this half: scores and products issued
+      int segs = 0, outs = 0;    // segments begun, their outputs begun
+      int f0 = 0, f1 = 0, st0 = 0, st1 = 0;  // the tiles between scores and product: the older, the younger
       bool ok = true;
-      auto take = [&]() {  // the flags of the tile in stage nx_st
-        ok = f8_wait(b, &b->kv_full[nx_st], kv_par, a.err);
-        nx = ok ? *reinterpret_cast<volatile int*>(&b->flags[nx_st]) : kF8End;
-        if (ok && (nx & kF8First)) {
-          ok = f8_wait(b, &b->q_full, q_par, a.err);
-          q_par ^= 1u;
+      auto step = [&]() {
+        if (++st == C::Stages) {
+          st = 0;
+          par ^= 1u;
         }
-        tc_fence_after();
       };
-      auto scores = [&](auto half) {  // S of a half for nx
-        constexpr int x = decltype(half)::value;
-        // descriptors count addresses in 16 bytes: steps along a row or to the next 64 dims are added to them
-        const uint64_t q = q_desc + (uint32_t)(x * (128 * HD * 2 / 16));
-        const uint64_t kd = k_desc + (uint32_t)(nx_st * (C::StageBytes / 16));
+      auto take = [&]() {  // the next tile's flags
+        ok = f8_wait(b, &b->kv_full[st], par, a.err);
+        flags = ok ? *reinterpret_cast<volatile int*>(&b->flags[st]) : kF8End;
+      };
+      take();
+      while (ok) {
+        const int open = tiles - done;
+        if (x == 1 && open == 0 && !(flags & (kF8End | kF8Two))) {
+          // a tile without rows of half B: passed over, but not before the products are issued that keep
+          // stages from the loaders
+          mbar_arrive(&b->kv_empty[st]);
+          step();
+          take();
+          continue;
+        }
+        // S = Q K^T, up to two tiles ahead of the products; over the P of the tile before the last,
+        // whose product has been issued: MMAs run in order.  A segment's first tile waits for the
+        // products of the one before (its queries come under their softmax).
+        if (!(flags & kF8End) && (x == 0 || (flags & kF8Two)) && open < 2 && !((flags & kF8First) && open > 0)) {
+          if (flags & kF8First) {
+            ok = f8_wait(b, &b->q_full[x], (uint32_t)segs & 1u, a.err);
+            if (!ok) break;
+            ++segs;
+          }
+          tc_fence_after();
+          const uint32_t kd = k_desc + (uint32_t)(st * (C::StageBytes / 16)), d = s_col + (tiles & 1) * BN;
 #pragma unroll
-        for (int kk = 0; kk < HD / 16; ++kk)
-          f8_mma_ss(tbase + x * BN, q + ((kk >> 2) * (128 * 128 / 16) + (kk & 3) * 2),
-                    kd + ((kk >> 2) * (BN * 128 / 16) + (kk & 3) * 2), id_s, kk > 0);
-        tc_commit(&b->s_full[x]);
-        // the queries are free once the segment's last scores are done
-        if ((nx & kF8Last) && (x == 1 || !(nx & kF8Two))) tc_commit(&b->q_empty);
-      };
-      auto product = [&](auto half) {  // O of a half += P V for cur
-        constexpr int x = decltype(half)::value;
-        ok = f8_wait(b, &b->p_full[x], (uint32_t)(used[x] & 1), a.err);
-        ++used[x];
-        if (ok && (cur & kF8First)) {
-          // the softmax warps have read the half's output of the segment before
-          if (segs[x] > 0) ok = f8_wait(b, &b->o_free[x], (uint32_t)(segs[x] - 1) & 1u, a.err);
-          ++segs[x];
+          for (int kk = 0; kk < HD / 16; ++kk)
+            f8_mma_ss(d, q_desc + ((kk >> 2) * (128 * 128 / 16) + (kk & 3) * 2),
+                      kd + ((kk >> 2) * (BN * 128 / 16) + (kk & 3) * 2), id_s, kk > 0);
+          tc_commit(&b->s_full[x][tiles & 1]);
+          f0 = f1, st0 = st1;
+          f1 = flags, st1 = st;
+          ++tiles;
+          step();
+          take();
+          continue;
         }
-        if (!ok) return;
+        if (open == 0) break;
+        // O += P V of the oldest
+        const int f = open == 2 ? f0 : f1, s = open == 2 ? st0 : st1;
+        ok = f8_wait(b, &b->p_full[x][done & 1], (uint32_t)(done >> 1) & 1u, a.err);
+        if (ok && (f & kF8First)) {
+          // the softmax warps have read the output of the segment before
+          if (outs > 0) ok = f8_wait(b, &b->o_free[x], (uint32_t)(outs - 1) & 1u, a.err);
+          ++outs;
+        }
+        if (!ok) break;
         tc_fence_after();
-        const uint64_t vd = v_desc + (uint32_t)(cur_st * (C::StageBytes / 16));
+        const uint32_t vd = v_desc + (uint32_t)(s * (C::StageBytes / 16)), pc = s_col + (done & 1) * BN;
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          f8_mma_ts(tbase + C::OCol + x * HD, tbase + x * BN + kk * 8, vd + kk * (2048 / 16), id_o, kk > 0 || !(cur & kF8First));
-        if (x == 1 || !(cur & kF8Two)) tc_commit(&b->kv_empty[cur_st]);
-        if (cur & kF8Last) tc_commit(&b->o_full[x]);
-      };
-      constexpr std::integral_constant<int, 0> A{};
-      constexpr std::integral_constant<int, 1> B{};
-      take();
-      if (ok && !(nx & kF8End)) {
-        scores(A);
-        if (nx & kF8Two) scores(B);
-        while (ok) {
-          cur = nx;
-          cur_st = nx_st;
-          if (++nx_st == kF8Stages) {
-            nx_st = 0;
-            kv_par ^= 1u;
-          }
-          product(A);
-          if (ok) take();
-          const bool more = ok && !(nx & kF8End);
-          if (more) scores(A);  // over the P that the product issued before reads: MMAs run in order
-          if (ok && (cur & kF8Two)) product(B);
-          if (ok && more && (nx & kF8Two)) scores(B);
-          if (!more) break;
-        }
+          f8_mma_ts(o_col, pc + kk * 8, vd + kk * (2048 / 16), id_o, kk > 0 || !(f & kF8First));
+        tc_commit(&b->kv_empty[s]);
+        tc_commit(&b->o_done[x]);
+        if (f & kF8Last) tc_commit(&b->o_full[x]);
+        ++done;
       }
       tc_commit(&b->done);
       mbar_wait_bounded(&b->done, 0, kF8Wait);
     }
     __syncwarp();
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ queries
-    constexpr int LPR = HD / 8, RP = 32 / LPR;     // lanes of a row, rows of a copy
-    const int c = lane % LPR;
-    const int dt = RP / a.group, dh = RP % a.group;  // tokens and heads from one of a lane's rows to its next
-    for (int k = 0; seg.valid(); seg.next(a, R), ++k) {
-      if (!f8_wait_idle(b, &b->q_empty, (uint32_t)(k + 1) & 1u, a.err)) break;
-      const int rows = seg.rows();
-      const uint32_t dst = smem_u32(sq) + (c >> 3) * (128 * 128);
-      int row = lane / LPR;
-      int tok = (seg.tile * kF8Rows + row) / a.group, head = (seg.tile * kF8Rows + row) % a.group;
-      const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)seg.x.first * a.q_stride + (int64_t)seg.h * a.group * HD + c * 8;
-      const int last = rows > 128 ? kF8Rows : 128;  // half B without rows is not used
-#pragma unroll 4
-      for (; row < last; row += RP) {  // rows that are not there become zeros
-        const bool there = row < rows;
-        f8_cp16(dst + (row >> 7) * (128 * HD * 2) + (row & 127) * 128 + (((c & 7) ^ (row & 7)) << 4),
-                there ? q + (int64_t)tok * a.q_stride + head * HD : q, there ? 16 : 0);
-        tok += dt;
-        head += dh;
-        if (head >= a.group) {
-          head -= a.group;
-          ++tok;
-        }
-      }
-      asm volatile("cp.async.wait_all;" ::: "memory");
-      fence_proxy_async_smem();
-      mbar_arrive(&b->q_full);
-    }
   } else {
     // ------------------------------------------------------ softmax warps
     const int x = warp >> 2;                       // half
     const int t = (warp & 3) * 32 + lane;          // row of the half, TMEM lane
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_addr = tbase + lane_off + x * BN, o_addr = tbase + lane_off + C::OCol + x * HD;
+    const uint32_t s_base = tbase + lane_off + x * 128, o_addr = tbase + lane_off + kF8OCol + x * HD;
     bool ok = true;
     int st = 0;             // stage of the key tile
     uint32_t kv_par = 0;    // and its phase parity
     int used = 0, segs = 0;
-    for (; ok && seg.valid(); seg.next(a, R)) {
+    // this thread's row of a segment's queries; zeros where there is none
+    auto load_queries = [&]() {
+      const int row = x * 128 + t, rows = seg.valid() ? seg.rows() : 0;
+      if (rows <= x * 128) return;
+      const int fr = seg.tile * kF8Rows + row;
+      const bool there = row < rows;
+      const T* q = reinterpret_cast<const T*>(a.q);
+      if (there) q += (int64_t)(seg.x.first + fr / a.group) * a.q_stride + (int64_t)(seg.h * a.group + fr % a.group) * HD;
+      const uint32_t dst = smem_u32(sq) + x * (128 * HD * 2) + t * 128;
+#pragma unroll
+      for (int c = 0; c < HD / 8; ++c)
+        f8_cp16(dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (t & 7)) << 4), q + c * 8, there ? 16 : 0);
+    };
+    auto queries_there = [&]() {
+      asm volatile("cp.async.wait_all;" ::: "memory");
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&b->q_full[x]);
+    };
+    load_queries();
+    if (seg.valid() && seg.rows() > x * 128) queries_there();
+    while (ok && seg.valid()) {
       const int rows = seg.rows();
       const int tlo = seg.t_lo(), thi = seg.t_hi();
       if (x == 1 && rows <= 128) {  // the half has no rows
         for (int kt = tlo; kt < thi; ++kt)
-          if (++st == kF8Stages) {
+          if (++st == C::Stages) {
             st = 0;
             kv_par ^= 1u;
           }
+        seg.next(a, R);
+        load_queries();
+        if (seg.valid() && seg.rows() > 128) queries_there();
         continue;
       }
       const bool active = x * 128 + (warp & 3) * 32 < rows;  // this warp has rows
       const int fr = seg.tile * kF8Rows + x * 128 + t;
       const int qpos = seg.x.ctx + fr / a.group;              // position of the row's token
       const int first_pos = seg.x.ctx + (fr - lane) / a.group;  // of the warp's first row
+      const bool whole = tlo == 0 && thi == seg.n;
+      T* op = reinterpret_cast<T*>(a.out) + (int64_t)(seg.x.first + fr / a.group) * a.out_stride +
+              (int64_t)(seg.h * a.group + fr % a.group) * HD;
+      if (tlo == 0 && !whole && threadIdx.x == 0)
+        p.cuts[blockIdx.x] = F8Cut{(int64_t)seg.tile * kF8Rows, seg.x.first, rows, seg.h,
+                                   (int)((lo + seg.start + seg.n - 1) / W - blockIdx.x), 0};
       float m_ref = -INFINITY, l = 0.f;
-      // One key tile of the row; MASK: some row of the warp does not see all of it.  Loops of 32 keys that
-      // stay loops: unrolled, the roles' code together outgrows the instruction caches.
-      auto softmax_tile = [&](int kt, auto masked) {
+      // One key tile of the row; MASK: some row of the warp does not see all of it.
+      auto softmax_tile = [&](int kt, auto masked) -> bool {
         constexpr bool MASK = decltype(masked)::value;
         const float4* info = b->info[st];
+        const uint32_t s_addr = s_base + (used & 1) * BN;
         const int seen = min(BN, max(0, qpos - kt * BN + 1));  // keys of the tile that the row sees
-        uint32_t v[32];
+        uint32_t v[BN];
+        tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
+        tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
+        float4 f[C::Subs];
+#pragma unroll
+        for (int u = 0; u < C::Subs; ++u) f[u] = info[u];
+        tmem_wait_ld();
+        if constexpr (MASK) {
+#pragma unroll
+          for (int e = 0; e < BN; ++e)
+            if (e >= seen) v[e] = 0xff800000u;
+        }
         // largest y: per 16 keys the largest score, since their factor is not negative
         float mx = -INFINITY;
-#pragma unroll 1
-        for (int c = 0; c < BN / 32; ++c) {
-          tmem_ld32(s_addr + 32 * c, v);
-          const float4 f0 = info[2 * c], f1 = info[2 * c + 1];
-          tmem_wait_ld();
-          if constexpr (MASK) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (32 * c + e >= seen) v[e] = 0xff800000u;
-          }
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float* s = reinterpret_cast<const float*>(&v[16 * h]);
-            const float s0 = f8_max3(f8_max3(s[0], s[1], s[2]), f8_max3(s[3], s[4], s[5]), f8_max3(s[6], s[7], s[8]));
-            const float s1 = f8_max3(f8_max3(s[9], s[10], s[11]), f8_max3(s[12], s[13], s[14]), s[15]);
-            mx = fmaxf(mx, fmaf(fmaxf(s0, s1), h ? f1.x : f0.x, h ? f1.y : f0.y));
-          }
+        for (int u = 0; u < C::Subs; ++u) {
+          const float* s = reinterpret_cast<const float*>(&v[16 * u]);
+          const float s0 = f8_max3(f8_max3(s[0], s[1], s[2]), f8_max3(s[3], s[4], s[5]), f8_max3(s[6], s[7], s[8]));
+          const float s1 = f8_max3(f8_max3(s[9], s[10], s[11]), f8_max3(s[12], s[13], s[14]), s[15]);
+          mx = fmaxf(mx, fmaf(fmaxf(s0, s1), f[u].x, f[u].y));
         }
         const bool raise = mx > m_ref + kF8Lazy;
         if (__any_sync(0xffffffffu, raise)) {
@@ -648,52 +671,60 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
             l *= keep;
             m_ref = mx;
           }
-          if (kt > tlo) {  // O is complete up to the last tile: these scores were issued after its product
+          if (kt > tlo) {
+            // O must hold the product of the tile before.  These scores were issued after the product of
+            // the tile before that, so o_done has one phase to go at most and its parity is no riddle.
+            if (!__all_sync(0xffffffffu, f8_wait(b, &b->o_done[x], (uint32_t)(used - 1) & 1u, a.err))) return false;
+            tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < HD / 32; ++c) {
-              tmem_ld32(o_addr + 32 * c, v);
+            for (int c = 0; c < HD / 16; ++c) {
+              uint32_t o[16];
+              f8_tmem_ld16(o_addr + 16 * c, o);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
-              tmem_st32(o_addr + 32 * c, v);
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
+              tmem_st16(o_addr + 16 * c, o);
             }
           }
         }
         const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-#pragma unroll 1
+#pragma unroll
         for (int c = 0; c < BN / 32; ++c) {
-          tmem_ld32(s_addr + 32 * c, v);
-          const float4 f0 = info[2 * c], f1 = info[2 * c + 1];
-          tmem_wait_ld();
           uint32_t pk[16];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const float fc = h ? f1.x : f0.x, fb = (h ? f1.y : f0.y) - ref;
+            const int u = 2 * c + h;
+            const float fc = f[u].x, fb = f[u].y - ref;
             float r0 = 0.f, r1 = 0.f;
 #pragma unroll
-            for (int e = 16 * h; e < 16 * h + 16; e += 2) {
+            for (int e = 0; e < 16; e += 2) {
               float y0, y1;
-              f8_fma2(y0, y1, __uint_as_float(v[e]), __uint_as_float(v[e + 1]), fc, fb);
-              if constexpr (MASK) {
-                if (32 * c + e >= seen) y0 = -INFINITY;
-                if (32 * c + e + 1 >= seen) y1 = -INFINITY;
+              f8_fma2(y0, y1, __uint_as_float(v[16 * u + e]), __uint_as_float(v[16 * u + e + 1]), fc, fb);
+              if constexpr (MASK) {  // a factor of 0 made NaN of the masked score
+                if (16 * u + e >= seen) y0 = -INFINITY;
+                if (16 * u + e + 1 >= seen) y1 = -INFINITY;
               }
               const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
               f8_add2(r0, r1, p0, p1);
-              pk[e / 2] = f8_pack(p0, p1);
+              pk[8 * h + e / 2] = f8_pack(p0, p1);
             }
-            l = fmaf(r0 + r1, h ? f1.z : f0.z, l);
+            l = fmaf(r0 + r1, f[u].z, l);
           }
-          tmem_st16(s_addr + 16 * c, pk);  // over scores that were taken
+          tmem_st16(s_addr + 16 * c, pk);  // over scores that are in registers
         }
         tmem_wait_st();
+        return true;
       };
       for (int kt = tlo; kt < thi; ++kt, ++used) {
-        if (!f8_wait(b, &b->s_full[x], (uint32_t)(used & 1), a.err)) {
+        if (!f8_wait(b, &b->s_full[x][used & 1], (uint32_t)(used >> 1) & 1u, a.err)) {
           ok = false;
           break;
         }
         tc_fence_after();
+        if (kt + 1 == thi) {  // the segment's queries are done with: the next one's, under this tile
+          seg.next(a, R);
+          load_queries();
+        }
         if (active) {
           // long since there (the scores came from it): makes the loaders' factors visible
           ok = f8_wait(b, &b->kv_full[st], kv_par, a.err);
@@ -701,27 +732,26 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
             ok = false;
             break;
           }
-          if (kt * BN + BN - 1 > first_pos) softmax_tile(kt, std::true_type{});
-          else softmax_tile(kt, std::false_type{});
+          if (kt * BN + BN - 1 > first_pos) ok = softmax_tile(kt, std::true_type{});
+          else ok = softmax_tile(kt, std::false_type{});
+          if (!ok) break;  // of one mind: the warp voted
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&b->p_full[x]);
-        if (++st == kF8Stages) {
+        if (lane == 0) mbar_arrive(&b->p_full[x][used & 1]);
+        if (++st == C::Stages) {
           st = 0;
           kv_par ^= 1u;
         }
       }
       if (!ok) break;
+      if (seg.valid() && seg.rows() > x * 128) queries_there();
       if (!f8_wait(b, &b->o_full[x], (uint32_t)(segs & 1), a.err)) break;
       ++segs;
       tc_fence_after();
-      const bool whole = tlo == 0 && thi == seg.n;
       const int row = x * 128 + t;
       float* ps = p.partials + (int64_t)(2 * blockIdx.x + (tlo == 0)) * (HD + 2) * kF8Rows + row;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      T* op = reinterpret_cast<T*>(a.out) + (int64_t)(seg.x.first + fr / a.group) * a.out_stride +
-              (int64_t)(seg.h * a.group + fr % a.group) * HD;
       if (active) {
 #pragma unroll
         for (int c = 0; c < HD / 32; ++c) {
@@ -751,16 +781,14 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, F8Cfg<HD>::Ctas)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&b->o_free[x]);
-      if (tlo == 0 && thi < seg.n && threadIdx.x == 0)
-        p.cuts[blockIdx.x] = F8Cut{(int64_t)seg.tile * kF8Rows, seg.x.first, rows, seg.h,
-                                   (int)((lo + seg.start + seg.n - 1) / W - blockIdx.x), 0};
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   }
   tc_fence_before();
   __syncthreads();
   if (warp == 8) {
     tc_fence_after();
-    tmem_dealloc(tbase, C::Cols);
+    tmem_dealloc(tbase, 512);
   }
 }
 
@@ -796,12 +824,10 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const __grid_con
   for (int d = 0; d < HD / 8; ++d) op[d0 + 8 * d] = Num<T>::from_f(O[d] * inv);
 }
 
-static int f8_ctas(int sms, int head_dim) { return sms * (head_dim == 64 ? F8Cfg<64>::Ctas : F8Cfg<128>::Ctas); }
 static size_t f8_cut_bytes(int ctas) { return ((size_t)ctas * sizeof(F8Cut) + 255) & ~size_t(255); }
 
 size_t kv8_prefill_workspace(int sms, int head_dim) {
-  const int ctas = f8_ctas(sms, head_dim);
-  return f8_cut_bytes(ctas) + (size_t)2 * ctas * (head_dim + 2) * kF8Rows * sizeof(float);
+  return f8_cut_bytes(sms) + (size_t)2 * sms * (head_dim + 2) * kF8Rows * sizeof(float);
 }
 
 bool kv8_prefill_takes(int dtype, const Kv8Args& a) {
@@ -814,14 +840,14 @@ bool kv8_prefill_takes(int dtype, const Kv8Args& a) {
 template <int HD, typename T>
 static int launch_prefill(const Kv8Args& a, const F8Plan& p, int sms, cudaStream_t s) {
   using C = F8Cfg<HD>;
-  const size_t smem = 1024 + C::QBytes + (size_t)kF8Stages * C::StageBytes + 2 * C::CodeBytes + sizeof(F8Bars);
+  const size_t smem = 1024 + C::QBytes + (size_t)C::Stages * C::StageBytes + 2 * C::CodeBytes + sizeof(F8Bars);
   auto* kernel = kv8_prefill_kernel<HD, T>;
   const int rc = opt_in_smem(kSmemKv8Prefill + (HD == 128) * 2 + std::is_same<T, __half>::value, (const void*)kernel, smem);
   if (rc != NIE_OK) return rc;
-  kernel<<<sms * C::Ctas, C::Threads, smem, s>>>(a, p);
+  kernel<<<sms, C::Threads, smem, s>>>(a, p);
   const int st = check_launch("kv8_prefill_kernel");
   if (st != NIE_OK) return st;
-  pdl_launch(kv8_prefill_merge_kernel<HD, T>, dim3((unsigned)(sms * C::Ctas), kF8Rows / 32), dim3(256), s, a, p);
+  pdl_launch(kv8_prefill_merge_kernel<HD, T>, dim3((unsigned)sms, kF8Rows / 32), dim3(256), s, a, p);
   return check_launch("kv8_prefill_merge_kernel");
 }
 
@@ -843,7 +869,7 @@ int launch_kv8_prefill(int dtype, const Kv8Args& args, int num_requests, int sms
       }
     }
     p.cuts = (F8Cut*)workspace;
-    p.partials = (float*)((char*)workspace + f8_cut_bytes(f8_ctas(sms, a.hd)));
+    p.partials = (float*)((char*)workspace + f8_cut_bytes(sms));
     int rc;
     if (a.hd == 64) rc = dtype == NIE_DTYPE_F16 ? launch_prefill<64, __half>(a, p, sms, s) : launch_prefill<64, __nv_bfloat16>(a, p, sms, s);
     else rc = dtype == NIE_DTYPE_F16 ? launch_prefill<128, __half>(a, p, sms, s) : launch_prefill<128, __nv_bfloat16>(a, p, sms, s);

@@ -356,3 +356,10 @@ def test_uneven_scales(cuda):
         want, bound = plain.attention(q[:1], kc[1], vc[1], ks[1], vs2[1], tables[0], 100, 100, 64**-0.5)
         for x in (got[:1], rows[:1]):
             assert ((x.double() - want).abs() <= step(BF16) * (want.abs() + bound) + bound).all()
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+def test_varlen_with_many_tiles_to_a_processor(cuda, hd):
+    """More row tiles than processors, whole and nearly empty ones in turn (a request's last tile has few rows)."""
+    run_attention(cuda, BF16, [900, 1300, 700, 513], [257, 513, 321, 513], 16, 4, hd, 16, seed=300 + hd)
+    run_attention(cuda, F16, [70] * 90, [65] * 90, 8, 2, hd, 32, seed=301 + hd)
