@@ -8,36 +8,37 @@
 // warps of its own.
 //
 // Rows.  The query heads of a kv head share its codes, so the rows of a tile are
-// (token, head of the group) pairs in that order: 256 rows of one kv head, two
-// MMA tiles A and B of 128.  A "segment" is one such tile of a request and kv
-// head against all keys that its last token sees.
+// (token, head of the group) pairs in that order, of one kv head, in MMA tiles of
+// 128 ("parts"): four at head_dim 64, two at 128.  A "segment" is one such tile of
+// a request and kv head against all keys that its last token sees.
 //
 // Split.  All segments lie end to end, each weighted as its key tiles plus a
 // fixed part; every CTA takes an equal stretch.  A segment cut by a border leaves
 // (max, sum, unnormalised output) of each part for a merging kernel; which parts
 // and in which order follows from the lengths alone.
 //
-// Latency is what the chain of a row costs (S, its softmax, P V, each waiting for
-// the one before): a half has two S buffers, so that the next tile's S is there
-// when a softmax ends, and P V runs under the next softmax.
+// Latency is what the chain of a row costs (S, its softmax, P V, the next S, each
+// waiting for the one before), so several chains share an SM: four parts at
+// head_dim 64; two at 128, where TMEM holds no more, with two S buffers each, so that
+// the next tile's S is there when a softmax ends.
 //
 // Roles:
-//   warps 0-3, 4-7  softmax of half A, B: a thread owns a row, and brings its row of
-//                   the next segment's queries to shared memory under the last tile
-//   warps 8, 9      one thread each issues S = Q K^T and O += P V (P from TMEM) of half
-//                   A, B (an issuing thread is slow, some ten instructions to an MMA)
-//   warps 10-13     codes to 16 bits (exact: K in the queries' type, V in f16) into
-//                   128-byte swizzled shared memory; they come two tiles ahead
-//                   by cp.async into a thread's own bytes
+//   softmax   four warps a part: a thread owns a row, and brings its row of the
+//             next segment's queries to shared memory under the last tile
+//   issuers   a warp a part, of which one thread issues S = Q K^T and O += P V (P
+//             from TMEM); an issuing thread is slow, some ten instructions to an MMA
+//   loaders   four warps: codes to 16 bits (exact: K in the queries' type, V in
+//             f16) into 128-byte swizzled shared memory; they come two tiles
+//             ahead by cp.async into a thread's own bytes
 //
 // Softmax with scales as in the single-token kernel: y = S c + log2 vs per block
 // of 16 keys, p = 2^(y - m) in f16 for the product (its error of 2^-12 is below
 // the output's step), O = sum p vcode, l = sum p / vs from the unrounded p.  m
 // is raised (and O and l rescaled) only when exceeded by more than 2^8.
 //
-// TMEM columns: two S buffers of A 0-127, of B 128-255 (P takes the place of the
-// scores it came from), then O of A and B.  Waits are bounded; one that runs out
-// raises NIE_DEV_ERR_TIMEOUT and ends the CTA.
+// TMEM columns: the parts' S buffers 0-255 (P takes the place of the scores it
+// came from), their O 256-511.  Waits are bounded; one that runs out raises
+// NIE_DEV_ERR_TIMEOUT and ends the CTA.
 #include <algorithm>
 #include <type_traits>
 
@@ -45,9 +46,8 @@
 
 namespace nie {
 
-constexpr int kF8Rows = 256;
 constexpr int kF8MaxReq = 256;     // requests of one launch
-constexpr int kF8MaxStages = 5;
+constexpr int kF8MaxStages = 4;
 constexpr uint32_t kF8OCol = 256;
 constexpr int kF8SegCost = 5;      // a segment's fixed part, in key tiles
 constexpr uint32_t kF8Wait = 1u << 22;
@@ -64,7 +64,7 @@ struct F8Cut {
 
 struct F8Plan {
   int num_req;
-  float* partials;  // [2 * ctas][2 + hd][256]: a CTA's first segment (cut in front), its last (cut behind)
+  float* partials;  // [2 * ctas][2 + hd][rows of a tile]: a CTA's first segment (cut in front), its last (cut behind)
   F8Cut* cuts;      // [ctas]
 };
 
@@ -72,24 +72,28 @@ template <int HD>
 struct F8Cfg {
   static constexpr int BN = 64;                           // keys of a tile
   static constexpr int Subs = BN / 16;
-  static constexpr int Stages = HD == 64 ? 5 : 3;         // 16-bit key tiles in shared memory
+  static constexpr int Parts = HD == 64 ? 4 : 2;
+  static constexpr int Rows = 128 * Parts;
+  static constexpr int SBufs = HD == 64 ? 1 : 2;          // S buffers of a part
+  static constexpr int Stages = HD == 64 ? 4 : 3;         // 16-bit key tiles in shared memory
   static constexpr int Loaders = 128;                     // threads
-  static constexpr int Threads = 10 * 32 + Loaders;
-  static constexpr int QBytes = kF8Rows * HD * 2;
+  static constexpr int IssueWarp = 4 * Parts, LoadWarp = 5 * Parts;
+  static constexpr int Threads = LoadWarp * 32 + Loaders;
+  static constexpr int PartBytes = 128 * HD * 2;          // queries of a part
   static constexpr int TileBytes = BN * HD * 2;           // K or V of a tile in 16 bits
   static constexpr int StageBytes = 2 * TileBytes;
   static constexpr int CodeBytes = 2 * BN * HD;           // codes of a tile
 };
 
-// A key tile of a segment: its first in this CTA, its last, with rows in half B; the end of the stretch.
-enum F8Flag { kF8First = 1, kF8Last = 2, kF8Two = 4, kF8End = 8 };
+// A key tile of a segment: its first in this CTA, its last; the end of the stretch; above them the parts with rows.
+enum F8Flag { kF8First = 1, kF8Last = 2, kF8End = 4, kF8PartShift = 4 };
 
 struct F8Bars {
-  uint64_t q_full[2];
+  uint64_t q_full[4];
   uint64_t kv_full[kF8MaxStages], kv_empty[kF8MaxStages];
-  uint64_t s_full[2][2], p_full[2][2];   // of a half's S buffers
-  uint64_t o_done[2];                    // a half's product is done
-  uint64_t o_full[2], o_free[2];         // a segment's last one; its output has been read
+  uint64_t s_full[4][2], p_full[4][2];   // of a part's S buffers
+  uint64_t o_done[4];                    // a part's product is done
+  uint64_t o_full[4], o_free[4];         // a segment's last one; its output has been read
   uint64_t done;
   uint32_t tmem_base;
   int abort;
@@ -161,7 +165,6 @@ struct F8Req {
   int ctx;    // keys before its first token (negative: the first tokens see none)
   int n;      // keys
   int trow;
-  int tiles;  // 256-row tiles
 };
 
 __device__ __noinline__ F8Req f8_request(const Kv8Args& a, int i, int32_t* err) {
@@ -179,31 +182,36 @@ __device__ __noinline__ F8Req f8_request(const Kv8Args& a, int i, int32_t* err) 
   x.ctx = (int)rows.keys;
   x.n = max(a.seq_lens[r], 0);
   x.trow = tr;
-  x.tiles = (x.rows + kF8Rows - 1) / kF8Rows;
   return x;
 }
 
-// Keys that the last token of a tile sees, and the tiles of BN keys they fill (at
-// least one: rows that see no key still get their zeros from a masked tile).
-__device__ __forceinline__ int f8_keys(const F8Req& x, int group, int tile) {
-  return max(0, x.ctx + (min(x.rows, (tile + 1) * kF8Rows) - 1) / group + 1);
+// Tiles of a request; keys that the last token of a tile sees, and the tiles of BN
+// keys they fill (at least one: rows that see no key still get their zeros from a
+// masked tile).
+template <class C>
+__device__ __forceinline__ int f8_tiles(const F8Req& x) {
+  return (x.rows + C::Rows - 1) / C::Rows;
 }
-template <int BN>
+template <class C>
+__device__ __forceinline__ int f8_keys(const F8Req& x, int group, int tile) {
+  return max(0, x.ctx + (min(x.rows, (tile + 1) * C::Rows) - 1) / group + 1);
+}
+template <class C>
 __device__ __forceinline__ int f8_key_tiles(int keys) {
-  return max(1, (keys + BN - 1) / BN);
+  return max(1, (keys + C::BN - 1) / C::BN);
 }
 
 // Walks the segments of a CTA's stretch: requests, tiles, kv heads.  Positions
 // are costs from the stretch's beginning; it ends at `hi`.
-template <int BN>
+template <class C>
 struct F8Walk {
   int hi, start;  // start: position of the segment's first key tile (may be negative)
   int i, tile, h, keys, n;
   F8Req x;
 
   __device__ __forceinline__ void load(const Kv8Args& a) {
-    keys = f8_keys(x, a.group, tile);
-    n = f8_key_tiles<BN>(keys);
+    keys = f8_keys<C>(x, a.group, tile);
+    n = f8_key_tiles<C>(keys);
   }
   __device__ __forceinline__ void init(const Kv8Args& a, const F8Bars* b, int64_t lo, int64_t end) {
     hi = (int)(end - lo);
@@ -217,12 +225,12 @@ struct F8Walk {
   __device__ __forceinline__ bool valid() const { return start < hi; }
   __device__ __forceinline__ int t_lo() const { return max(0, -start); }
   __device__ __forceinline__ int t_hi() const { return min(hi - start, n); }
-  __device__ __forceinline__ int rows() const { return min(kF8Rows, x.rows - tile * kF8Rows); }
+  __device__ __forceinline__ int rows() const { return min(C::Rows, x.rows - tile * C::Rows); }
   __device__ __forceinline__ void next(const Kv8Args& a, int num_req) {
     start += n;
     if (++h == a.hkv) {
       h = 0;
-      if (++tile >= x.tiles) {
+      if (++tile >= f8_tiles<C>(x)) {
         tile = 0;
         do {
           if (++i >= num_req) {
@@ -230,7 +238,7 @@ struct F8Walk {
             return;
           }
           x = f8_request(a, i, nullptr);
-        } while (x.tiles == 0);
+        } while (x.rows == 0);
       }
       load(a);
     }
@@ -255,14 +263,6 @@ __device__ __forceinline__ void f8_mma_ts(uint32_t d, uint32_t a, uint32_t b, ui
       "r"(a), "r"(b), "r"(idesc), "r"((uint32_t)add), "n"(kF8DescHi)
       : "memory");
 }
-// 32 lanes x 16 consecutive 32-bit columns.
-__device__ __forceinline__ void f8_tmem_ld16(uint32_t taddr, uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-        "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
-      : "r"(taddr));
-}
 __device__ __forceinline__ uint32_t f8_desc(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | ((lbo >> 4) << 16); }
 
 template <int HD, typename T>
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
   extern __shared__ uint8_t f8_raw[];
   uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(f8_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sq = sm;
-  uint8_t* skv = sq + C::QBytes;
+  uint8_t* skv = sq + C::Parts * C::PartBytes;
   uint8_t* scode = skv + C::Stages * C::StageBytes;
   F8Bars* b = reinterpret_cast<F8Bars*>(scode + 2 * C::CodeBytes);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -285,14 +285,14 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
   for (int i = warp; i < R; i += C::Threads / 32) {
     const F8Req x = f8_request(a, i, blockIdx.x == 0 && lane == 0 ? a.err : nullptr);
     int64_t cost = 0;
-    for (int tile = lane; tile < x.tiles; tile += 32) cost += f8_key_tiles<BN>(f8_keys(x, a.group, tile)) + kF8SegCost;
+    for (int tile = lane; tile < f8_tiles<C>(x); tile += 32) cost += f8_key_tiles<C>(f8_keys<C>(x, a.group, tile)) + kF8SegCost;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) cost += __shfl_xor_sync(0xffffffffu, cost, o);
     if (lane == 0) b->cum[i + 1] = cost * a.hkv;
   }
   if (threadIdx.x == 0) {
     b->cum[0] = 0;
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < C::Parts; ++i) {
       mbar_init(&b->q_full[i], 4);
       for (int u = 0; u < 2; ++u) {
         mbar_init(&b->s_full[i][u], 1);
@@ -304,9 +304,9 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
     }
     for (int s = 0; s < C::Stages; ++s) {
       mbar_init(&b->kv_full[s], C::Loaders);
-      mbar_init(&b->kv_empty[s], 2);
+      mbar_init(&b->kv_empty[s], C::Parts);
     }
-    mbar_init(&b->done, 2);
+    mbar_init(&b->done, C::Parts);
     b->abort = 0;
     fence_mbar_init();
   }
@@ -341,8 +341,9 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
     }
     const F8Req x = f8_request(a, l, nullptr);
     int64_t pos = b->cum[l];
-    for (int t0 = 0; t0 < x.tiles; t0 += 32) {
-      const int64_t c = t0 + lane < x.tiles ? f8_key_tiles<BN>(f8_keys(x, a.group, t0 + lane)) + kF8SegCost : 0;
+    const int tiles = f8_tiles<C>(x);
+    for (int t0 = 0; t0 < tiles; t0 += 32) {
+      const int64_t c = t0 + lane < tiles ? f8_key_tiles<C>(f8_keys<C>(x, a.group, t0 + lane)) + kF8SegCost : 0;
       int64_t v = c * a.hkv;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
       if (lo < pos) break;
     }
   }
-  if (warp == 8) {
+  if (warp == C::IssueWarp) {
     tmem_alloc(&b->tmem_base, 512);
     tmem_relinquish();
   }
@@ -368,19 +369,19 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tbase = b->tmem_base;
-  F8Walk<BN> seg;
+  F8Walk<C> seg;
   seg.init(a, b, lo, hi);
 
-  if (warp >= 10) {
+  if (warp >= C::LoadWarp) {
     // ------------------------------------------------------------ loaders
-    const int tid = threadIdx.x - 320;
+    const int tid = threadIdx.x - C::LoadWarp * 32;
     constexpr int Pass = C::Loaders / 4, Passes = BN / Pass;  // rows of a copy, copies for 64 dims of all rows
     constexpr int Copies = Passes * HD / 64;                  // of K, and of V
     const int64_t row_bytes = (int64_t)a.hkv * HD;
     const float coef = fabsf(a.scale) * kF8Log2e;
     const uint32_t flip = a.scale < 0.f ? 0x80808080u : 0u;  // a negative scale's sign goes to the keys
     // tiles come two ahead: `ahead` walks in front of `seg`
-    F8Walk<BN> ahead = seg;
+    F8Walk<C> ahead = seg;
     int a_kt = ahead.valid() ? ahead.t_lo() : 0;
     // Lane s of each warp looks up the block of the tile's s-th 16 keys, a tile
     // before its codes are fetched; all rows of a warp's copy j lie in 16 keys.
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
                                  : make_float4(0.f, -INFINITY, 0.f, 0.f);
         }
         if (tid == 0)
-          b->flags[st] = (kt == seg.t_lo() ? kF8First : 0) | (kt + 1 == thi ? kF8Last : 0) | (rows > 128 ? kF8Two : 0);
+          b->flags[st] = (kt == seg.t_lo() ? kF8First : 0) | (kt + 1 == thi ? kF8Last : 0) | ((rows + 127) / 128) << kF8PartShift;
         fence_proxy_async_smem();
         mbar_arrive(&b->kv_full[st]);
         ks0 = ks1, vs0 = vs1, ok0 = ok1;
@@ -497,19 +498,19 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
       }
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
-  } else if (warp >= 8) {
+  } else if (warp >= C::IssueWarp) {
     // -------------------------------------------------------- MMA issuers
-    // One thread for each half.  What it has to know of a key tile stands beside the tile.
+    // One thread for each part.  What it has to know of a key tile stands beside the tile.
     if (lane == 0) {
-      const int x = warp - 8;
-      const uint32_t q_desc = f8_desc(smem_u32(sq) + x * (128 * HD * 2), 16);
+      const int x = warp - C::IssueWarp;
+      const uint32_t q_desc = f8_desc(smem_u32(sq) + x * C::PartBytes, 16);
       const uint32_t k_desc = f8_desc(smem_u32(skv), 16), v_desc = f8_desc(smem_u32(skv + C::TileBytes), BN * 128);
-      const uint32_t s_col = tbase + x * 128, o_col = tbase + kF8OCol + x * HD;
+      const uint32_t s_col = tbase + x * (BN * C::SBufs), o_col = tbase + kF8OCol + x * HD;
       constexpr uint32_t id_s = f8_idesc(128, BN, false, !std::is_same<T, __half>::value);
       constexpr uint32_t id_o = f8_idesc(128, HD, true, false);
       int flags = 0, st = 0;     // of the tile whose scores come next
       uint32_t par = 0;          // phase parity of its stage
-      int tiles = 0, done = 0;   // of this half: scores and products issued
+      int tiles = 0, done = 0;   // of this part: scores and products issued
       int segs = 0, outs = 0;    // segments begun, their outputs begun
       int f0 = 0, f1 = 0, st0 = 0, st1 = 0;  // the tiles between scores and product: the older, the younger
       bool ok = true;
@@ -526,30 +527,31 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
       take();
       while (ok) {
         const int open = tiles - done;
-        if (x == 1 && open == 0 && !(flags & (kF8End | kF8Two))) {
-          // a tile without rows of half B: passed over, but not before the products are issued that keep
-          // stages from the loaders
+        const bool mine = (flags >> kF8PartShift) > x;
+        if (open == 0 && !mine && !(flags & kF8End)) {
+          // a tile without rows of this part: passed over, but not before the products are issued that
+          // keep stages from the loaders
           mbar_arrive(&b->kv_empty[st]);
           step();
           take();
           continue;
         }
-        // S = Q K^T, up to two tiles ahead of the products; over the P of the tile before the last,
-        // whose product has been issued: MMAs run in order.  A segment's first tile waits for the
+        // S = Q K^T, as far ahead of the products as there are buffers; over a P whose product has been
+        // issued: MMAs run in order.  A segment's first tile waits for the
         // products of the one before (its queries come under their softmax).
-        if (!(flags & kF8End) && (x == 0 || (flags & kF8Two)) && open < 2 && !((flags & kF8First) && open > 0)) {
+        if (mine && !(flags & kF8End) && open < C::SBufs && !((flags & kF8First) && open > 0)) {
           if (flags & kF8First) {
             ok = f8_wait(b, &b->q_full[x], (uint32_t)segs & 1u, a.err);
             if (!ok) break;
             ++segs;
           }
           tc_fence_after();
-          const uint32_t kd = k_desc + (uint32_t)(st * (C::StageBytes / 16)), d = s_col + (tiles & 1) * BN;
+          const uint32_t kd = k_desc + (uint32_t)(st * (C::StageBytes / 16)), d = s_col + tiles % C::SBufs * BN;
 #pragma unroll
           for (int kk = 0; kk < HD / 16; ++kk)
             f8_mma_ss(d, q_desc + ((kk >> 2) * (128 * 128 / 16) + (kk & 3) * 2),
                       kd + ((kk >> 2) * (BN * 128 / 16) + (kk & 3) * 2), id_s, kk > 0);
-          tc_commit(&b->s_full[x][tiles & 1]);
+          tc_commit(&b->s_full[x][tiles % C::SBufs]);
           f0 = f1, st0 = st1;
           f1 = flags, st1 = st;
           ++tiles;
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
         if (open == 0) break;
         // O += P V of the oldest
         const int f = open == 2 ? f0 : f1, s = open == 2 ? st0 : st1;
-        ok = f8_wait(b, &b->p_full[x][done & 1], (uint32_t)(done >> 1) & 1u, a.err);
+        ok = f8_wait(b, &b->p_full[x][done % C::SBufs], (uint32_t)(done / C::SBufs) & 1u, a.err);
         if (ok && (f & kF8First)) {
           // the softmax warps have read the output of the segment before
           if (outs > 0) ok = f8_wait(b, &b->o_free[x], (uint32_t)(outs - 1) & 1u, a.err);
@@ -568,7 +570,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
         }
         if (!ok) break;
         tc_fence_after();
-        const uint32_t vd = v_desc + (uint32_t)(s * (C::StageBytes / 16)), pc = s_col + (done & 1) * BN;
+        const uint32_t vd = v_desc + (uint32_t)(s * (C::StageBytes / 16)), pc = s_col + done % C::SBufs * BN;
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
           f8_mma_ts(o_col, pc + kk * 8, vd + kk * (2048 / 16), id_o, kk > 0 || !(f & kF8First));
@@ -583,10 +585,10 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
     __syncwarp();
   } else {
     // ------------------------------------------------------ softmax warps
-    const int x = warp >> 2;                       // half
-    const int t = (warp & 3) * 32 + lane;          // row of the half, TMEM lane
+    const int x = warp >> 2;                       // part
+    const int t = (warp & 3) * 32 + lane;          // row of the part, TMEM lane
     const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t s_base = tbase + lane_off + x * 128, o_addr = tbase + lane_off + kF8OCol + x * HD;
+    const uint32_t s_base = tbase + lane_off + x * (BN * C::SBufs), o_addr = tbase + lane_off + kF8OCol + x * HD;
     bool ok = true;
     int st = 0;             // stage of the key tile
     uint32_t kv_par = 0;    // and its phase parity
@@ -595,11 +597,11 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
     auto load_queries = [&]() {
       const int row = x * 128 + t, rows = seg.valid() ? seg.rows() : 0;
       if (rows <= x * 128) return;
-      const int fr = seg.tile * kF8Rows + row;
+      const int fr = seg.tile * C::Rows + row;
       const bool there = row < rows;
       const T* q = reinterpret_cast<const T*>(a.q);
       if (there) q += (int64_t)(seg.x.first + fr / a.group) * a.q_stride + (int64_t)(seg.h * a.group + fr % a.group) * HD;
-      const uint32_t dst = smem_u32(sq) + x * (128 * HD * 2) + t * 128;
+      const uint32_t dst = smem_u32(sq) + x * C::PartBytes + t * 128;
 #pragma unroll
       for (int c = 0; c < HD / 8; ++c)
         f8_cp16(dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (t & 7)) << 4), q + c * 8, there ? 16 : 0);
@@ -615,7 +617,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
     while (ok && seg.valid()) {
       const int rows = seg.rows();
       const int tlo = seg.t_lo(), thi = seg.t_hi();
-      if (x == 1 && rows <= 128) {  // the half has no rows
+      if (rows <= x * 128) {  // the part has no rows
         for (int kt = tlo; kt < thi; ++kt)
           if (++st == C::Stages) {
             st = 0;
@@ -623,46 +625,47 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
           }
         seg.next(a, R);
         load_queries();
-        if (seg.valid() && seg.rows() > 128) queries_there();
+        if (seg.valid() && seg.rows() > x * 128) queries_there();
         continue;
       }
       const bool active = x * 128 + (warp & 3) * 32 < rows;  // this warp has rows
-      const int fr = seg.tile * kF8Rows + x * 128 + t;
+      const int fr = seg.tile * C::Rows + x * 128 + t;
       const int qpos = seg.x.ctx + fr / a.group;              // position of the row's token
       const int first_pos = seg.x.ctx + (fr - lane) / a.group;  // of the warp's first row
       const bool whole = tlo == 0 && thi == seg.n;
       T* op = reinterpret_cast<T*>(a.out) + (int64_t)(seg.x.first + fr / a.group) * a.out_stride +
               (int64_t)(seg.h * a.group + fr % a.group) * HD;
       if (tlo == 0 && !whole && threadIdx.x == 0)
-        p.cuts[blockIdx.x] = F8Cut{(int64_t)seg.tile * kF8Rows, seg.x.first, rows, seg.h,
+        p.cuts[blockIdx.x] = F8Cut{(int64_t)seg.tile * C::Rows, seg.x.first, rows, seg.h,
                                    (int)((lo + seg.start + seg.n - 1) / W - blockIdx.x), 0};
       float m_ref = -INFINITY, l = 0.f;
       // One key tile of the row; MASK: some row of the warp does not see all of it.
       auto softmax_tile = [&](int kt, auto masked) -> bool {
         constexpr bool MASK = decltype(masked)::value;
         const float4* info = b->info[st];
-        const uint32_t s_addr = s_base + (used & 1) * BN;
+        const uint32_t s_addr = s_base + used % C::SBufs * BN;
         const int seen = min(BN, max(0, qpos - kt * BN + 1));  // keys of the tile that the row sees
-        uint32_t v[BN];
-        tmem_ld32(s_addr, *reinterpret_cast<uint32_t(*)[32]>(&v[0]));
-        tmem_ld32(s_addr + 32, *reinterpret_cast<uint32_t(*)[32]>(&v[32]));
-        float4 f[C::Subs];
-#pragma unroll
-        for (int u = 0; u < C::Subs; ++u) f[u] = info[u];
-        tmem_wait_ld();
-        if constexpr (MASK) {
-#pragma unroll
-          for (int e = 0; e < BN; ++e)
-            if (e >= seen) v[e] = 0xff800000u;
-        }
+        // Loops of 32 keys that stay loops: unrolled, the roles' code outgrows the instruction caches.
+        uint32_t v[32];
         // largest y: per 16 keys the largest score, since their factor is not negative
         float mx = -INFINITY;
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; ++c) {
+          tmem_ld32(s_addr + 32 * c, v);
+          const float4 f0 = info[2 * c], f1 = info[2 * c + 1];
+          tmem_wait_ld();
+          if constexpr (MASK) {
 #pragma unroll
-        for (int u = 0; u < C::Subs; ++u) {
-          const float* s = reinterpret_cast<const float*>(&v[16 * u]);
-          const float s0 = f8_max3(f8_max3(s[0], s[1], s[2]), f8_max3(s[3], s[4], s[5]), f8_max3(s[6], s[7], s[8]));
-          const float s1 = f8_max3(f8_max3(s[9], s[10], s[11]), f8_max3(s[12], s[13], s[14]), s[15]);
-          mx = fmaxf(mx, fmaf(fmaxf(s0, s1), f[u].x, f[u].y));
+            for (int e = 0; e < 32; ++e)
+              if (32 * c + e >= seen) v[e] = 0xff800000u;
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const float* s = reinterpret_cast<const float*>(&v[16 * h]);
+            const float s0 = f8_max3(f8_max3(s[0], s[1], s[2]), f8_max3(s[3], s[4], s[5]), f8_max3(s[6], s[7], s[8]));
+            const float s1 = f8_max3(f8_max3(s[9], s[10], s[11]), f8_max3(s[12], s[13], s[14]), s[15]);
+            mx = fmaxf(mx, fmaf(fmaxf(s0, s1), h ? f1.x : f0.x, h ? f1.y : f0.y));
+          }
         }
         const bool raise = mx > m_ref + kF8Lazy;
         if (__any_sync(0xffffffffu, raise)) {
@@ -673,50 +676,53 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
           }
           if (kt > tlo) {
             // O must hold the product of the tile before.  These scores were issued after the product of
-            // the tile before that, so o_done has one phase to go at most and its parity is no riddle.
+            // the tile before that at least, so o_done has one phase to go at most: its parity is no riddle.
             if (!__all_sync(0xffffffffu, f8_wait(b, &b->o_done[x], (uint32_t)(used - 1) & 1u, a.err))) return false;
             tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < HD / 16; ++c) {
-              uint32_t o[16];
-              f8_tmem_ld16(o_addr + 16 * c, o);
+            for (int c = 0; c < HD / 32; ++c) {
+              tmem_ld32(o_addr + 32 * c, v);
               tmem_wait_ld();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-              tmem_st16(o_addr + 16 * c, o);
+              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * keep);
+              tmem_st32(o_addr + 32 * c, v);
             }
           }
         }
         const float ref = m_ref == -INFINITY ? 0.f : m_ref;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < BN / 32; ++c) {
+          tmem_ld32(s_addr + 32 * c, v);
+          const float4 f0 = info[2 * c], f1 = info[2 * c + 1];
+          tmem_wait_ld();
           uint32_t pk[16];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int u = 2 * c + h;
-            const float fc = f[u].x, fb = f[u].y - ref;
+            const float fc = h ? f1.x : f0.x, fb = (h ? f1.y : f0.y) - ref;
             float r0 = 0.f, r1 = 0.f;
 #pragma unroll
-            for (int e = 0; e < 16; e += 2) {
+            for (int e = 16 * h; e < 16 * h + 16; e += 2) {
               float y0, y1;
-              f8_fma2(y0, y1, __uint_as_float(v[16 * u + e]), __uint_as_float(v[16 * u + e + 1]), fc, fb);
-              if constexpr (MASK) {  // a factor of 0 made NaN of the masked score
-                if (16 * u + e >= seen) y0 = -INFINITY;
-                if (16 * u + e + 1 >= seen) y1 = -INFINITY;
+              f8_fma2(y0, y1, __uint_as_float(v[e]), __uint_as_float(v[e + 1]), fc, fb);
+              if constexpr (MASK) {
+                if (32 * c + e >= seen) y0 = -INFINITY;
+                if (32 * c + e + 1 >= seen) y1 = -INFINITY;
               }
               const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
               f8_add2(r0, r1, p0, p1);
-              pk[8 * h + e / 2] = f8_pack(p0, p1);
+              pk[e / 2] = f8_pack(p0, p1);
             }
-            l = fmaf(r0 + r1, f[u].z, l);
+            l = fmaf(r0 + r1, h ? f1.z : f0.z, l);
           }
-          tmem_st16(s_addr + 16 * c, pk);  // over scores that are in registers
+          tmem_st16(s_addr + 16 * c, pk);  // over scores that were taken
         }
         tmem_wait_st();
         return true;
       };
       for (int kt = tlo; kt < thi; ++kt, ++used) {
-        if (!f8_wait(b, &b->s_full[x][used & 1], (uint32_t)(used >> 1) & 1u, a.err)) {
+        // the loaders' factors are there before the scores: waited for while there is time
+        if (!f8_wait(b, &b->kv_full[st], kv_par, a.err) ||
+            !f8_wait(b, &b->s_full[x][used % C::SBufs], (uint32_t)(used / C::SBufs) & 1u, a.err)) {
           ok = false;
           break;
         }
@@ -726,19 +732,13 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
           load_queries();
         }
         if (active) {
-          // long since there (the scores came from it): makes the loaders' factors visible
-          ok = f8_wait(b, &b->kv_full[st], kv_par, a.err);
-          if (!__all_sync(0xffffffffu, ok)) {
-            ok = false;
-            break;
-          }
           if (kt * BN + BN - 1 > first_pos) ok = softmax_tile(kt, std::true_type{});
           else ok = softmax_tile(kt, std::false_type{});
           if (!ok) break;  // of one mind: the warp voted
         }
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&b->p_full[x][used & 1]);
+        if (lane == 0) mbar_arrive(&b->p_full[x][used % C::SBufs]);
         if (++st == C::Stages) {
           st = 0;
           kv_par ^= 1u;
@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
       ++segs;
       tc_fence_after();
       const int row = x * 128 + t;
-      float* ps = p.partials + (int64_t)(2 * blockIdx.x + (tlo == 0)) * (HD + 2) * kF8Rows + row;
+      float* ps = p.partials + (int64_t)(2 * blockIdx.x + (tlo == 0)) * (HD + 2) * C::Rows + row;
       const float inv = l == 0.f ? 0.f : 1.f / l;
       if (active) {
 #pragma unroll
@@ -769,13 +769,13 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
               }
             } else {
 #pragma unroll
-              for (int e = 0; e < 32; ++e) ps[(2 + 32 * c + e) * kF8Rows] = __uint_as_float(o[e]);
+              for (int e = 0; e < 32; ++e) ps[(2 + 32 * c + e) * C::Rows] = __uint_as_float(o[e]);
             }
           }
         }
         if (!whole && row < rows) {
           ps[0] = m_ref;
-          ps[kF8Rows] = l;
+          ps[C::Rows] = l;
         }
       }
       tc_fence_before();
@@ -786,7 +786,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) {
+  if (warp == C::IssueWarp) {
     tc_fence_after();
     tmem_dealloc(tbase, 512);
   }
@@ -801,7 +801,8 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const __grid_con
   const F8Cut cut = p.cuts[blockIdx.x];
   const int row = blockIdx.y * 32 + (threadIdx.x & 31), d0 = threadIdx.x >> 5;
   if (cut.parts == 0 || row >= cut.rows) return;
-  const int64_t size = (int64_t)(HD + 2) * kF8Rows;
+  using C = F8Cfg<HD>;
+  const int64_t size = (int64_t)(HD + 2) * C::Rows;
   // part 0 is the CTA's last segment, the others the first one of the CTAs behind it
   auto part = [&](int k) { return p.partials + (2 * (int64_t)(blockIdx.x + k) + (k == 0)) * size + row; };
   float M = -INFINITY;
@@ -812,9 +813,9 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const __grid_con
   for (int k = 0; k <= cut.parts; ++k) {
     const float* ps = part(k);
     const float f = ps[0] == -INFINITY ? 0.f : fast_exp2(ps[0] - M);
-    L += ps[kF8Rows] * f;
+    L += ps[C::Rows] * f;
 #pragma unroll
-    for (int d = 0; d < HD / 8; ++d) O[d] = fmaf(ps[(2 + d0 + 8 * d) * kF8Rows], f, O[d]);
+    for (int d = 0; d < HD / 8; ++d) O[d] = fmaf(ps[(2 + d0 + 8 * d) * C::Rows], f, O[d]);
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;
   const int64_t fr = cut.row0 + row;
@@ -827,7 +828,8 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(const __grid_con
 static size_t f8_cut_bytes(int ctas) { return ((size_t)ctas * sizeof(F8Cut) + 255) & ~size_t(255); }
 
 size_t kv8_prefill_workspace(int sms, int head_dim) {
-  return f8_cut_bytes(sms) + (size_t)2 * sms * (head_dim + 2) * kF8Rows * sizeof(float);
+  const int rows = head_dim == 64 ? F8Cfg<64>::Rows : F8Cfg<128>::Rows;
+  return f8_cut_bytes(sms) + (size_t)2 * sms * (head_dim + 2) * rows * sizeof(float);
 }
 
 bool kv8_prefill_takes(int dtype, const Kv8Args& a) {
@@ -840,14 +842,14 @@ bool kv8_prefill_takes(int dtype, const Kv8Args& a) {
 template <int HD, typename T>
 static int launch_prefill(const Kv8Args& a, const F8Plan& p, int sms, cudaStream_t s) {
   using C = F8Cfg<HD>;
-  const size_t smem = 1024 + C::QBytes + (size_t)C::Stages * C::StageBytes + 2 * C::CodeBytes + sizeof(F8Bars);
+  const size_t smem = 1024 + (size_t)C::Parts * C::PartBytes + (size_t)C::Stages * C::StageBytes + 2 * C::CodeBytes + sizeof(F8Bars);
   auto* kernel = kv8_prefill_kernel<HD, T>;
   const int rc = opt_in_smem(kSmemKv8Prefill + (HD == 128) * 2 + std::is_same<T, __half>::value, (const void*)kernel, smem);
   if (rc != NIE_OK) return rc;
   kernel<<<sms, C::Threads, smem, s>>>(a, p);
   const int st = check_launch("kv8_prefill_kernel");
   if (st != NIE_OK) return st;
-  pdl_launch(kv8_prefill_merge_kernel<HD, T>, dim3((unsigned)sms, kF8Rows / 32), dim3(256), s, a, p);
+  pdl_launch(kv8_prefill_merge_kernel<HD, T>, dim3((unsigned)sms, C::Rows / 32), dim3(256), s, a, p);
   return check_launch("kv8_prefill_merge_kernel");
 }
 
