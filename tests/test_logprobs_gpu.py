@@ -126,3 +126,15 @@ def test_strided_rows_and_missing_tokens(cuda):
 def test_no_rows(cuda):
     got = ops().token_logprobs(torch.empty(0, 50, device=cuda), torch.empty(0, dtype=torch.int64, device=cuda), top=3)
     assert got.logprobs.shape == (0,) and got.top_ids.shape == (0, 3)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_masks_of_the_lowest_value(cuda, dtype):
+    """Rows masked by the type's lowest value, wholly and in part, some with -inf beside it."""
+    low = torch.finfo(dtype).min
+    x = torch.full((5, 3001), low, dtype=dtype, device=cuda)
+    x[1, 7] = 3.0
+    x[2, ::2] = float("-inf")
+    x[3, 5:] = float("-inf")
+    x[4, 2000:] = 1.0
+    check(x, torch.tensor([3, 7, 11, 4, 2999], device=cuda), 8)
