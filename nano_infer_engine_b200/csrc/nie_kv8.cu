@@ -19,6 +19,11 @@
 // beyond 448 * 2^48 saturate.  Non-finite values are stored as NaN and do not
 // count for the scale.
 //
+// What bounds it: each byte in and out once, some 60 operations to 16 of them, so
+// bandwidth from a few thousand tokens on and latency below.  One kernel does all:
+// some CTAs rotate queries, the others store; rows move in 16-byte pieces and a
+// run of up to 2 pairs of pieces a lane stays in registers between its maximum and its codes.
+//
 // One warp owns a (block, kv head, K or V) and takes the block's runs in turn,
 // as calls of their own would be, so no two warps write one scale or one code
 // and the result does not depend on the order of the warps.
@@ -48,7 +53,9 @@ struct AppendArgs {
 // The block of a token's slot; -1 for a token that is not stored.
 __device__ __forceinline__ int64_t block_of(const AppendArgs& a, int64_t t) {
   const int64_t slot = a.slots[t];
-  return slot < 0 || slot >= a.total_slots ? -1 : slot / a.bs;
+  if (slot < 0 || slot >= a.total_slots) return -1;
+  // a 32-bit division is a fifth of a 64-bit one
+  return slot <= 0xffffffffll ? (int64_t)((uint32_t)slot / (uint32_t)a.bs) : slot / a.bs;
 }
 
 // True if token t (of block >= 0) is the first of its block's stretch: the
@@ -61,13 +68,17 @@ __device__ __forceinline__ bool begins_block(const AppendArgs& a, int64_t t, int
   return true;
 }
 
-// Number of tokens of the run that starts at t: slots that follow one another in one block.
+// Number of tokens of the run that starts at t: slots that follow one another in
+// one block.  Called by a whole warp.
 __device__ __forceinline__ int run_length(const AppendArgs& a, int64_t t, int64_t block) {
   const int64_t slot = a.slots[t];
-  const int64_t most = min(a.tokens - t, (block + 1) * a.bs - slot);
-  int n = 1;
-  while (n < most && a.slots[t + n] == slot + n) ++n;
-  return n;
+  const int most = (int)min(a.tokens - t, (block + 1) * a.bs - slot);
+  for (int n = 0; n < most; n += 32) {
+    const int i = n + (int)(threadIdx.x & 31);
+    const unsigned same = __ballot_sync(0xffffffffu, i < most && a.slots[t + i] == slot + i);
+    if (same != 0xffffffffu) return n + __ffs(~same) - 1;
+  }
+  return most;
 }
 
 // First token of the block's next run behind token t, or -1: tokens without a slot are passed over.
@@ -183,6 +194,249 @@ __global__ void __launch_bounds__(256) append_kv8_kernel(AppendArgs a) {
   }
 }
 
+// ------------------------------------------------ 16-byte variants
+// The same arithmetic for rows whose halves are whole 16-byte pieces at 16-byte
+// boundaries, and head_dim a multiple of 16 (that of the codes' pieces).
+template <typename T>
+struct Piece {
+  static constexpr int V = 16 / (int)sizeof(T);
+  float f[V];
+  __device__ __forceinline__ void load(const T* p) {
+    const uint4 u = *reinterpret_cast<const uint4*>(p);
+    const T* e = reinterpret_cast<const T*>(&u);
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = Num<T>::to_f(e[i]);
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    uint4 u;
+    T* e = reinterpret_cast<T*>(&u);
+#pragma unroll
+    for (int i = 0; i < V; ++i) e[i] = Num<T>::from_f(f[i]);
+    *reinterpret_cast<uint4*>(p) = u;
+  }
+  // V codes of f / s; s a power of two: f * inv is the quotient
+  __device__ __forceinline__ void store_codes(uint8_t* p, float s, float inv) const {
+    uint16_t c[V / 2];
+#pragma unroll
+    for (int i = 0; i < V / 2; ++i)
+      c[i] = inv != 0.f ? floats_to_e4m3x2(f[2 * i] * inv, f[2 * i + 1] * inv) : floats_to_e4m3x2(f[2 * i] / s, f[2 * i + 1] / s);
+    if constexpr (V == 8) *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(c);
+    else *reinterpret_cast<uint32_t*>(p) = *reinterpret_cast<const uint32_t*>(c);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void rotate_pieces(Piece<T>& a, Piece<T>& b, const Piece<T>& c, const Piece<T>& s) {
+#pragma unroll
+  for (int i = 0; i < Piece<T>::V; ++i) {
+    const float x = a.f[i], y = b.f[i];
+    a.f[i] = __fsub_rn(__fmul_rn(x, c.f[i]), __fmul_rn(y, s.f[i]));
+    b.f[i] = __fadd_rn(__fmul_rn(y, c.f[i]), __fmul_rn(x, s.f[i]));
+  }
+}
+
+// settle_scale() with 16 codes a lane.
+__device__ __forceinline__ float settle_scale_vec(const AppendArgs& a, int kv, int64_t block, int head, int off, float amax,
+                                                  int lane) {
+  float* sp = a.scales[kv] + block * a.hkv + head;
+  float s = scale_for(amax);
+  if (off > 0) {
+    const float old = fminf(fmaxf(*sp, kScaleMin), kScaleMax);
+    if (s > old) {
+      const float ratio = old / s;
+      const int64_t row = (int64_t)a.hkv * a.hd;
+      const int per_row = a.hd / 16;
+      uint8_t* base = a.codes[kv] + block * a.bs * row + (int64_t)head * a.hd;
+      for (int i = lane; i < off * per_row; i += 32) {
+        uint4* p = reinterpret_cast<uint4*>(base + (int64_t)(i / per_row) * row + i % per_row * 16);
+        uint4 u = *p;
+        uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 lo = f16x2_to_float2(e4m3x2_to_f16x2((uint16_t)(w[e] & 0xffffu)));
+          const float2 hi = f16x2_to_float2(e4m3x2_to_f16x2((uint16_t)(w[e] >> 16)));
+          w[e] = (uint32_t)floats_to_e4m3x2(lo.x * ratio, lo.y * ratio) |
+                 ((uint32_t)floats_to_e4m3x2(hi.x * ratio, hi.y * ratio) << 16);
+        }
+        *p = u;
+      }
+    } else {
+      s = old;
+    }
+  }
+  __syncwarp();
+  if (lane == 0) *sp = s;
+  return s;
+}
+
+constexpr int kQHeads = 4;  // query heads that a thread rotates with one piece of sin and cos
+
+// CTAs [0, kv_ctas): `tile` tokens each and K (even) or V (odd), the heads of whose
+// blocks the warps take in turn; first, since theirs is the longer chain of loads.
+// The others: a thread rotates one pair of pieces of kQHeads heads of a token.
+template <typename T>
+__global__ void __launch_bounds__(256, 4) append_kv8_vec_kernel(const __grid_constant__ AppendArgs a, int kv_ctas, int tile) {
+  constexpr int V = Piece<T>::V, KEEP = 2;
+  pdl_wait();     // dependent launch: q/k/v come from the projection before
+  pdl_trigger();  // the kernel after this one may start its prologue
+  const int half = a.hd / 2, per_half = half / V;
+  const T* sn = reinterpret_cast<const T*>(a.sin);
+  const T* cs = reinterpret_cast<const T*>(a.cos);
+  if ((int)blockIdx.x >= kv_ctas) {
+    const int sets = (a.hq + kQHeads - 1) / kQHeads, per_token = per_half * sets;
+    const int64_t x = (int64_t)(blockIdx.x - kv_ctas) * 256 + threadIdx.x;
+    const int64_t t = x <= 0xffffffffll ? (int64_t)((uint32_t)x / (uint32_t)per_token) : x / per_token;
+    if (t >= a.tokens) return;
+    const int e = (int)(x - t * per_token);
+    const int c = e % per_half * V, h0 = e / per_half * kQHeads;
+    const T* q = reinterpret_cast<const T*>(a.q) + t * a.q_stride + (int64_t)h0 * a.hd + c;
+    T* out = reinterpret_cast<T*>(a.q_out) + (t * a.hq + h0) * a.hd + c;
+    Piece<T> lo[kQHeads], hi[kQHeads], co, si;
+    co.load(cs + t * half + c);
+    si.load(sn + t * half + c);
+#pragma unroll
+    for (int h = 0; h < kQHeads; ++h) {
+      if (h0 + h < a.hq) {
+        lo[h].load(q + h * a.hd);
+        hi[h].load(q + h * a.hd + half);
+      }
+    }
+#pragma unroll
+    for (int h = 0; h < kQHeads; ++h) {
+      if (h0 + h < a.hq) {
+        rotate_pieces(lo[h], hi[h], co, si);
+        lo[h].store(out + h * a.hd);
+        hi[h].store(out + h * a.hd + half);
+      }
+    }
+    return;
+  }
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int kv = blockIdx.x & 1;
+  const int64_t t0 = (int64_t)(blockIdx.x >> 1) * tile;
+  // the tile's tokens at which a block begins
+  int64_t my_block = -1;
+  bool begins = false;
+  if (lane < tile && t0 + lane < a.tokens) {
+    my_block = block_of(a, t0 + lane);
+    if (my_block < 0 && kv == 0 && a.slots[t0 + lane] >= a.total_slots) raise_flag(a.err, NIE_DEV_ERR_SLOT_RANGE);
+    begins = my_block >= 0 && begins_block(a, t0 + lane, my_block);
+  }
+  const unsigned heads = __ballot_sync(0xffffffffu, begins);
+  const int tasks = __popc(heads) * a.hkv;
+  const int row_lanes = per_half, rows = 32 / row_lanes;  // lanes of a row, rows of a pass
+  const int c = lane % row_lanes * V, sub = lane / row_lanes;
+  const bool in = sub < rows;  // row_lanes need not divide 32
+  const int64_t row = (int64_t)a.hkv * a.hd;
+  for (int task = warp; task < tasks; task += 8) {
+    const int which = (int)__fns(heads, 0, task / a.hkv + 1);
+    const int64_t block = __shfl_sync(0xffffffffu, my_block, which);
+    const int head = task % a.hkv;
+    const bool rotate = kv == 0 && a.sin != nullptr;
+    const T* src = reinterpret_cast<const T*>(kv ? a.v : a.k) + (int64_t)head * a.hd + c;
+    const int64_t stride = kv ? a.v_stride : a.k_stride;
+    for (int64_t first = t0 + which; first >= 0;) {
+      const int n = run_length(a, first, block);
+      const int off = (int)(a.slots[first] - block * a.bs);
+      auto get = [&](int j, Piece<T>& lo, Piece<T>& hi) {
+        lo.load(src + (first + j) * stride);
+        hi.load(src + (first + j) * stride + half);
+        if (rotate) {
+          Piece<T> co, si;
+          co.load(cs + (first + j) * half + c);
+          si.load(sn + (first + j) * half + c);
+          rotate_pieces(lo, hi, co, si);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          lo.f[i] = finite_or_nan(lo.f[i]);
+          hi.f[i] = finite_or_nan(hi.f[i]);
+        }
+      };
+      Piece<T> lo[KEEP], hi[KEEP];
+      float amax = 0.f;
+      auto largest = [&](const Piece<T>& p, const Piece<T>& q) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) amax = fmaxf(amax, fmaxf(fabsf(p.f[i]), fabsf(q.f[i])));  // skips NaN
+      };
+#pragma unroll
+      for (int u = 0; u < KEEP; ++u) {
+        const int j = u * rows + sub;
+        if (in && j < n) {
+          get(j, lo[u], hi[u]);
+          largest(lo[u], hi[u]);
+        }
+      }
+      for (int j = KEEP * rows + sub; in && j < n; j += rows) {
+        Piece<T> p, q;
+        get(j, p, q);
+        largest(p, q);
+      }
+      const float s = settle_scale_vec(a, kv, block, head, off, warp_max(amax), lane);
+      const uint32_t bits = __float_as_uint(s);
+      const float inv = (bits & 0x7fffffu) == 0 ? __uint_as_float((254u << 23) - bits) : 0.f;
+      uint8_t* dst = a.codes[kv] + (block * a.bs + off) * row + (int64_t)head * a.hd + c;
+      auto put = [&](int j, const Piece<T>& p, const Piece<T>& q) {
+        p.store_codes(dst + j * row, s, inv);
+        q.store_codes(dst + j * row + half, s, inv);
+      };
+#pragma unroll
+      for (int u = 0; u < KEEP; ++u) {
+        const int j = u * rows + sub;
+        if (in && j < n) put(j, lo[u], hi[u]);
+      }
+      for (int j = KEEP * rows + sub; in && j < n; j += rows) {
+        Piece<T> p, q;
+        get(j, p, q);
+        put(j, p, q);
+      }
+      __syncwarp();
+      first = next_run(a, first + n, block);
+    }
+  }
+}
+
+// Values of a table's first n tokens, 16 of K or V to a thread.
+template <typename T>
+__global__ void __launch_bounds__(256) gather_kv8_vec_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
+                                                             const float* __restrict__ ks, const float* __restrict__ vs,
+                                                             int64_t nb, int bs, int hkv, int hd,
+                                                             const int32_t* __restrict__ table, int64_t n,
+                                                             T* __restrict__ ok, T* __restrict__ ov,
+                                                             int32_t* __restrict__ err) {
+  const int per_head = hd / 16, per_row = hkv * per_head;
+  const int64_t x = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t t = x / per_row;
+  if (t >= n) return;
+  const int e = (int)(x % per_row), head = e / per_head;
+  const int64_t block = table[t / bs];
+  const bool there = block >= 0 && block < nb;
+  if (!there) raise_flag(err, NIE_DEV_ERR_BLOCK_RANGE);
+  const int64_t at = ((there ? block * bs + t % bs : 0) * per_row + e) * 16;
+  const int64_t scale_at = (there ? block : 0) * hkv + head;
+  const uint4 raw[2] = {*reinterpret_cast<const uint4*>(kc + at), *reinterpret_cast<const uint4*>(vc + at)};
+  const float scale[2] = {ks[scale_at], vs[scale_at]};
+#pragma unroll
+  for (int kv = 0; kv < 2; ++kv) {
+    const uint32_t w[4] = {raw[kv].x, raw[kv].y, raw[kv].z, raw[kv].w};
+    float f[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 p = f16x2_to_float2(e4m3x2_to_f16x2((uint16_t)(w[i / 2] >> (16 * (i & 1)))));
+      f[2 * i] = there ? p.x * scale[kv] : 0.f;
+      f[2 * i + 1] = there ? p.y * scale[kv] : 0.f;
+    }
+    T* out = (kv ? ov : ok) + x * 16;
+#pragma unroll
+    for (int i = 0; i < 16; i += Piece<T>::V) {
+      Piece<T> p;
+#pragma unroll
+      for (int u = 0; u < Piece<T>::V; ++u) p.f[u] = f[i + u];
+      p.store(out + i);
+    }
+  }
+}
+
 // Values of a table's first T tokens, one element per thread and step.
 template <typename T>
 __global__ void __launch_bounds__(256) gather_kv8_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
@@ -209,8 +463,25 @@ __global__ void __launch_bounds__(256) gather_kv8_kernel(const uint8_t* __restri
   }
 }
 
+static bool at16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
 template <typename T>
 static void launch_append(const AppendArgs& a, cudaStream_t s) {
+  constexpr int V = Piece<T>::V;
+  if (a.hd % 16 == 0 && a.hd / 2 % V == 0 && a.hd / 2 / V <= 32 && a.k_stride % V == 0 && a.v_stride % V == 0 &&
+      (!a.q || a.q_stride % V == 0) && at16(a.q) && at16(a.k) && at16(a.v) && at16(a.sin) && at16(a.cos) && at16(a.q_out) &&
+      at16(a.codes[0]) && at16(a.codes[1])) {
+    const int64_t threads = a.q ? a.tokens * (a.hd / 2 / V) * ((a.hq + kQHeads - 1) / kQHeads) : 0;
+    const int64_t q_ctas = (threads + 255) / 256;
+    // Few tokens are likely to lie in as many blocks: one to a CTA.  Many are prompts, whose 16 neighbours
+    // share one or two blocks: 16384 tokens in 5 requests take 29 us with 16 to a CTA, 36 us with one.
+    const int tile = a.tokens <= 2048 ? 1 : 16;
+    const int64_t kv_ctas = 2 * ((a.tokens + tile - 1) / tile);
+    if (q_ctas + kv_ctas < (int64_t(1) << 31)) {
+      pdl_launch(append_kv8_vec_kernel<T>, dim3((unsigned)(q_ctas + kv_ctas)), dim3(256), s, a, (int)kv_ctas, tile);
+      return;
+    }
+  }
   pdl_launch(append_kv8_kernel<T>, dim3((unsigned)a.tokens), dim3(256), s, a);
 }
 
@@ -295,6 +566,26 @@ extern "C" int nie_gather_kv8(const void* key_cache, const void* value_cache, co
   const uint8_t* vc = (const uint8_t*)value_cache + codes;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int64_t n = num_tokens * kv_heads * head_dim;
+  const int64_t pieces = n / 16;
+  if (head_dim % 16 == 0 && at16(kc) && at16(vc) && at16(out_keys) && at16(out_values) && pieces < (int64_t(1) << 38)) {
+    const unsigned ctas = (unsigned)((pieces + 255) / 256);
+    const float *sk = key_scales + scales, *sv = value_scales + scales;
+    switch (out_dtype) {
+      case NIE_DTYPE_BF16:
+        gather_kv8_vec_kernel<<<ctas, 256, 0, s>>>(kc, vc, sk, sv, num_blocks, block_size, kv_heads, head_dim, block_table,
+                                                   num_tokens, (__nv_bfloat16*)out_keys, (__nv_bfloat16*)out_values, err_flag);
+        break;
+      case NIE_DTYPE_F32:
+        gather_kv8_vec_kernel<<<ctas, 256, 0, s>>>(kc, vc, sk, sv, num_blocks, block_size, kv_heads, head_dim, block_table,
+                                                   num_tokens, (float*)out_keys, (float*)out_values, err_flag);
+        break;
+      default:
+        gather_kv8_vec_kernel<<<ctas, 256, 0, s>>>(kc, vc, sk, sv, num_blocks, block_size, kv_heads, head_dim, block_table,
+                                                   num_tokens, (__half*)out_keys, (__half*)out_values, err_flag);
+        break;
+    }
+    return check_launch("gather_kv8_vec_kernel");
+  }
   const unsigned grid = (unsigned)std::min<int64_t>((n + 255) / 256, 148 * 32);
   switch (out_dtype) {
     case NIE_DTYPE_BF16:
