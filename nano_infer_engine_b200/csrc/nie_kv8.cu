@@ -314,15 +314,20 @@ __global__ void __launch_bounds__(256, 4) append_kv8_vec_kernel(const __grid_con
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int kv = blockIdx.x & 1;
   const int64_t t0 = (int64_t)(blockIdx.x >> 1) * tile;
-  // the tile's tokens at which a block begins
-  int64_t my_block = -1;
-  bool begins = false;
-  if (lane < tile && t0 + lane < a.tokens) {
-    my_block = block_of(a, t0 + lane);
-    if (my_block < 0 && kv == 0 && a.slots[t0 + lane] >= a.total_slots) raise_flag(a.err, NIE_DEV_ERR_SLOT_RANGE);
-    begins = my_block >= 0 && begins_block(a, t0 + lane, my_block);
+  // Lane i looks at token t0 - 1 + i, so that the tile's blocks and the runs at their
+  // beginnings (16 tokens at least) follow from one load.
+  const int64_t seen = t0 - 1 + lane;
+  int64_t my_slot = -1, my_block = -1;
+  if (seen >= 0 && seen < a.tokens) {
+    my_slot = a.slots[seen];
+    my_block = block_of(a, seen);
+    if (lane >= 1 && lane <= tile && kv == 0 && my_slot >= a.total_slots) raise_flag(a.err, NIE_DEV_ERR_SLOT_RANGE);
   }
-  const unsigned heads = __ballot_sync(0xffffffffu, begins);
+  const int64_t before_slot = __shfl_up_sync(0xffffffffu, my_slot, 1), before_block = __shfl_up_sync(0xffffffffu, my_block, 1);
+  bool begins = lane >= 1 && lane <= tile && my_block >= 0;
+  if (begins && seen > 0) begins = before_block >= 0 ? before_block != my_block : begins_block(a, seen, my_block);
+  const unsigned heads = __ballot_sync(0xffffffffu, begins) >> 1;  // bit i: token t0 + i
+  const unsigned goes_on = __ballot_sync(0xffffffffu, lane >= 1 && my_block >= 0 && my_block == before_block && my_slot == before_slot + 1);
   const int tasks = __popc(heads) * a.hkv;
   const int row_lanes = per_half, rows = 32 / row_lanes;  // lanes of a row, rows of a pass
   const int c = lane % row_lanes * V, sub = lane / row_lanes;
@@ -330,14 +335,20 @@ __global__ void __launch_bounds__(256, 4) append_kv8_vec_kernel(const __grid_con
   const int64_t row = (int64_t)a.hkv * a.hd;
   for (int task = warp; task < tasks; task += 8) {
     const int which = (int)__fns(heads, 0, task / a.hkv + 1);
-    const int64_t block = __shfl_sync(0xffffffffu, my_block, which);
+    const int64_t block = __shfl_sync(0xffffffffu, my_block, which + 1);
     const int head = task % a.hkv;
     const bool rotate = kv == 0 && a.sin != nullptr;
     const T* src = reinterpret_cast<const T*>(kv ? a.v : a.k) + (int64_t)head * a.hd + c;
     const int64_t stride = kv ? a.v_stride : a.k_stride;
+    // the first run from the lanes, and whether another one can follow it in the block
+    const unsigned stops = ~goes_on >> (which + 1) & ~1u;
+    int n = stops ? __ffs(stops) - 1 : 32;
+    const bool known = which + 1 + n < 32;
+    int off = (int)(__shfl_sync(0xffffffffu, my_slot, which + 1) - block * a.bs);
+    const int64_t behind = __shfl_sync(0xffffffffu, my_block, known ? which + 1 + n : 0);
+    const bool alone = known && (t0 + which + n >= a.tokens || (behind >= 0 && behind != block));
+    if (!known) n = run_length(a, t0 + which, block);
     for (int64_t first = t0 + which; first >= 0;) {
-      const int n = run_length(a, first, block);
-      const int off = (int)(a.slots[first] - block * a.bs);
       auto get = [&](int j, Piece<T>& lo, Piece<T>& hi) {
         lo.load(src + (first + j) * stride);
         hi.load(src + (first + j) * stride + half);
@@ -390,8 +401,13 @@ __global__ void __launch_bounds__(256, 4) append_kv8_vec_kernel(const __grid_con
         get(j, p, q);
         put(j, p, q);
       }
+      if (alone) break;
       __syncwarp();
       first = next_run(a, first + n, block);
+      if (first >= 0) {
+        n = run_length(a, first, block);
+        off = (int)(a.slots[first] - block * a.bs);
+      }
     }
   }
 }
