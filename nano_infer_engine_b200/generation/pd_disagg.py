@@ -238,6 +238,8 @@ class RemotePool:
 
 
 def export_pool(cache: PagedKVCache) -> dict:
+    if cache.quantized:
+        raise ValueError("8-bit caches are not handed over between processes (their scales have no place in the protocol)")
     kh, ko = ops.ipc_export(cache.keys)
     vh, vo = ops.ipc_export(cache.values)
     return {

@@ -33,7 +33,7 @@ from .paged_prefill import _validate_paged_prefill_inputs, paged_prefill, paged_
 # (what must agree, test) for a model and the pool it runs on
 _PAIRING = (
     ("be on the same device", lambda m, c: m.embed.weight.device == c.keys.device),
-    ("have the same dtype", lambda m, c: m.embed.weight.dtype == c.keys.dtype),
+    ("have the same dtype", lambda m, c: m.embed.weight.dtype == c.keys.dtype or getattr(c, "quantized", False)),
     ("have the same layer count", lambda m, c: len(m.decoders) == c.num_layers),
     ("have the same KV head count", lambda m, c: m.config.kv_head_num == c.kv_head_num),
     ("have the same head dimension", lambda m, c: m.config.head_dim == c.head_dim),

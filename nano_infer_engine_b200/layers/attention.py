@@ -119,6 +119,9 @@ class GroupedQueryAttention(nn.Module):
             q = self.q_proj(x)
             k = self.k_proj(x)
             v = self.v_proj(x)
+        if cache.quantized:
+            return ops.rope_write_kv8(q, k, v, sin, cos, cache.keys, cache.values, cache.key_scales, cache.value_scales,
+                                      layer_index, meta.slot_mapping, self.q_head_num)
         return ops.rope_write_kv(q, k, v, sin, cos, cache.keys, cache.values, layer_index, meta.slot_mapping,
                                  self.q_head_num)
 
@@ -140,6 +143,9 @@ class GroupedQueryAttention(nn.Module):
         T = x.shape[0]
         q = self.rotate_and_store(x, meta, cache, layer_index, sin, cos)
         out = torch.empty_like(q)
+        if cache.quantized:
+            self._attend_kv8(q, out, meta, cache, layer_index)
+            return apply_linear(self.o_proj, out.view(T, self.hidden_size))
         if meta.num_decode:
             ops.paged_decode(
                 q,
@@ -173,6 +179,40 @@ class GroupedQueryAttention(nn.Module):
             )
         # out comes from the attention (or its combine) kernel just before: it does not write weights
         return apply_linear(self.o_proj, out.view(T, self.hidden_size), overlap=True)
+
+    def _attend_kv8(
+        self, q: torch.Tensor, out: torch.Tensor, meta: ops.RaggedMeta, cache: PagedKVCache, layer_index: int
+    ) -> None:
+        """The decode and varlen attention of :meth:`attend` over an 8-bit cache."""
+        tensors = (cache.keys, cache.values, cache.key_scales, cache.value_scales)
+        if meta.num_decode:
+            ops.paged_decode_kv8(
+                q,
+                *tensors,
+                layer_index,
+                meta.block_tables,
+                meta.seq_lens,
+                out=out,
+                table_rows=meta.table_rows,
+                q_rows=meta.query_start_loc,
+                req_list=meta.decode_list,
+                num_requests=meta.num_decode,
+                overlap=True,  # follows the RoPE + KV append; the metadata comes from the packing kernel
+            )
+        if meta.num_prefill:
+            ops.varlen_attention_kv8(
+                q,
+                *tensors,
+                layer_index,
+                meta.block_tables,
+                meta.seq_lens,
+                meta.query_start_loc,
+                meta.max_query_len,
+                out=out,
+                table_rows=meta.table_rows,
+                req_list=meta.prefill_list,
+                num_requests=meta.num_prefill,
+            )
 
     # ---------------------------------------------------- reference entry
     def forward(

@@ -240,7 +240,8 @@ class Llama3_2(nn.Module):
         x = ops.embed_rows(input_ids, table) if ops.embed_eligible(table) else self.embed(input_ids)
         positions = meta.positions if rope_positions is None else rope_positions
         sin, cos = self.rope.sin_cos(positions, x.dtype)
-        ext = ops.layer_loop_ext() if (self.native_layer_loop and x.is_cuda) else None
+        # an 8-bit cache is served by the Python loop
+        ext = ops.layer_loop_ext() if (self.native_layer_loop and x.is_cuda and not cache.quantized) else None
         layer_args = self._layer_loop_args(x.dtype) if ext is not None else None
         if layer_args is not None:
             normed = self._run_layers_native(ext, layer_args, x, meta, cache, sin, cos, logit_rows)

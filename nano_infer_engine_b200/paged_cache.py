@@ -16,6 +16,13 @@ what changes is where the data moves:
   when the pools are on different GPUs), the P/D handoff of
   nano_infer_engine/generation/pd_scheduler.py:144-145 (export_sequence
   then import_sequence) without the intermediate stacked tensor.
+
+A cache of dtype ``torch.float8_e4m3fn`` holds 8-bit codes and one fp32 scale
+per layer, block and kv head (``key_scales`` / ``value_scales``; no reference
+counterpart): half the bytes of a bf16 cache.  Keys and values are given in the
+activation's dtype; ``gather`` returns values; the model appends and attends
+with the 8-bit kernels (``ops.rope_write_kv8``, ``ops.paged_decode_kv8``,
+``ops.varlen_attention_kv8``).
 """
 
 from __future__ import annotations
@@ -51,6 +58,8 @@ class PagedKVTransfer:
     head_dim: int
     keys: torch.Tensor
     values: torch.Tensor
+    key_scales: torch.Tensor | None = None  # [layers, blocks, kv heads] of an 8-bit cache
+    value_scales: torch.Tensor | None = None
 
 
 class PagedKVCache:
@@ -89,9 +98,18 @@ class PagedKVCache:
         self._block_tables: dict[str, list[int]] = {}
         self._sequence_lengths: dict[str, int] = {}
 
+        self.quantized = dtype == ops.KV8_DTYPE
+        if self.quantized and head_dim % 2:
+            raise ValueError("an 8-bit cache needs an even head_dim")
         shape = (num_layers, num_blocks, block_size, kv_head_num, head_dim)
         self.keys = torch.empty(shape, dtype=dtype, device=device)
         self.values = torch.empty(shape, dtype=dtype, device=device)
+        self.key_scales: torch.Tensor | None = None
+        self.value_scales: torch.Tensor | None = None
+        if self.quantized:
+            self.key_scales, self.value_scales = (
+                torch.zeros((num_layers, num_blocks, kv_head_num), dtype=torch.float32, device=device) for _ in range(2)
+            )
 
         # device block-table mirror: sequence -> row
         self._rows: dict[str, int] = {}
@@ -280,16 +298,30 @@ class PagedKVCache:
             raise ValueError("keys and values must contain at least one token")
         if kv_head_num != self.kv_head_num or head_dim != self.head_dim:
             raise ValueError("keys and values must match the cache KV head count and head dimension")
-        if keys.dtype != self.keys.dtype or values.dtype != self.values.dtype:
+        if self.quantized:
+            if keys.dtype != values.dtype:
+                raise ValueError("keys and values must share a dtype")
+            ops.dtype_code(keys.dtype)
+        elif keys.dtype != self.keys.dtype or values.dtype != self.values.dtype:
             raise ValueError("keys and values must match the cache dtype")
         if keys.device != self.keys.device or values.device != self.values.device:
             raise ValueError("keys and values must be on the cache device")
         self._resolve_position(sequence_id, start_position + token_count - 1)
         meta = self.pack((sequence_id,), (start_position,), (token_count,))
+        if self.quantized:
+            ops.write_kv8(keys, values, self.keys, self.values, self.key_scales, self.value_scales, layer_index,
+                          meta.slot_mapping)
+            return
         ops.write_kv(keys, values, self.keys, self.values, layer_index, meta.slot_mapping)
 
-    def gather(self, layer_index: int, sequence_id: str, token_count: int) -> tuple[torch.Tensor, torch.Tensor]:
-        """Contiguous copies of the first ``token_count`` K/V rows (reference paged_cache.py:324-362)."""
+    def gather(
+        self, layer_index: int, sequence_id: str, token_count: int, *, dtype: torch.dtype | None = None
+    ) -> tuple[torch.Tensor, torch.Tensor]:
+        """Contiguous copies of the first ``token_count`` K/V rows (reference paged_cache.py:324-362).
+
+        An 8-bit cache gives values of ``dtype`` (bf16 unless told otherwise); any other its own dtype."""
+        if dtype is not None and not self.quantized and dtype != self.keys.dtype:
+            raise ValueError("only an 8-bit cache is gathered in another dtype")
         if not _is_int(layer_index):
             raise TypeError("layer_index must be an integer")
         if layer_index < 0 or layer_index >= self.num_layers:
@@ -302,6 +334,9 @@ class PagedKVCache:
         self._resolve_position(sequence_id, token_count - 1)
         tables = self.device_block_tables()
         row = tables[self._rows[sequence_id]]
+        if self.quantized:
+            return ops.gather_kv8(self.keys, self.values, self.key_scales, self.value_scales, layer_index, row, token_count,
+                                  dtype=dtype or torch.bfloat16)
         return ops.gather_kv(self.keys, self.values, layer_index, row, token_count)
 
     def export_sequence(self, sequence_id: str) -> PagedKVTransfer:
@@ -315,8 +350,14 @@ class PagedKVCache:
         keys = torch.empty(shape, dtype=self.keys.dtype, device=self.device)
         values = torch.empty_like(keys)
         src_ids = torch.tensor(table[:n], dtype=torch.int32).pin_memory().to(self.device, non_blocking=True)
-        ops.copy_blocks(
-            self.keys, self.values, src_ids, keys, values, None, n, length % self.block_size, run_on=self.device
+        key_scales = value_scales = None
+        if self.quantized:
+            key_scales, value_scales = (
+                torch.empty((self.num_layers, n, self.kv_head_num), dtype=torch.float32, device=self.device) for _ in range(2)
+            )
+        _copy_blocks(
+            (self.keys, self.values, self.key_scales, self.value_scales), src_ids, (keys, values, key_scales, value_scales),
+            None, n, length % self.block_size, self.device,
         )
         return PagedKVTransfer(
             sequence_id=sequence_id,
@@ -327,6 +368,8 @@ class PagedKVCache:
             head_dim=self.head_dim,
             keys=keys,
             values=values,
+            key_scales=key_scales,
+            value_scales=value_scales,
         )
 
     def import_sequence(self, sequence_id: str, transfer: PagedKVTransfer) -> None:
@@ -355,6 +398,11 @@ class PagedKVCache:
             raise ValueError("transfer keys must match the cache dtype")
         if transfer.values.dtype != self.values.dtype:
             raise ValueError("transfer values must match the cache dtype")
+        if self.quantized:
+            expected = (self.num_layers, n, self.kv_head_num)
+            for scales in (transfer.key_scales, transfer.value_scales):
+                if scales is None or scales.shape != expected or scales.dtype != torch.float32:
+                    raise ValueError("transfer scales have an invalid shape")
 
         self.ensure_capacity(sequence_id, transfer.sequence_length)
         try:
@@ -363,21 +411,27 @@ class PagedKVCache:
             src_device = transfer.keys.device
             if src_device != self.device:
                 _order_after(self.device, src_device)
-            ops.copy_blocks(
-                transfer.keys.contiguous(),
-                transfer.values.contiguous(),
-                None,
-                self.keys,
-                self.values,
-                dst_ids,
-                n,
-                0,
-                run_on=self.device,
+            source = (transfer.keys, transfer.values, transfer.key_scales, transfer.value_scales)
+            _copy_blocks(
+                tuple(None if t is None else t.contiguous() for t in source), None,
+                (self.keys, self.values, self.key_scales, self.value_scales), dst_ids, n, 0, self.device,
             )
             self.advance(sequence_id, transfer.sequence_length)
         except Exception:
             self.release(sequence_id)
             raise
+
+
+def _copy_blocks(source, src_ids, destination, dst_ids, n: int, tail: int, run_on: torch.device) -> None:
+    """``ops.copy_blocks`` of (keys, values, key scales, value scales); the scales are None but in 8-bit caches."""
+    keys, values, key_scales, value_scales = source
+    dst_keys, dst_values, dst_key_scales, dst_value_scales = destination
+    if key_scales is not None:
+        # codes move as pairs of bytes, a block's scales as one row of a block of one token
+        keys, values, dst_keys, dst_values = (t.view(torch.bfloat16) for t in (keys, values, dst_keys, dst_values))
+        rows = [t[:, :, None, None] for t in (key_scales, value_scales, dst_key_scales, dst_value_scales)]
+        ops.copy_blocks(rows[0], rows[1], src_ids, rows[2], rows[3], dst_ids, n, 0, run_on=run_on)
+    ops.copy_blocks(keys, values, src_ids, dst_keys, dst_values, dst_ids, n, tail, run_on=run_on)
 
 
 def _order_after(waiter: torch.device, producer: torch.device) -> None:
@@ -428,16 +482,10 @@ def transfer_sequence(source: PagedKVCache, destination: PagedKVCache, sequence_
         dst_ids = torch.tensor(dst_table[:n], dtype=torch.int32).pin_memory().to(run_device, non_blocking=True)
         if destination.device != run_device:
             _order_after(run_device, destination.device)
-        ops.copy_blocks(
-            source.keys,
-            source.values,
-            src_ids,
-            destination.keys,
-            destination.values,
-            dst_ids,
-            n,
-            length % bs,
-            run_on=run_device,
+        _copy_blocks(
+            (source.keys, source.values, source.key_scales, source.value_scales), src_ids,
+            (destination.keys, destination.values, destination.key_scales, destination.value_scales), dst_ids,
+            n, length % bs, run_device,
         )
         if destination.device != run_device:
             _order_after(destination.device, run_device)

@@ -165,3 +165,49 @@ def test_least_scale_holds_the_largest_value_and_no_smaller_one_does():
 
 def test_runs():
     assert plain.runs_of([3, 4, 5, 8, 9, -1, 10, 16, 2, 40], 4, 32) == [(0, 1), (1, 2), (3, 2), (6, 1), (7, 1), (8, 1)]
+
+
+# ------------------------------------------------------------------ the cache's bookkeeping
+def test_an_8_bit_cache_has_scales_and_others_have_none():
+    from nano_infer_engine_b200.paged_cache import PagedKVCache
+
+    c = PagedKVCache(8, 16, 2, 4, 64, torch.float8_e4m3fn, "cpu")
+    assert c.quantized and c.key_scales.shape == c.value_scales.shape == (2, 8, 4) and c.keys.element_size() == 1
+    d = PagedKVCache(8, 16, 2, 4, 64, BF16, "cpu")
+    assert not d.quantized and d.key_scales is None and d.value_scales is None
+    with pytest.raises(ValueError, match="even head_dim"):
+        PagedKVCache(8, 16, 2, 4, 63, torch.float8_e4m3fn, "cpu")
+    d.ensure_capacity("s", 3)
+    with pytest.raises(ValueError, match="only an 8-bit cache"):
+        d.gather(0, "s", 2, dtype=torch.float32)
+
+
+def test_processes_do_not_hand_8_bit_pools_over():
+    from nano_infer_engine_b200.generation.pd_disagg import export_pool
+    from nano_infer_engine_b200.paged_cache import PagedKVCache
+
+    with pytest.raises(ValueError, match="8-bit caches"):
+        export_pool(PagedKVCache(8, 16, 2, 4, 64, torch.float8_e4m3fn, "cpu"))
+
+
+def test_score_refuses_before_it_touches_the_cache():
+    from nano_infer_engine_b200.generation.score import paged_score
+    from nano_infer_engine_b200.paged_cache import PagedKVCache
+
+    c = PagedKVCache(8, 16, 1, 1, 8, BF16, "cpu")
+    prompt = torch.zeros(1, 5, dtype=torch.int64)
+    for change, message in ((dict(chunk_size=0), "chunk_size"), (dict(chunk_size=True), "chunk_size"), (dict(top=33), "top"),
+                            (dict(top=1.0), "top")):
+        with pytest.raises(ValueError, match=message):
+            paged_score(None, (prompt,), c, ("a",), **change)
+    with pytest.raises(ValueError, match="two tokens"):
+        paged_score(None, (prompt[:, :1],), c, ("a",))
+
+    class Broken:
+        def __call__(self, x, kv_cache, sequence_id):
+            kv_cache.ensure_capacity(sequence_id, 5)
+            raise RuntimeError("no")
+
+    with pytest.raises(RuntimeError, match="no"):
+        paged_score(Broken(), (prompt, prompt), c, ("a", "b"))
+    assert c.allocator.free_block_count == 8
