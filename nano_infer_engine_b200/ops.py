@@ -9,6 +9,7 @@ is no CPU implementation.  Shapes follow the reference's cache layout
 from __future__ import annotations
 
 import ctypes
+import functools
 import importlib.machinery
 import importlib.util
 from dataclasses import dataclass
@@ -883,30 +884,29 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     if isinstance(top, bool) or not isinstance(top, int) or not 0 <= top <= min(LOGPROBS_MAX_TOP, cols):
         raise ValueError(f"top must be an integer in [0, {min(LOGPROBS_MAX_TOP, cols)}]")
     code = dtype_code(logits.dtype)
-    _require_cuda(logits, tokens)
-    device = _one_device(logits, tokens)
+    index = _cuda_device(logits, tokens)
     tokens = tokens.contiguous()
+    device = logits.device
     out = torch.empty((2, rows), dtype=torch.float32, device=device)
     top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
     top_ids = torch.empty((rows, top), dtype=torch.int64, device=device)
     if rows == 0:
         return TokenLogprobs(out[0], out[1], top_logprobs, top_ids)
-    with _on(device):
-        status = lib.nie_token_logprobs(
-            logits.data_ptr(),
-            rows,
-            cols,
-            logits.stride(0) if rows > 1 else cols,
-            code,
-            tokens.data_ptr(),
-            top,
-            out[0].data_ptr(),
-            out[1].data_ptr(),
-            top_logprobs.data_ptr(),
-            top_ids.data_ptr(),
-            error_flag(device).data_ptr(),
-            _stream(device),
-        )
+    status = _launch(
+        index,
+        lib.nie_token_logprobs,
+        logits.data_ptr(),
+        rows,
+        cols,
+        logits.stride(0) if rows > 1 else cols,
+        code,
+        tokens.data_ptr(),
+        top,
+        out.data_ptr(),
+        out.data_ptr() + 4 * rows,
+        top_logprobs.data_ptr(),
+        top_ids.data_ptr(),
+    )
     check(status, "nie_token_logprobs")
     _count()
     return TokenLogprobs(out[0], out[1], top_logprobs, top_ids)
@@ -918,28 +918,35 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
 KV8_DTYPE = torch.float8_e4m3fn
 
 
-class _NoGuard:
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return None
-
-
-_no_guard = _NoGuard()
-
-
-def _on(device: torch.device):
-    """Guard that makes ``device`` current (nothing to do when it is)."""
-    return _no_guard if device.index == torch.cuda.current_device() else torch.cuda.device(device)
-
-
-def _one_device(*tensors: torch.Tensor | None) -> torch.device:
-    device = tensors[0].device
+def _cuda_device(*tensors: torch.Tensor | None) -> int:
+    """Index of the CUDA device that all of the tensors are on; refuses any other mix."""
+    index = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"tensors must share a device (got {device} and {t.device})")
-    return device
+        if t is not None and (t.get_device() != index or index < 0):
+            _require_cuda(*tensors)
+            raise ValueError(f"tensors must share a device (got {tensors[0].device} and {t.device})")
+    return index
+
+
+def _launch(index: int, entry, *args) -> int:
+    """``entry(*args, error flag, stream)`` of device ``index``, made current for the call if it is not."""
+    flag = _err_flags.get(index)
+    if flag is None:
+        flag = error_flag(torch.device("cuda", index))
+    if index == torch.cuda.current_device():
+        return entry(*args, flag.data_ptr(), _raw_stream(index) if _raw_stream else _stream(flag))
+    with torch.cuda.device(index):
+        return entry(*args, flag.data_ptr(), _stream(flag))
+
+
+@functools.lru_cache(maxsize=None)
+def _kv8_decode_workspace_bytes(index: int, num_requests: int, q_heads: int, head_dim: int) -> int:
+    return int(lib.nie_paged_decode_kv8_workspace_size(index, num_requests, q_heads, head_dim))
+
+
+@functools.lru_cache(maxsize=None)
+def _kv8_varlen_workspace_bytes(index: int, head_dim: int) -> int:
+    return int(lib.nie_varlen_kv8_workspace_size(index, head_dim))
 
 
 def _kv8_geometry(
@@ -998,39 +1005,37 @@ def rope_write_kv8(
             raise ValueError("sin/cos must be contiguous [T, head_dim/2] of q's dtype")
     _check_slots(slot_mapping, T)
     code = dtype_code(q.dtype)
-    _require_cuda(q, k, v, sin, cos, key_cache, value_cache, key_scales, value_scales, slot_mapping)
-    device = _one_device(q, k, v, sin, cos, key_cache, value_cache, key_scales, value_scales, slot_mapping)
-    q_out = torch.empty((T, q_heads, d), dtype=q.dtype, device=device)
+    index = _cuda_device(q, k, v, sin, cos, key_cache, value_cache, key_scales, value_scales, slot_mapping)
+    q_out = torch.empty((T, q_heads, d), dtype=q.dtype, device=q.device)
     if T == 0:
         return q_out
-    with _on(device):
-        status = lib.nie_rope_write_kv8(
-            q.data_ptr(),
-            q.stride(0),
-            k.data_ptr(),
-            k.stride(0),
-            v.data_ptr(),
-            v.stride(0),
-            sin.data_ptr(),
-            cos.data_ptr(),
-            T,
-            q_heads,
-            h,
-            d,
-            q_out.data_ptr(),
-            key_cache.data_ptr(),
-            value_cache.data_ptr(),
-            key_scales.data_ptr(),
-            value_scales.data_ptr(),
-            code,
-            layer,
-            L,
-            nb,
-            bs,
-            slot_mapping.data_ptr(),
-            error_flag(device).data_ptr(),
-            _stream(device),
-        )
+    status = _launch(
+        index,
+        lib.nie_rope_write_kv8,
+        q.data_ptr(),
+        q.stride(0),
+        k.data_ptr(),
+        k.stride(0),
+        v.data_ptr(),
+        v.stride(0),
+        sin.data_ptr(),
+        cos.data_ptr(),
+        T,
+        q_heads,
+        h,
+        d,
+        q_out.data_ptr(),
+        key_cache.data_ptr(),
+        value_cache.data_ptr(),
+        key_scales.data_ptr(),
+        value_scales.data_ptr(),
+        code,
+        layer,
+        L,
+        nb,
+        bs,
+        slot_mapping.data_ptr(),
+    )
     check(status, "nie_rope_write_kv8")
     _count()
     return q_out
@@ -1053,34 +1058,32 @@ def write_kv8(
     T = keys.shape[0]
     _check_slots(slot_mapping, T)
     code = dtype_code(keys.dtype)
-    _require_cuda(keys, values, key_cache, value_cache, key_scales, value_scales, slot_mapping)
-    device = _one_device(keys, values, key_cache, value_cache, key_scales, value_scales, slot_mapping)
+    index = _cuda_device(keys, values, key_cache, value_cache, key_scales, value_scales, slot_mapping)
     keys = keys.contiguous()
     values = values.contiguous()
     if T == 0:
         return
-    with _on(device):
-        status = lib.nie_write_kv8(
-            keys.data_ptr(),
-            h * d,
-            values.data_ptr(),
-            h * d,
-            T,
-            key_cache.data_ptr(),
-            value_cache.data_ptr(),
-            key_scales.data_ptr(),
-            value_scales.data_ptr(),
-            code,
-            layer,
-            L,
-            nb,
-            bs,
-            h,
-            d,
-            slot_mapping.data_ptr(),
-            error_flag(device).data_ptr(),
-            _stream(device),
-        )
+    status = _launch(
+        index,
+        lib.nie_write_kv8,
+        keys.data_ptr(),
+        h * d,
+        values.data_ptr(),
+        h * d,
+        T,
+        key_cache.data_ptr(),
+        value_cache.data_ptr(),
+        key_scales.data_ptr(),
+        value_scales.data_ptr(),
+        code,
+        layer,
+        L,
+        nb,
+        bs,
+        h,
+        d,
+        slot_mapping.data_ptr(),
+    )
     check(status, "nie_write_kv8")
     _count()
 
@@ -1103,32 +1106,30 @@ def gather_kv8(
     if not 0 <= num_tokens <= block_table.numel() * bs:
         raise ValueError("num_tokens must be covered by the block table")
     code = dtype_code(dtype)
-    _require_cuda(key_cache, value_cache, key_scales, value_scales, block_table)
-    device = _one_device(key_cache, value_cache, key_scales, value_scales, block_table)
-    out_k = torch.empty((num_tokens, h, d), dtype=dtype, device=device)
+    index = _cuda_device(key_cache, value_cache, key_scales, value_scales, block_table)
+    out_k = torch.empty((num_tokens, h, d), dtype=dtype, device=key_cache.device)
     out_v = torch.empty_like(out_k)
     if num_tokens == 0:
         return out_k, out_v
-    with _on(device):
-        status = lib.nie_gather_kv8(
-            key_cache.data_ptr(),
-            value_cache.data_ptr(),
-            key_scales.data_ptr(),
-            value_scales.data_ptr(),
-            layer,
-            L,
-            nb,
-            bs,
-            h,
-            d,
-            block_table.data_ptr(),
-            num_tokens,
-            out_k.data_ptr(),
-            out_v.data_ptr(),
-            code,
-            error_flag(device).data_ptr(),
-            _stream(device),
-        )
+    status = _launch(
+        index,
+        lib.nie_gather_kv8,
+        key_cache.data_ptr(),
+        value_cache.data_ptr(),
+        key_scales.data_ptr(),
+        value_scales.data_ptr(),
+        layer,
+        L,
+        nb,
+        bs,
+        h,
+        d,
+        block_table.data_ptr(),
+        num_tokens,
+        out_k.data_ptr(),
+        out_v.data_ptr(),
+        code,
+    )
     check(status, "nie_gather_kv8")
     _count()
     return out_k, out_v
@@ -1192,54 +1193,51 @@ def paged_decode_kv8(
                                or q_rows.numel() < seq_lens.numel()):
         raise ValueError("q_rows must be contiguous int64 with an entry per request")
     code = dtype_code(query.dtype)
-    _require_cuda(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, out, table_rows, q_rows,
-                  req_list)
-    device = _one_device(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, out, table_rows,
+    index = _cuda_device(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, out, table_rows,
                          q_rows, req_list)
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if R == 0:
         return out
     # of this call alone: calls on other streams and captured graphs have their own
-    need = lib.nie_paged_decode_kv8_workspace_size(device.index, R, query.shape[1], d)
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    with _on(device):
-        status = lib.nie_paged_decode_kv8(
-            query.data_ptr(),
-            query.stride(0),
-            out.data_ptr(),
-            out.stride(0),
-            query.shape[0],
-            key_cache.data_ptr(),
-            value_cache.data_ptr(),
-            key_scales.data_ptr(),
-            value_scales.data_ptr(),
-            code,
-            layer,
-            L,
-            nb,
-            bs,
-            h,
-            d,
-            query.shape[1],
-            block_tables.data_ptr(),
-            block_tables.stride(0),
-            block_tables.shape[0],
-            _ptr(table_rows),
-            seq_lens.data_ptr(),
-            seq_lens.numel(),
-            _ptr(q_rows),
-            _ptr(req_list),
-            R,
-            float(d**-0.5 if scale is None else scale),
-            ws.data_ptr(),
-            need,
-            int(overlap),
-            error_flag(device).data_ptr(),
-            _stream(device),
-        )
+    need = _kv8_decode_workspace_bytes(index, R, query.shape[1], d)
+    ws = torch.empty(need, dtype=torch.uint8, device=query.device)
+    status = _launch(
+        index,
+        lib.nie_paged_decode_kv8,
+        query.data_ptr(),
+        query.stride(0),
+        out.data_ptr(),
+        out.stride(0),
+        query.shape[0],
+        key_cache.data_ptr(),
+        value_cache.data_ptr(),
+        key_scales.data_ptr(),
+        value_scales.data_ptr(),
+        code,
+        layer,
+        L,
+        nb,
+        bs,
+        h,
+        d,
+        query.shape[1],
+        block_tables.data_ptr(),
+        block_tables.stride(0),
+        block_tables.shape[0],
+        _ptr(table_rows),
+        seq_lens.data_ptr(),
+        seq_lens.numel(),
+        _ptr(q_rows),
+        _ptr(req_list),
+        R,
+        float(d**-0.5 if scale is None else scale),
+        ws.data_ptr(),
+        need,
+        int(overlap),
+    )
     check(status, "nie_paged_decode_kv8")
-    _count(kv8_launch_count(query.dtype, bs, d, R))
+    _count(kv8_launch_count(query.dtype, bs, d, R, block_tables.stride(0) * bs))
     return out
 
 
@@ -1274,54 +1272,51 @@ def varlen_attention_kv8(
     if int(max_query_len) < 1:
         raise ValueError("max_query_len must be positive")
     code = dtype_code(query.dtype)
-    _require_cuda(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, query_start_loc, out,
-                  table_rows, req_list)
-    device = _one_device(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, query_start_loc,
+    index = _cuda_device(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, query_start_loc,
                          out, table_rows, req_list)
     if out is None:
-        out = torch.empty(query.shape, dtype=query.dtype, device=device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if R == 0:
         return out
     # of this call alone: calls on other streams and captured graphs have their own
-    need = lib.nie_varlen_kv8_workspace_size(device.index, d)
-    ws = torch.empty(need, dtype=torch.uint8, device=device)
-    with _on(device):
-        status = lib.nie_varlen_attention_kv8(
-            query.data_ptr(),
-            query.stride(0),
-            out.data_ptr(),
-            out.stride(0),
-            query.shape[0],
-            key_cache.data_ptr(),
-            value_cache.data_ptr(),
-            key_scales.data_ptr(),
-            value_scales.data_ptr(),
-            code,
-            layer,
-            L,
-            nb,
-            bs,
-            h,
-            d,
-            query.shape[1],
-            block_tables.data_ptr(),
-            block_tables.stride(0),
-            block_tables.shape[0],
-            _ptr(table_rows),
-            seq_lens.data_ptr(),
-            seq_lens.numel(),
-            query_start_loc.data_ptr(),
-            _ptr(req_list),
-            R,
-            int(max_query_len),
-            float(d**-0.5 if scale is None else scale),
-            ws.data_ptr(),
-            need,
-            error_flag(device).data_ptr(),
-            _stream(device),
-        )
+    need = _kv8_varlen_workspace_bytes(index, d)
+    ws = torch.empty(need, dtype=torch.uint8, device=query.device)
+    status = _launch(
+        index,
+        lib.nie_varlen_attention_kv8,
+        query.data_ptr(),
+        query.stride(0),
+        out.data_ptr(),
+        out.stride(0),
+        query.shape[0],
+        key_cache.data_ptr(),
+        value_cache.data_ptr(),
+        key_scales.data_ptr(),
+        value_scales.data_ptr(),
+        code,
+        layer,
+        L,
+        nb,
+        bs,
+        h,
+        d,
+        query.shape[1],
+        block_tables.data_ptr(),
+        block_tables.stride(0),
+        block_tables.shape[0],
+        _ptr(table_rows),
+        seq_lens.data_ptr(),
+        seq_lens.numel(),
+        query_start_loc.data_ptr(),
+        _ptr(req_list),
+        R,
+        int(max_query_len),
+        float(d**-0.5 if scale is None else scale),
+        ws.data_ptr(),
+        need,
+    )
     check(status, "nie_varlen_attention_kv8")
-    _count(kv8_launch_count(query.dtype, bs, d, R))
+    _count(kv8_launch_count(query.dtype, bs, d, R, None))
     return out
 
 
@@ -1354,7 +1349,11 @@ def decode_launch_count(dtype: torch.dtype, block_size: int, kv_heads: int, head
     return 2 if fast else 1
 
 
-def kv8_launch_count(dtype: torch.dtype, block_size: int, head_dim: int, num_requests: int) -> int:
-    """Kernels one :func:`paged_decode_kv8` or :func:`varlen_attention_kv8` call launches (two per 512 requests, or the generic one)."""
-    fast = dtype != torch.float32 and head_dim in (64, 128) and block_size % 16 == 0
-    return 2 * -(-num_requests // 512) if fast else 1
+def kv8_launch_count(dtype: torch.dtype, block_size: int, head_dim: int, num_requests: int, max_keys: int | None) -> int:
+    """Kernels of one :func:`paged_decode_kv8` call whose tables hold ``max_keys`` keys, or (None) of one
+    :func:`varlen_attention_kv8` call: one and its merging kernel per 512 or 256 requests, or the generic one."""
+    if dtype == torch.float32 or head_dim not in (64, 128) or block_size % 16:
+        return 1
+    if max_keys is None:
+        return 2 * -(-num_requests // 256)
+    return (1 if max_keys <= 1024 else 2) * -(-num_requests // 512)
