@@ -419,7 +419,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
   };
 
   // ---- warps to the CTA, the CTA to the output or the merging kernel
-  auto finish = [&](int i, bool whole) {
+  auto finish = [&](int i, bool whole, bool last) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
         if (d == 0) *reinterpret_cast<float2*>(ps + HD) = make_float2(M, L);
       }
     }
-    __syncthreads();
+    if (!last) __syncthreads();
   };
 
   refill(0);
@@ -487,19 +487,19 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
       issue(j + kD8Stages - 1);
       tile(j % kD8Stages);
     }
-    finish(i, cum[i] >= lo && cum[i + 1] <= hi);
+    finish(i, cum[i] >= lo && cum[i + 1] <= hi, end == hi);
     at = end;
   }
   cp_wait<0>();
 }
 
 // Requests cut by a border: merge the CTAs' partials in order.  One CTA per
-// (request, query head); 16 groups of its threads take every 16th partial, all of
-// a thread's loads go out together.  Requests without keys get zeros.
-template <int HD, typename T>
-__global__ void __launch_bounds__(HD * 4) kv8_decode_merge_kernel(const __grid_constant__ Kv8Args a,
+// (request, query head); GROUPS groups of its threads take every GROUPS-th partial,
+// all of a thread's loads go out together.  Requests without keys get zeros.
+template <int HD, int GROUPS, typename T>
+__global__ void __launch_bounds__(HD / 4 * GROUPS) kv8_decode_merge_kernel(const __grid_constant__ Kv8Args a,
                                                                            const __grid_constant__ D8Plan p) {
-  constexpr int GROUPS = 16, LANES = HD / 4;
+  constexpr int LANES = HD / 4;
   __shared__ float4 so[GROUPS][LANES];
   __shared__ float sm_m[GROUPS], sm_l[GROUPS];
   pdl_wait();
@@ -591,7 +591,7 @@ bool kv8_decode_takes(int dtype, const Kv8Args& a) {
 }
 
 template <int HD, int NT, typename T>
-static int launch_decode(const Kv8Args& a, const D8Plan& p, dim3 grid, bool overlap, cudaStream_t s) {
+static int launch_decode(const Kv8Args& a, const D8Plan& p, dim3 grid, int sms, bool overlap, cudaStream_t s) {
   constexpr int SUBS = 2048 / HD / 16;
   const size_t smem = (size_t)kD8Warps * kD8Stages * (kD8Stage + SUBS * 16) +
                       (size_t)kD8Warps * NT * 8 * (HD + 4 + 2) * sizeof(float) + (size_t)(4 * p.num_req + 1) * sizeof(int);
@@ -608,7 +608,15 @@ static int launch_decode(const Kv8Args& a, const D8Plan& p, dim3 grid, bool over
     if (st != NIE_OK) return st;
   }
   if (p.whole) return NIE_OK;
-  pdl_launch(kv8_decode_merge_kernel<HD, T>, dim3((unsigned)p.num_req, (unsigned)a.hq), dim3(HD * 4), s, a, p);
+  // A request is cut into 1 + grid.x / requests parts on average, so a large batch's requests into few: four groups
+  // take them in one round of loads, and more of the small CTAs are on the GPU at once.  In all, 64 requests of
+  // 29600 keys x 32 heads take 169.2 us with 4 groups and 173.2 with 16; 16 of 4001 keys 16.9 and 16.35; one of
+  // 131072 keys 46.1 and 35.9 (34.7 with 32, which costs the other two 2 and 7 us).
+  const dim3 merge_grid((unsigned)p.num_req, (unsigned)a.hq);
+  if (p.num_req * a.hq > 4 * sms)
+    pdl_launch(kv8_decode_merge_kernel<HD, 4, T>, merge_grid, dim3(HD), s, a, p);
+  else
+    pdl_launch(kv8_decode_merge_kernel<HD, 16, T>, merge_grid, dim3(HD * 4), s, a, p);
   return check_launch("kv8_decode_merge_kernel");
 }
 
@@ -645,7 +653,7 @@ int launch_kv8_decode(int dtype, const Kv8Args& args, int num_requests, int sms,
     p.ts = kD8Warps / p.hc;
     p.min_tiles = p.ts;
     // Where the tables hold 1024 keys at most, a CTA takes a request (at most 8 tiles to a warp) and no second
-    // launch is needed: 100 keys take 4.9 us and one launch, against 7.2 us and two.
+    // launch is needed: 100 keys take 5.6 us and one launch, against 7.2 us and two.
     p.whole = a.tstride * a.bs <= 1024;
     const int ctas = p.whole ? p.num_req : std::max(1, 2 * sms / (heads / p.hc));
     p.cum_out = (int32_t*)workspace;
@@ -654,11 +662,11 @@ int launch_kv8_decode(int dtype, const Kv8Args& args, int num_requests, int sms,
     const bool half = dtype == NIE_DTYPE_F16, wide = p.rows > 8;
     int rc;
     if (a.hd == 64) {
-      if (half) rc = wide ? launch_decode<64, 2, __half>(a, p, grid, overlap, s) : launch_decode<64, 1, __half>(a, p, grid, overlap, s);
-      else rc = wide ? launch_decode<64, 2, __nv_bfloat16>(a, p, grid, overlap, s) : launch_decode<64, 1, __nv_bfloat16>(a, p, grid, overlap, s);
+      if (half) rc = wide ? launch_decode<64, 2, __half>(a, p, grid, sms, overlap, s) : launch_decode<64, 1, __half>(a, p, grid, sms, overlap, s);
+      else rc = wide ? launch_decode<64, 2, __nv_bfloat16>(a, p, grid, sms, overlap, s) : launch_decode<64, 1, __nv_bfloat16>(a, p, grid, sms, overlap, s);
     } else {
-      if (half) rc = wide ? launch_decode<128, 2, __half>(a, p, grid, overlap, s) : launch_decode<128, 1, __half>(a, p, grid, overlap, s);
-      else rc = wide ? launch_decode<128, 2, __nv_bfloat16>(a, p, grid, overlap, s) : launch_decode<128, 1, __nv_bfloat16>(a, p, grid, overlap, s);
+      if (half) rc = wide ? launch_decode<128, 2, __half>(a, p, grid, sms, overlap, s) : launch_decode<128, 1, __half>(a, p, grid, sms, overlap, s);
+      else rc = wide ? launch_decode<128, 2, __nv_bfloat16>(a, p, grid, sms, overlap, s) : launch_decode<128, 1, __nv_bfloat16>(a, p, grid, sms, overlap, s);
     }
     if (rc != NIE_OK) return rc;
   }
