@@ -97,6 +97,8 @@ struct F8Bars {
   uint64_t done;
   uint32_t tmem_base;
   int abort;
+  int nan_codes;                         // a NaN of V has been kept out of a product
+  int4 row_of[16];                       // of a softmax warp's segment: its table row, kv head, first key of a NaN search
   int start_req, start_tile, start_head;
   int64_t start_pos;
   int flags[kF8MaxStages];                  // of a stage's tile: kF8First, ...
@@ -265,6 +267,27 @@ __device__ __forceinline__ void f8_mma_ts(uint32_t d, uint32_t a, uint32_t b, ui
 }
 __device__ __forceinline__ uint32_t f8_desc(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | ((lbo >> 4) << 16); }
 
+// First tile of a segment that some row does not see all of.  There the loaders put
+// zeros for NaN codes of V: 0 * NaN would reach the rows that do not see the key.
+template <class C>
+__device__ __forceinline__ int f8_masked_from(const Kv8Args& a, const F8Walk<C>& s) {
+  return max(0, s.x.ctx + s.tile * C::Rows / a.group + 1) / C::BN;
+}
+
+// The NaN that were left out, for one row that sees the keys [from, to): out + d * step gets one for
+// each dimension d in which one of them has it.
+template <typename T>
+__device__ __noinline__ void f8_put_nan(const Kv8Args& a, int trow, int h, int from, int to, T* out, int step) {
+  for (int key = from; key < to; ++key) {
+    const int lb = key / a.bs;
+    const int64_t block = lb < a.tstride ? (int64_t)a.tables[(int64_t)trow * a.tstride + lb] : -1;
+    if (block < 0 || block >= a.nb) continue;
+    const uint8_t* codes = a.vc + ((block * a.bs + key % a.bs) * a.hkv + h) * a.hd;
+    for (int d = 0; d < a.hd; ++d)
+      if ((codes[d] & 0x7f) == 0x7f) out[(int64_t)d * step] = Num<T>::from_f(__int_as_float(0x7fffffff));
+  }
+}
+
 template <int HD, typename T>
 __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
     kv8_prefill_kernel(const __grid_constant__ Kv8Args a, const __grid_constant__ F8Plan p) {
@@ -308,6 +331,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
     }
     mbar_init(&b->done, C::Parts);
     b->abort = 0;
+    b->nan_codes = 0;
     fence_mbar_init();
   }
   __syncthreads();
@@ -439,7 +463,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
     uint32_t par = 1;  // parity of the stage's last release; the first round finds the stages free
     for (; ok && seg.valid(); seg.next(a, R)) {
       const int rows = seg.rows();
-      const int thi = seg.t_hi();
+      const int thi = seg.t_hi(), masked = f8_masked_from(a, seg);
       for (int kt = seg.t_lo(); kt < thi; ++kt) {
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         if (!f8_wait_idle(b, &b->kv_empty[st], par, a.err)) {
@@ -454,6 +478,16 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
           const int row = (tid >> 2) + Pass * (jj % Passes), half = jj / Passes;
           const uint4 x = *reinterpret_cast<const uint4*>(src + j * (C::Loaders * 16));
           uint32_t w[4] = {x.x, x.y, x.z, x.w}, h[8];
+          if (j >= Copies && kt >= masked) {
+            uint32_t any = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const uint32_t nan = __vcmpeq4(w[e] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              w[e] &= ~nan;
+              any |= nan;
+            }
+            if (any) *reinterpret_cast<volatile int*>(&b->nan_codes) = 1;
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             if (j < Copies) w[e] ^= flip;
@@ -638,6 +672,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
       if (tlo == 0 && !whole && threadIdx.x == 0)
         p.cuts[blockIdx.x] = F8Cut{(int64_t)seg.tile * C::Rows, seg.x.first, rows, seg.h,
                                    (int)((lo + seg.start + seg.n - 1) / W - blockIdx.x), 0};
+      if (lane == 0) b->row_of[warp] = make_int4(seg.x.trow, seg.h, max(tlo, f8_masked_from(a, seg)) * BN, seg.x.n);
       float m_ref = -INFINITY, l = 0.f;
       // One key tile of the row; MASK: some row of the warp does not see all of it.
       auto softmax_tile = [&](int kt, auto masked) -> bool {
@@ -776,6 +811,12 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
         if (!whole && row < rows) {
           ps[0] = m_ref;
           ps[C::Rows] = l;
+        }
+        if (row < rows && *reinterpret_cast<volatile int*>(&b->nan_codes)) {  // known since the tile's kv_full
+          const int4 of = b->row_of[warp];
+          const int to = min(min(qpos + 1, thi * BN), of.w);
+          if (whole) f8_put_nan(a, of.x, of.y, of.z, to, op, 1);
+          else f8_put_nan(a, of.x, of.y, of.z, to, ps + 2 * C::Rows, C::Rows);
         }
       }
       tc_fence_before();
