@@ -473,6 +473,9 @@ int nie_gather_kv8(const void* key_cache, const void* value_cache,
  * is outside the pool raises NIE_DEV_ERR_BLOCK_RANGE.  seq_lens, table_rows and
  * q_rows have num_seqs entries, block_tables num_table_rows rows; a request of
  * req_list or a row of table_rows outside them is flagged and skipped likewise.
+ * No request has more than max_query_len tokens: where that times the query
+ * heads of a kv head times head_dim is 4096 at most, longer ones are flagged
+ * (NIE_DEV_ERR_CAPACITY) and skipped.
  * head_dim <= 256.  The workspace (nie_paged_decode_kv8_workspace_size,
  * nie_varlen_kv8_workspace_size bytes, 256-byte aligned) holds partial sums of
  * one call; calls that share it must not overlap on the GPU.  overlap != 0: the kernel may start before the

@@ -29,9 +29,9 @@ enum SmemSlot {
   kSmemPrefill = 2,
   kSmemLinear = 3,
   kSmemLinear64 = 4,
-  kSmemKv8Decode = 5,   // 8 instances
-  kSmemKv8Prefill = 13,  // 4 instances
-  kSmemSlots = 17
+  kSmemKv8Decode = 5,    // 12 instances
+  kSmemKv8Prefill = 17,  // 4 instances
+  kSmemSlots = 21
 };
 int opt_in_smem(int slot, const void* kernel, size_t bytes);
 

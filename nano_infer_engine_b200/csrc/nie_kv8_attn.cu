@@ -204,6 +204,8 @@ extern "C" int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, voi
     NIE_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
                     workspace_bytes >= kv8_prefill_workspace(sms, head_dim),
                 "workspace too small or not 256-byte aligned");
+    if (kv8_short_takes(dtype, a, num_requests, max_query_len, sms, workspace_bytes))
+      return launch_kv8_short(dtype, a, num_requests, max_query_len, sms, workspace, s);
     return launch_kv8_prefill(dtype, a, num_requests, sms, workspace, s);
   }
   return launch_kv8_generic(dtype, a, num_requests, max_query_len, s);

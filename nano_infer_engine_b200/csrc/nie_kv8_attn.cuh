@@ -62,6 +62,11 @@ size_t kv8_decode_workspace(int sms, int num_requests, int q_heads, int head_dim
 int launch_kv8_decode(int dtype, const Kv8Args& a, int num_requests, int sms, void* workspace, bool overlap,
                       cudaStream_t s);
 
+// The same for requests of a few query tokens each (max_query_len at most), where kv8_short_takes().
+bool kv8_short_takes(int dtype, const Kv8Args& a, int num_requests, int max_query_len, int sms, size_t workspace_bytes);
+int launch_kv8_short(int dtype, const Kv8Args& a, int num_requests, int max_query_len, int sms, void* workspace,
+                     cudaStream_t s);
+
 // The tcgen05 kernel of ragged queries (nie_kv8_prefill.cu), likewise.
 bool kv8_prefill_takes(int dtype, const Kv8Args& a);
 size_t kv8_prefill_workspace(int sms, int head_dim);

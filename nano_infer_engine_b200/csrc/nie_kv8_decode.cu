@@ -1,5 +1,5 @@
-// Single-token attention over the 8-bit paged cache for bf16 / f16 queries,
-// head_dim 64 or 128, blocks of a multiple of 16 tokens.
+// Attention of one query token, or of a few, over the 8-bit paged cache for bf16 /
+// f16 queries, head_dim 64 or 128, blocks of a multiple of 16 tokens.
 //
 // What bounds it: the codes, read once.  One query token gives each code two
 // multiply-adds per query head of its group, far below the tensor rate, so the
@@ -17,7 +17,8 @@
 // One warp and tile.  cp.async brings the tile's codes to the warp's own ring of
 // two stages: no barrier between warps.  The products are transposed, so that
 // the 16 tokens of a sub-block fill the 16 rows of an m16n8k16 f16 MMA and the
-// query heads of the group its 8 columns (two MMAs for up to 16 heads):
+// query heads of the group its 8 columns (two MMAs for up to 16).  With several
+// query tokens the columns are (token, head) pairs, each with its own last key:
 //   S^T[token, head] = K Q^T      A = codes as f16 (exact), B = q in registers
 //   O^T[dim, head]  += V^T P^T    A = codes as f16 (exact), B = P^T (movmatrix)
 // q is f16 as it is, or bf16 scaled by a power of two per head so that its
@@ -42,16 +43,21 @@ constexpr int kD8Warps = 8;
 constexpr int kD8Stages = 2;
 constexpr int kD8Stage = 4096;     // bytes of K and V codes of one tile
 constexpr int kD8MaxReq = 512;     // requests of one launch (their lengths sit in shared memory)
+// Columns x head_dim of a kv head up to which requests of several tokens come here; above it the tensor tiles of the
+// ragged kernel are filled well enough.  8 requests of 8 tokens behind 2000 keys, 32 heads on 8 of 64: 23.5 us here
+// and 49.2 there (of 16 tokens: 31.6 and 50.3); 16 on 4 of 128: 27.5 and 37.6 (38.3 and 38.9).
+constexpr int kD8ShortCols = 4096;
 constexpr float kD8Log2e = 1.4426950408889634f;
 constexpr float kD8Lazy = 8.f;
 
 struct D8Plan {
   int num_req;
   int hc, ts;          // kv heads and token splits of a CTA: hc * ts = 8
-  int rows, subs;      // query heads of one MMA column set; column sets per kv head
+  int cols;            // columns per kv head: its query heads, or (token, query head) pairs of the longest request
+  int rows, subs;      // columns of one MMA column set; column sets per kv head
   int min_tiles;       // a CTA takes at least this many tiles
   int whole;           // a CTA takes one request: nothing to merge
-  float* partials;     // [ctas + num_req][hq][hd + 2]
+  float* partials;     // [ctas + num_req][hkv * cols][hd + 4]
   int32_t* cum_out;    // [num_req + 2]: tiles before each request, then tiles per CTA
 };
 
@@ -95,12 +101,21 @@ __device__ __forceinline__ void codes_to_f16(uint32_t w, uint32_t& lo, uint32_t&
 // t + 12, whose V rows lie in different banks.
 __device__ __forceinline__ int row_token(int i) { return (i & 8) + ((i & 7) >> 1) + 4 * (i & 1); }
 
+// Column `col` of kv head kvh, of a request whose first row is `row`.
+template <bool MULTI, typename P>
+__device__ __forceinline__ P* d8_row(P* base, int64_t stride, const Kv8Args& a, int row, int kvh, int col) {
+  const int64_t token = MULTI ? col / a.group : 0;
+  return base + (row + token) * stride + (int64_t)(kvh * a.group + (MULTI ? col % a.group : col)) * (int64_t)a.hd;
+}
+
 // Merge factor of a partial with reference m against M: one that saw no key has
 // nothing to add (and NaN, which leaves m alone, must reach the result).
 __device__ __forceinline__ float merge_weight(float m, float M) { return m == -INFINITY ? 0.f : fast_exp2(m - M); }
 
-template <int HD, int NT, typename T>
-__global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) kv8_decode_kernel(const __grid_constant__ Kv8Args a,
+// MULTI: requests of several query tokens.  A column is a (token, query head of the group) pair then, and sees
+// the keys up to its token's.
+template <int HD, int NT, bool MULTI, typename T>
+__global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __grid_constant__ Kv8Args a,
                                                                            const __grid_constant__ D8Plan p) {
   constexpr int TOK = 2048 / HD, SUBS = TOK / 16, CPR = HD / 16;  // tokens, sub-blocks, 16-byte chunks per row
   constexpr int ITEMS = 32 / SUBS;                                // tiles whose rows a warp looks up at once
@@ -117,22 +132,28 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
   int* len = cum + R + 1;
   int* trow = len + R;
   int* qrow = trow + R;
+  int* count = qrow + R;  // MULTI: query tokens
   __shared__ int warp_sum[kD8Warps];
 
   pdl_trigger();  // the merging kernel may be staged now (it waits for this grid)
   // ---- lengths, tables and query rows of the requests; tiles before each
   for (int i = threadIdx.x; i < R; i += kD8Warps * 32) {
     const int r = a.req_list ? a.req_list[i] : i;
-    int n = 0, tr = 0, qr = -1;
+    int n = 0, tr = 0, qr = -1, c = 0;
     if (r >= 0 && r < a.num_seqs) {
       tr = a.table_rows ? a.table_rows[r] : r;
       const Kv8Rows rows = kv8_rows(a, r, a.err);
       if (rows.count > 0 && tr >= 0 && tr < a.num_table_rows) {
         n = max(a.seq_lens[r], 0);
         qr = (int)rows.first;
+        c = (int)rows.count;
+        if (MULTI && rows.count * a.group > p.cols) n = 0, qr = -1, c = 0;  // longer than the call said
+      } else if (MULTI && rows.count <= 0 && tr >= 0 && tr < a.num_table_rows) {
+        qr = 0;  // no query token: nothing to do, nothing wrong
       }
     }
     if (qr < 0) raise_flag(a.err, NIE_DEV_ERR_CAPACITY);
+    if constexpr (MULTI) count[i] = c;
     len[i] = n;
     trow[i] = tr;
     qrow[i] = qr;
@@ -165,11 +186,12 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
   pdl_wait();
   if (p.whole) {
     if (lo == hi && qrow[blockIdx.x] >= 0) {  // a request without keys: zeros
-      T* out = reinterpret_cast<T*>(a.out) + (int64_t)qrow[blockIdx.x] * a.out_stride;
       for (int c = 0; c < p.hc; ++c) {
-        const int v = blockIdx.y * p.hc + c, first_head = v / p.subs * a.group + v % p.subs * p.rows;
-        const int n = min(p.rows, a.group - v % p.subs * p.rows) * HD;
-        for (int x = threadIdx.x; x < n; x += kD8Warps * 32) out[(int64_t)first_head * HD + x] = Num<T>::from_f(0.f);
+        const int v = blockIdx.y * p.hc + c, first = v % p.subs * p.rows;
+        const int n = min(p.rows, (MULTI ? count[blockIdx.x] * a.group : a.group) - first) * HD;
+        for (int x = threadIdx.x; x < n; x += kD8Warps * 32)
+          *(d8_row<MULTI>(reinterpret_cast<T*>(a.out), a.out_stride, a, qrow[blockIdx.x], v / p.subs, first + x / HD) + x % HD) =
+              Num<T>::from_f(0.f);
       }
     }
   } else if (blockIdx.x == 0 && blockIdx.y == 0) {
@@ -189,8 +211,8 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
 
   // ---- this warp: kv head and column set, and its tiles lo + split, + ts, ...
   const int vh = blockIdx.y * p.hc + warp % p.hc, split = warp / p.hc;
-  const int kvh = vh / p.subs, head0 = kvh * a.group + (vh % p.subs) * p.rows;
-  const int nrows = min(p.rows, a.group - (vh % p.subs) * p.rows);  // query heads of this warp
+  const int kvh = vh / p.subs, col0 = (vh % p.subs) * p.rows;
+  int nrows = min(p.rows, p.cols - col0);  // columns of this warp
   const int first = lo + split;
   const int items = first < hi ? (hi - first - 1) / p.ts + 1 : 0;
   const int64_t row_bytes = (int64_t)a.hkv * HD;
@@ -220,7 +242,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
           raise_flag(a.err, NIE_DEV_ERR_BLOCK_RANGE);
         } else {
           win_row = (int)(block * a.bs + tok % a.bs);
-          win_n = n;
+          win_n = MULTI ? len[i] - tok : n;  // MULTI: all keys from here on, for the columns' ends
           win_ks = a.ks[block * a.hkv + kvh];
           win_vs = fminf(fmaxf(a.vs[block * a.hkv + kvh], kScaleMin), kScaleMax);
         }
@@ -256,15 +278,24 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
   float qs[NT][2];  // what undoes the scaling of heads 2t, 2t + 1
   float o[HD / 16][NT][4];
   float m[NT][2], l[NT][2];
+  int back[NT][2], back_max = 0;  // MULTI: keys at the end that columns 2t, 2t + 1 (that any column) do not see
 
   auto begin = [&](int i) {
-    const T* q = reinterpret_cast<const T*>(a.q) + (int64_t)qrow[i] * a.q_stride + (int64_t)head0 * HD;
+    if constexpr (MULTI) {
+      nrows = min(min(p.rows, p.cols - col0), count[i] * a.group - col0);
+      back_max = count[i] - 1;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) back[nt][e] = max(0, back_max - (col0 + nt * 8 + 2 * t + e) / a.group);
+      }
+    }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int h = nt * 8 + g;  // this lane: dims [HD / 4 * t, + HD / 4) of head h
+      const int h = nt * 8 + g;  // this lane: dims [HD / 4 * t, + HD / 4) of column h
       uint32_t raw[HD / 8];
       if (h < nrows) {
-        const T* qh = q + (int64_t)h * HD + HD / 4 * t;
+        const T* qh = d8_row<MULTI>(reinterpret_cast<const T*>(a.q), a.q_stride, a, qrow[i], kvh, col0 + h) + HD / 4 * t;
 #pragma unroll
         for (int u = 0; u < HD / 8; ++u) raw[u] = *reinterpret_cast<const uint32_t*>(qh + 2 * u);
       } else {
@@ -336,12 +367,12 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[u][nt][e] = fmaf(s[u][nt][e], f.x * qs[nt][e & 1], f.y);
       }
-      if (n < 16) {  // the end of the sequence, or a block that does not exist
+      if (n < 16 + (MULTI ? back_max : 0)) {  // the end of the sequence, or a block that does not exist
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (row_token(e < 2 ? g : g + 8) >= n) s[u][nt][e] = -INFINITY;
+            if (row_token(e < 2 ? g : g + 8) >= n - (MULTI ? back[nt][e & 1] : 0)) s[u][nt][e] = -INFINITY;
         }
       }
 #pragma unroll
@@ -405,6 +436,38 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
           *reinterpret_cast<uint4*>(w[k]) = *reinterpret_cast<const uint4*>(vt + (u * 16 + tok) * HD + ((g ^ (t << 1)) * 16));
         }
       }
+      if constexpr (MULTI) {
+        const int n = __float_as_int(info[st * SUBS + u].w);
+        if (n < 16 + back_max) {
+          // some columns do not see all of it: NaN codes stay out of the product and go to those that do
+          uint32_t any = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+#pragma unroll
+            for (int c = 0; c < HD / 32; ++c) {
+              const uint32_t nan = __vcmpeq4(w[k][c] & 0x7f7f7f7fu, 0x7f7f7f7fu);
+              w[k][c] &= ~nan;
+              any |= nan;
+            }
+          }
+          if (__any_sync(0xffffffffu, any != 0)) {
+            for (int tok = 0; tok < min(n, 16); ++tok) {
+              const uint8_t* row = vt + (u * 16 + tok) * HD +
+                                   (HD == 64 ? ((g >> 1) ^ (tok & 2)) * 16 + (g & 1) * 8 : (g ^ ((tok & 3) << 1)) * 16);
+#pragma unroll
+              for (int d = 0; d < HD / 8; ++d) {
+                if ((row[d] & 0x7f) != 0x7f) continue;
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+                  for (int e = 0; e < 2; ++e)
+                    if (tok < n - back[nt][e]) o[d >> 1][nt][e + 2 * (d & 1)] = __int_as_float(0x7fffffff);
+                }
+              }
+            }
+          }
+        }
+      }
 #pragma unroll
       for (int j = 0; j < HD / 16; ++j) {
         // rows g and g + 8 of M-tile j are dims HD / 8 * g + 2 j and the next
@@ -444,8 +507,8 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
     for (int x = threadIdx.x; x < p.hc * per_head; x += kD8Warps * 32) {
       const int c = x / per_head, h = x % per_head / (HD / 4), d = x % (HD / 4) * 4;
       const int v = blockIdx.y * p.hc + c, sub = v % p.subs;
-      if (sub * p.rows + h >= a.group) continue;
-      const int head = v / p.subs * a.group + sub * p.rows + h;
+      const int col = sub * p.rows + h, kv = v / p.subs;
+      if (col >= (MULTI ? count[i] * a.group : p.cols)) continue;
       float M = -INFINITY;
       for (int s = 0; s < p.ts; ++s) M = fmaxf(M, merge_ml[((s * p.hc + c) * NT * 8 + h) * 2]);
       float L = 0.f;
@@ -459,13 +522,13 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
       }
       if (whole) {
         const float inv = L == 0.f ? 0.f : 1.f / L;
-        T* out = reinterpret_cast<T*>(a.out) + (int64_t)qrow[i] * a.out_stride + (int64_t)head * HD + d;
+        T* out = d8_row<MULTI>(reinterpret_cast<T*>(a.out), a.out_stride, a, qrow[i], kv, col) + d;
         out[0] = Num<T>::from_f(O.x * inv);
         out[1] = Num<T>::from_f(O.y * inv);
         out[2] = Num<T>::from_f(O.z * inv);
         out[3] = Num<T>::from_f(O.w * inv);
       } else {
-        float* ps = p.partials + ((int64_t)(blockIdx.x + i) * a.hq + head) * (HD + 4);
+        float* ps = p.partials + ((int64_t)(blockIdx.x + i) * a.hkv * p.cols + kv * p.cols + col) * (HD + 4);
         *reinterpret_cast<float4*>(ps + d) = O;
         if (d == 0) *reinterpret_cast<float2*>(ps + HD) = make_float2(M, L);
       }
@@ -494,9 +557,9 @@ __global__ void __launch_bounds__(kD8Warps * 32, HD == 128 && NT == 2 ? 1 : 2) k
 }
 
 // Requests cut by a border: merge the CTAs' partials in order.  One CTA per
-// (request, query head); GROUPS groups of its threads take every GROUPS-th partial,
+// (request, column); GROUPS groups of its threads take every GROUPS-th partial,
 // all of a thread's loads go out together.  Requests without keys get zeros.
-template <int HD, int GROUPS, typename T>
+template <int HD, int GROUPS, bool MULTI, typename T>
 __global__ void __launch_bounds__(HD / 4 * GROUPS) kv8_decode_merge_kernel(const __grid_constant__ Kv8Args a,
                                                                            const __grid_constant__ D8Plan p) {
   constexpr int LANES = HD / 4;
@@ -509,9 +572,10 @@ __global__ void __launch_bounds__(HD / 4 * GROUPS) kv8_decode_merge_kernel(const
   const int r = a.req_list ? a.req_list[i] : i;
   if (r < 0 || r >= a.num_seqs) return;  // flagged by the first kernel
   if (a.table_rows && (a.table_rows[r] < 0 || a.table_rows[r] >= a.num_table_rows)) return;
-  const int64_t row = a.q_rows ? a.q_rows[r] : (int64_t)r;
-  if (row < 0 || row >= a.num_q_rows) return;
-  T* out = reinterpret_cast<T*>(a.out) + row * a.out_stride + (int64_t)h * HD;
+  const Kv8Rows rows = kv8_rows(a, r, nullptr);
+  const int col = h % p.cols;
+  if (rows.count <= 0 || (MULTI && (rows.count * a.group > p.cols || col >= rows.count * a.group))) return;
+  T* out = d8_row<MULTI>(reinterpret_cast<T*>(a.out), a.out_stride, a, (int)rows.first, h / p.cols, col);
   if (lo == hi) {
     if (group == 0) {
 #pragma unroll
@@ -521,8 +585,8 @@ __global__ void __launch_bounds__(HD / 4 * GROUPS) kv8_decode_merge_kernel(const
   }
   const int c0 = lo / W, n = (hi - 1) / W - c0 + 1;
   if (n == 1) return;
-  const float* base = p.partials + ((int64_t)(c0 + i) * a.hq + h) * (HD + 4);
-  const int64_t stride = (int64_t)a.hq * (HD + 4);
+  const float* base = p.partials + ((int64_t)(c0 + i) * a.hkv * p.cols + h) * (HD + 4);
+  const int64_t stride = (int64_t)a.hkv * p.cols * (HD + 4);
   constexpr int K = 5;
   float M = -INFINITY, L = 0.f;
   float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -590,13 +654,13 @@ bool kv8_decode_takes(int dtype, const Kv8Args& a) {
          aligned(a.q, 4) && a.q_stride % 2 == 0 && a.hq <= 65535;
 }
 
-template <int HD, int NT, typename T>
+template <int HD, int NT, bool MULTI, typename T>
 static int launch_decode(const Kv8Args& a, const D8Plan& p, dim3 grid, int sms, bool overlap, cudaStream_t s) {
   constexpr int SUBS = 2048 / HD / 16;
   const size_t smem = (size_t)kD8Warps * kD8Stages * (kD8Stage + SUBS * 16) +
-                      (size_t)kD8Warps * NT * 8 * (HD + 4 + 2) * sizeof(float) + (size_t)(4 * p.num_req + 1) * sizeof(int);
-  auto* kernel = kv8_decode_kernel<HD, NT, T>;
-  const int rc = opt_in_smem(kSmemKv8Decode + (HD == 128) * 4 + (NT == 2) * 2 + std::is_same<T, __half>::value,
+                      (size_t)kD8Warps * NT * 8 * (HD + 4 + 2) * sizeof(float) + (size_t)((4 + MULTI) * p.num_req + 1) * sizeof(int);
+  auto* kernel = kv8_decode_kernel<HD, NT, MULTI, T>;
+  const int rc = opt_in_smem(kSmemKv8Decode + MULTI * 6 + (HD == 128 ? 4 : (NT == 2) * 2) + std::is_same<T, __half>::value,
                              (const void*)kernel, smem);
   if (rc != NIE_OK) return rc;
   if (overlap) {
@@ -612,16 +676,33 @@ static int launch_decode(const Kv8Args& a, const D8Plan& p, dim3 grid, int sms, 
   // take them in one round of loads, and more of the small CTAs are on the GPU at once.  In all, 64 requests of
   // 29600 keys x 32 heads take 169.2 us with 4 groups and 173.2 with 16; 16 of 4001 keys 16.9 and 16.35; one of
   // 131072 keys 46.1 and 35.9 (34.7 with 32, which costs the other two 2 and 7 us).
-  const dim3 merge_grid((unsigned)p.num_req, (unsigned)a.hq);
-  if (p.num_req * a.hq > 4 * sms)
-    pdl_launch(kv8_decode_merge_kernel<HD, 4, T>, merge_grid, dim3(HD), s, a, p);
+  const dim3 merge_grid((unsigned)p.num_req, (unsigned)(a.hkv * p.cols));
+  if ((int64_t)p.num_req * a.hkv * p.cols > 4 * sms)
+    pdl_launch(kv8_decode_merge_kernel<HD, 4, MULTI, T>, merge_grid, dim3(HD), s, a, p);
   else
-    pdl_launch(kv8_decode_merge_kernel<HD, 16, T>, merge_grid, dim3(HD * 4), s, a, p);
+    pdl_launch(kv8_decode_merge_kernel<HD, 16, MULTI, T>, merge_grid, dim3(HD * 4), s, a, p);
   return check_launch("kv8_decode_merge_kernel");
 }
 
-int launch_kv8_decode(int dtype, const Kv8Args& args, int num_requests, int sms, void* workspace, bool overlap,
-                      cudaStream_t s) {
+// Columns to a kv head and how many of them a warp takes: up to 16 share a warp's pass over the codes at head_dim 64;
+// 8 at 128, where 16 leave registers for one CTA to an SM.  8 requests of 16000 keys, 20 columns: 72.8 us with 8 to a
+// warp and 85.4 with 16 at head_dim 128, 68.2 and 66.0 at 64; one of 2000 keys: 13.7 and 16.1, 11.6 and 13.2.
+static void d8_columns(D8Plan& p, const Kv8Args& a, int max_query_len) {
+  p.cols = a.group * max_query_len;
+  const int most = a.hd == 64 ? 16 : 8;
+  p.subs = (p.cols + most - 1) / most;
+  p.rows = (p.cols + p.subs - 1) / p.subs;
+  const int sets = a.hkv * p.subs;
+  // Two column sets to a CTA halve the warps that are merged per set.  64 requests of 29600 keys, 8 sets: 178.7 us
+  // with one, 173.1 with two, 174.2 and 176 with four and eight; one of 131072 keys: 33.9, 35.9, 40.2, 40.1.
+  p.hc = sets % 2 == 0 ? 2 : 1;
+  p.ts = kD8Warps / p.hc;
+  p.min_tiles = p.ts;
+}
+
+template <bool MULTI>
+static int run_decode(int dtype, const Kv8Args& args, int num_requests, int max_query_len, int sms, void* workspace,
+                      bool overlap, cudaStream_t s) {
   Kv8Args a = args;
   for (int at = 0; at < num_requests; at += kD8MaxReq) {
     D8Plan p{};
@@ -635,7 +716,9 @@ int launch_kv8_decode(int dtype, const Kv8Args& args, int num_requests, int sms,
         a.num_seqs -= kD8MaxReq;
         if (a.table_rows) a.table_rows += kD8MaxReq;
         else a.tables += kD8MaxReq * a.tstride, a.num_table_rows -= kD8MaxReq;
-        if (a.q_rows) {
+        if (MULTI) {
+          a.qsl += kD8MaxReq;
+        } else if (a.q_rows) {
           a.q_rows += kD8MaxReq;
         } else {
           a.q = (const char*)a.q + kD8MaxReq * a.q_stride * 2;
@@ -645,32 +728,45 @@ int launch_kv8_decode(int dtype, const Kv8Args& args, int num_requests, int sms,
       }
       overlap = false;  // the kernel before is this function's own, which reads the same workspace
     }
-    // up to 16 query heads share a warp's pass over the codes; wider groups take several
-    p.subs = (a.group + 15) / 16;
-    p.rows = (a.group + p.subs - 1) / p.subs;
-    const int heads = a.hkv * p.subs;
-    p.hc = heads % 2 == 0 ? 2 : 1;
-    p.ts = kD8Warps / p.hc;
-    p.min_tiles = p.ts;
+    d8_columns(p, a, max_query_len);
     // Where the tables hold 1024 keys at most, a CTA takes a request (at most 8 tiles to a warp) and no second
     // launch is needed: 100 keys take 5.6 us and one launch, against 7.2 us and two.
     p.whole = a.tstride * a.bs <= 1024;
-    const int ctas = p.whole ? p.num_req : std::max(1, 2 * sms / (heads / p.hc));
+    const int sets = a.hkv * p.subs / p.hc;
+    const int ctas = p.whole ? p.num_req : std::max(1, 2 * sms / sets);
     p.cum_out = (int32_t*)workspace;
     p.partials = (float*)((char*)workspace + d8_header(std::min(num_requests, kD8MaxReq)));
-    const dim3 grid((unsigned)ctas, (unsigned)(heads / p.hc));
-    const bool half = dtype == NIE_DTYPE_F16, wide = p.rows > 8;
-    int rc;
-    if (a.hd == 64) {
-      if (half) rc = wide ? launch_decode<64, 2, __half>(a, p, grid, sms, overlap, s) : launch_decode<64, 1, __half>(a, p, grid, sms, overlap, s);
-      else rc = wide ? launch_decode<64, 2, __nv_bfloat16>(a, p, grid, sms, overlap, s) : launch_decode<64, 1, __nv_bfloat16>(a, p, grid, sms, overlap, s);
-    } else {
-      if (half) rc = wide ? launch_decode<128, 2, __half>(a, p, grid, sms, overlap, s) : launch_decode<128, 1, __half>(a, p, grid, sms, overlap, s);
-      else rc = wide ? launch_decode<128, 2, __nv_bfloat16>(a, p, grid, sms, overlap, s) : launch_decode<128, 1, __nv_bfloat16>(a, p, grid, sms, overlap, s);
-    }
+    const dim3 grid((unsigned)ctas, (unsigned)sets);
+    const bool half = dtype == NIE_DTYPE_F16;
+    auto launch = [&](auto type) {
+      using T = decltype(type);
+      if (a.hd == 128) return launch_decode<128, 1, MULTI, T>(a, p, grid, sms, overlap, s);
+      return p.rows > 8 ? launch_decode<64, 2, MULTI, T>(a, p, grid, sms, overlap, s)
+                        : launch_decode<64, 1, MULTI, T>(a, p, grid, sms, overlap, s);
+    };
+    const int rc = half ? launch(__half()) : launch(__nv_bfloat16());
     if (rc != NIE_OK) return rc;
   }
   return NIE_OK;
+}
+
+int launch_kv8_decode(int dtype, const Kv8Args& a, int num_requests, int sms, void* workspace, bool overlap,
+                      cudaStream_t s) {
+  return run_decode<false>(dtype, a, num_requests, 1, sms, workspace, overlap, s);
+}
+
+bool kv8_short_takes(int dtype, const Kv8Args& a, int num_requests, int max_query_len, int sms, size_t workspace_bytes) {
+  if (!kv8_decode_takes(dtype, a) || (int64_t)max_query_len * a.group * a.hd > kD8ShortCols) return false;
+  D8Plan p{};
+  d8_columns(p, a, max_query_len);
+  const int R = std::min(num_requests, kD8MaxReq), ctas = std::max(1, 2 * sms / (a.hkv * p.subs / p.hc));
+  return a.hkv * p.cols <= 65535 &&
+         d8_header(R) + (size_t)(ctas + R) * a.hkv * p.cols * (a.hd + 4) * sizeof(float) <= workspace_bytes;
+}
+
+int launch_kv8_short(int dtype, const Kv8Args& a, int num_requests, int max_query_len, int sms, void* workspace,
+                     cudaStream_t s) {
+  return run_decode<true>(dtype, a, num_requests, max_query_len, sms, workspace, false, s);
 }
 
 }  // namespace nie

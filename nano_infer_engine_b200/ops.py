@@ -1261,7 +1261,9 @@ def varlen_attention_kv8(
 ) -> torch.Tensor:
     """:func:`varlen_attention` over an 8-bit cache: fp32 scores, softmax and sums, the output rounded once.
 
-    ``max_query_len`` sizes the launch; it need not be exact.  A row that sees no key gives zeros; rows
+    No request has more than ``max_query_len`` tokens; a short one is worth stating, since requests of a few
+    tokens (drafts to verify) have a form of their own.  Requests that have more raise the device error flag
+    there and are left out.  A row that sees no key gives zeros; rows
     of ``out`` that no request has are left as they were.
     """
     L, nb, bs, h, d = _kv8_geometry(key_cache, value_cache, key_scales, value_scales, layer)
@@ -1316,7 +1318,7 @@ def varlen_attention_kv8(
         need,
     )
     check(status, "nie_varlen_attention_kv8")
-    _count(kv8_launch_count(query.dtype, bs, d, R, None))
+    _count(kv8_launch_count(query.dtype, bs, d, R, block_tables.stride(0) * bs, int(max_query_len) * (query.shape[1] // h)))
     return out
 
 
@@ -1349,11 +1351,14 @@ def decode_launch_count(dtype: torch.dtype, block_size: int, kv_heads: int, head
     return 2 if fast else 1
 
 
-def kv8_launch_count(dtype: torch.dtype, block_size: int, head_dim: int, num_requests: int, max_keys: int | None) -> int:
-    """Kernels of one :func:`paged_decode_kv8` call whose tables hold ``max_keys`` keys, or (None) of one
-    :func:`varlen_attention_kv8` call: one and its merging kernel per 512 or 256 requests, or the generic one."""
+def kv8_launch_count(
+    dtype: torch.dtype, block_size: int, head_dim: int, num_requests: int, max_keys: int, columns: int | None = None
+) -> int:
+    """Kernels of one :func:`paged_decode_kv8` call whose tables hold ``max_keys`` keys, or of one
+    :func:`varlen_attention_kv8` call with ``columns`` (tokens x query heads) to a kv head: one, and its
+    merging kernel where a request is split, per 512 or 256 requests, or the generic one."""
     if dtype == torch.float32 or head_dim not in (64, 128) or block_size % 16:
         return 1
-    if max_keys is None:
+    if columns is not None and columns * head_dim > 4096:
         return 2 * -(-num_requests // 256)
     return (1 if max_keys <= 1024 else 2) * -(-num_requests // 512)

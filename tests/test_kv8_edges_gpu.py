@@ -199,3 +199,33 @@ def test_a_cache_whose_offsets_pass_31_and_32_bits(cuda):
     for a, b in zip(*results):
         assert torch.equal(a, b)
     ops().check_device_errors(cuda)
+
+
+SHORT = [
+    # lens, new, hq, hkv, hd, bs: few tokens to a request, at and around what one warp and the short form take
+    ([2000, 2004, 5, 1], [5, 1, 5, 1], 32, 8, 64, 16),
+    ([700, 16, 33], [16, 16, 2], 32, 8, 64, 16),  # 64 columns
+    ([700, 17, 33], [17, 17, 2], 32, 8, 64, 16),  # one token more
+    ([900, 8, 64], [8, 8, 3], 16, 4, 128, 32),
+    ([900, 9, 64], [9, 9, 3], 16, 4, 128, 32),
+    ([3, 0, 2, 100], [4, 2, 3, 0], 8, 2, 64, 16),  # more tokens than keys; no key; no token
+    ([5000], [3], 6, 2, 128, 16),
+    ([1100, 40], [7, 3], 5, 5, 64, 32),  # an odd number of column sets
+    ([1100, 40], [5, 3], 24, 1, 64, 16),  # a wide group: past the short form
+    ([260] * 70, [1 + i % 4 for i in range(70)], 16, 4, 64, 16),
+]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("case", range(len(SHORT)))
+def test_requests_of_a_few_tokens(cuda, case, dtype):
+    run_attention(cuda, dtype, *SHORT[case], seed=600 + case)
+
+
+def test_a_request_longer_than_the_call_says(cuda):
+    q, (kc, vc, ks, vs), tables, sl, want = run_attention(cuda, BF16, [300, 77], [6, 2], 8, 2, 64, 16, seed=640)
+    out = torch.full_like(q, 3.0)
+    ops().varlen_attention_kv8(q, kc, vc, ks, vs, 1, tables, sl, torch.tensor([0, 6, 8], device=cuda), 2, out=out)
+    with pytest.raises(RuntimeError):
+        ops().check_device_errors(cuda)
+    assert (out[:6] == 3.0).all() and close(out[6:8], want[6:8], BF16)
