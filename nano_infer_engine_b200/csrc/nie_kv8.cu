@@ -489,9 +489,11 @@ static void launch_append(const AppendArgs& a, cudaStream_t s) {
       at16(a.codes[0]) && at16(a.codes[1])) {
     const int64_t threads = a.q ? a.tokens * (a.hd / 2 / V) * ((a.hq + kQHeads - 1) / kQHeads) : 0;
     const int64_t q_ctas = (threads + 255) / 256;
-    // Few tokens are likely to lie in as many blocks: one to a CTA.  Many are prompts, whose 16 neighbours
-    // share one or two blocks: 16384 tokens in 5 requests take 29 us with 16 to a CTA, 36 us with one.
-    const int tile = a.tokens <= 2048 ? 1 : 16;
+    // Tokens to a CTA.  Few are likely to be of as many requests and lie in as many blocks, which a CTA takes in
+    // turn; many are of prompts, whose neighbours share blocks.  With 1, 8 and 16 to a CTA (8 kv heads of 64):
+    // 64 tokens of as many requests 4.0, 20 and 38 us, 512 12, 21 and 38, 2048 36, 34 and 56; of one prompt 512
+    // tokens 8.2, 6.5 and 5.1 us, 2048 16.7, 9.3 and 9.6, 16384 116, 60 and 56.
+    const int tile = a.tokens <= 512 ? 1 : a.tokens <= 4096 ? 8 : 16;
     const int64_t kv_ctas = 2 * ((a.tokens + tile - 1) / tile);
     if (q_ctas + kv_ctas < (int64_t(1) << 31)) {
       pdl_launch(append_kv8_vec_kernel<T>, dim3((unsigned)(q_ctas + kv_ctas)), dim3(256), s, a, (int)kv_ctas, tile);

@@ -22,7 +22,7 @@
 // (values that rise all the way) are gone through again, with the bound raised
 // after every load.
 //
-// Few rows are split over a cluster of up to 8 CTAs; the first one merges the
+// Few rows are split over a cluster of up to 4 CTAs; the first one merges the
 // others' sums and keys through distributed shared memory.
 #include <cooperative_groups.h>
 
@@ -39,7 +39,7 @@ constexpr int kLpWarps = kLpThreads / 32;
 constexpr int kLpMaxTop = 32;
 constexpr int kLpCap = 1024;      // keys of the buffer (a load of every thread and the k best fit)
 constexpr int kLpQueue = 512;     // loads that hold a value above the bound
-constexpr int kLpMaxCluster = 8;
+constexpr int kLpMaxCluster = 4;
 // Rows with larger values, or with none above its negative, are taken apart; a reference starts below.
 constexpr float kLpRange = 1.3e38f;
 constexpr float kLpLog2e = 1.4426950408889634f;
@@ -540,10 +540,12 @@ extern "C" int nie_token_logprobs(const void* logits, int64_t rows, int64_t cols
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   const int sms = sm_count(stream_device(s));
   NIE_REQUIRE(sms > 0, "cannot query the SM count");
-  // rows that do not fill the SMs (four CTAs each) are split, down to a round's worth of values
+  // Rows that do not bring a CTA to each SM are split, down to a round's worth of values.  128256 bf16 values, 5
+  // alternatives, in 1, 2, 4 and 8 parts: one row 17.4, 13.5, 11.5 and 11.4 us, 64 rows 17.8, 14.5, 13.5 and 16.2,
+  // 128 rows 17.9, 16.6, 18.3 and 29, 256 rows 22, 24, 33 and 54.
   const int64_t round = (int64_t)kLpThreads * 4 * (16 / dtype_size(dtype));
   int parts = 1;
-  while (parts < kLpMaxCluster && rows * parts * 2 <= 4 * sms && cols > parts * round) parts *= 2;
+  while (parts < kLpMaxCluster && rows * parts <= sms && cols > parts * round) parts *= 2;
   LogprobArgs a{logits, row_stride, (int)cols, tokens, top, logprobs, entropy, top_logprobs, top_ids, err_flag};
   switch (dtype) {
     case NIE_DTYPE_BF16: return launch_logprobs<__nv_bfloat16>(a, rows, parts, s);
