@@ -21,8 +21,11 @@
 //
 // What bounds it: each byte in and out once, some 60 operations to 16 of them, so
 // bandwidth from a few thousand tokens on and latency below.  One kernel does all:
-// some CTAs rotate queries, the others store; rows move in 16-byte pieces and a
-// run of up to 2 pairs of pieces a lane stays in registers between its maximum and its codes.
+// some CTAs rotate queries, the others store; rows move in 16-byte pieces, and a lane's
+// first pair of them stays in registers between the run's maximum and its codes.
+// Registers decide: with two pairs and four CTAs to an SM the loops' state went to
+// memory and 16384 tokens (32 + 2 x 8 heads of 64, bf16) took 55 us; with one and
+// three CTAs 44 us, 185 MB at 4.2 TB/s, of which the queries' 134 MB take 24.
 //
 // One warp owns a (block, kv head, K or V) and takes the block's runs in turn,
 // as calls of their own would be, so no two warps write one scale or one code
@@ -201,8 +204,8 @@ template <typename T>
 struct Piece {
   static constexpr int V = 16 / (int)sizeof(T);
   float f[V];
-  __device__ __forceinline__ void load(const T* p) {
-    const uint4 u = *reinterpret_cast<const uint4*>(p);
+  __device__ __forceinline__ void load(const T* p) { expand(*reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void expand(const uint4 u) {
     const T* e = reinterpret_cast<const T*>(&u);
 #pragma unroll
     for (int i = 0; i < V; ++i) f[i] = Num<T>::to_f(e[i]);
@@ -225,17 +228,38 @@ struct Piece {
   }
 };
 
+// Rotation of a pair of pieces from the loaded words, so that no more of them than needed are values at a time.
 template <typename T>
-__device__ __forceinline__ void rotate_pieces(Piece<T>& a, Piece<T>& b, const Piece<T>& c, const Piece<T>& s) {
+__device__ __forceinline__ void rotate_raw(const uint4& a, const uint4& b, const uint4& c, const uint4& s, Piece<T>& x, Piece<T>& y) {
+  const T *pa = reinterpret_cast<const T*>(&a), *pb = reinterpret_cast<const T*>(&b);
+  const T *pc = reinterpret_cast<const T*>(&c), *ps = reinterpret_cast<const T*>(&s);
 #pragma unroll
   for (int i = 0; i < Piece<T>::V; ++i) {
-    const float x = a.f[i], y = b.f[i];
-    a.f[i] = __fsub_rn(__fmul_rn(x, c.f[i]), __fmul_rn(y, s.f[i]));
-    b.f[i] = __fadd_rn(__fmul_rn(y, c.f[i]), __fmul_rn(x, s.f[i]));
+    const float u = Num<T>::to_f(pa[i]), v = Num<T>::to_f(pb[i]), co = Num<T>::to_f(pc[i]), si = Num<T>::to_f(ps[i]);
+    x.f[i] = __fsub_rn(__fmul_rn(u, co), __fmul_rn(v, si));
+    y.f[i] = __fadd_rn(__fmul_rn(v, co), __fmul_rn(u, si));
   }
 }
 
-// settle_scale() with 16 codes a lane.
+// The codes of a block's rows [0, off) times ratio, 16 a lane.
+__device__ __noinline__ void rescale_codes(uint8_t* base, int64_t row, int hd, int off, float ratio) {
+  const int per_row = hd / 16;
+  for (int i = threadIdx.x & 31; i < off * per_row; i += 32) {
+    uint4* p = reinterpret_cast<uint4*>(base + (int64_t)(i / per_row) * row + i % per_row * 16);
+    uint4 u = *p;
+    uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float2 lo = f16x2_to_float2(e4m3x2_to_f16x2((uint16_t)(w[e] & 0xffffu)));
+      const float2 hi = f16x2_to_float2(e4m3x2_to_f16x2((uint16_t)(w[e] >> 16)));
+      w[e] = (uint32_t)floats_to_e4m3x2(lo.x * ratio, lo.y * ratio) |
+             ((uint32_t)floats_to_e4m3x2(hi.x * ratio, hi.y * ratio) << 16);
+    }
+    *p = u;
+  }
+}
+
+// settle_scale() on it.
 __device__ __forceinline__ float settle_scale_vec(const AppendArgs& a, int kv, int64_t block, int head, int off, float amax,
                                                   int lane) {
   float* sp = a.scales[kv] + block * a.hkv + head;
@@ -243,23 +267,8 @@ __device__ __forceinline__ float settle_scale_vec(const AppendArgs& a, int kv, i
   if (off > 0) {
     const float old = fminf(fmaxf(*sp, kScaleMin), kScaleMax);
     if (s > old) {
-      const float ratio = old / s;
       const int64_t row = (int64_t)a.hkv * a.hd;
-      const int per_row = a.hd / 16;
-      uint8_t* base = a.codes[kv] + block * a.bs * row + (int64_t)head * a.hd;
-      for (int i = lane; i < off * per_row; i += 32) {
-        uint4* p = reinterpret_cast<uint4*>(base + (int64_t)(i / per_row) * row + i % per_row * 16);
-        uint4 u = *p;
-        uint32_t* w = reinterpret_cast<uint32_t*>(&u);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 lo = f16x2_to_float2(e4m3x2_to_f16x2((uint16_t)(w[e] & 0xffffu)));
-          const float2 hi = f16x2_to_float2(e4m3x2_to_f16x2((uint16_t)(w[e] >> 16)));
-          w[e] = (uint32_t)floats_to_e4m3x2(lo.x * ratio, lo.y * ratio) |
-                 ((uint32_t)floats_to_e4m3x2(hi.x * ratio, hi.y * ratio) << 16);
-        }
-        *p = u;
-      }
+      rescale_codes(a.codes[kv] + block * a.bs * row + (int64_t)head * a.hd, row, a.hd, off, old / s);
     } else {
       s = old;
     }
@@ -275,8 +284,8 @@ constexpr int kQHeads = 4;  // query heads that a thread rotates with one piece 
 // blocks the warps take in turn; first, since theirs is the longer chain of loads.
 // The others: a thread rotates one pair of pieces of kQHeads heads of a token.
 template <typename T>
-__global__ void __launch_bounds__(256, 4) append_kv8_vec_kernel(const __grid_constant__ AppendArgs a, int kv_ctas, int tile) {
-  constexpr int V = Piece<T>::V, KEEP = 2;
+__global__ void __launch_bounds__(256, 3) append_kv8_vec_kernel(const __grid_constant__ AppendArgs a, int kv_ctas, int tile) {
+  constexpr int V = Piece<T>::V;
   pdl_wait();     // dependent launch: q/k/v come from the projection before
   pdl_trigger();  // the kernel after this one may start its prologue
   const int half = a.hd / 2, per_half = half / V;
@@ -291,52 +300,54 @@ __global__ void __launch_bounds__(256, 4) append_kv8_vec_kernel(const __grid_con
     const int c = e % per_half * V, h0 = e / per_half * kQHeads;
     const T* q = reinterpret_cast<const T*>(a.q) + t * a.q_stride + (int64_t)h0 * a.hd + c;
     T* out = reinterpret_cast<T*>(a.q_out) + (t * a.hq + h0) * a.hd + c;
-    Piece<T> lo[kQHeads], hi[kQHeads], co, si;
-    co.load(cs + t * half + c);
-    si.load(sn + t * half + c);
+    uint4 lo[kQHeads], hi[kQHeads];  // all loads go out together
 #pragma unroll
     for (int h = 0; h < kQHeads; ++h) {
       if (h0 + h < a.hq) {
-        lo[h].load(q + h * a.hd);
-        hi[h].load(q + h * a.hd + half);
+        lo[h] = *reinterpret_cast<const uint4*>(q + h * a.hd);
+        hi[h] = *reinterpret_cast<const uint4*>(q + h * a.hd + half);
       }
     }
+    const uint4 co = *reinterpret_cast<const uint4*>(cs + t * half + c), si = *reinterpret_cast<const uint4*>(sn + t * half + c);
 #pragma unroll
     for (int h = 0; h < kQHeads; ++h) {
       if (h0 + h < a.hq) {
-        rotate_pieces(lo[h], hi[h], co, si);
-        lo[h].store(out + h * a.hd);
-        hi[h].store(out + h * a.hd + half);
+        Piece<T> x, y;
+        rotate_raw(lo[h], hi[h], co, si, x, y);
+        x.store(out + h * a.hd);
+        y.store(out + h * a.hd + half);
       }
     }
     return;
   }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int kv = blockIdx.x & 1;
-  const int64_t t0 = (int64_t)(blockIdx.x >> 1) * tile;
+  const int t0 = (int)(blockIdx.x >> 1) * tile;
   // Lane i looks at token t0 - 1 + i, so that the tile's blocks and the runs at their
   // beginnings (16 tokens at least) follow from one load.
-  const int64_t seen = t0 - 1 + lane;
-  int64_t my_slot = -1, my_block = -1;
-  if (seen >= 0 && seen < a.tokens) {
-    my_slot = a.slots[seen];
-    my_block = block_of(a, seen);
-    if (lane >= 1 && lane <= tile && kv == 0 && my_slot >= a.total_slots) raise_flag(a.err, NIE_DEV_ERR_SLOT_RANGE);
+  const int seen = t0 - 1 + lane, tokens = (int)a.tokens;
+  int my_block = -1, my_off = 0;  // its block, and its place in it
+  if (seen >= 0 && seen < tokens) {
+    my_block = (int)block_of(a, seen);
+    if (my_block >= 0) my_off = (int)(a.slots[seen] - (int64_t)my_block * a.bs);
+    if (lane >= 1 && lane <= tile && kv == 0 && a.slots[seen] >= a.total_slots) raise_flag(a.err, NIE_DEV_ERR_SLOT_RANGE);
   }
-  const int64_t before_slot = __shfl_up_sync(0xffffffffu, my_slot, 1), before_block = __shfl_up_sync(0xffffffffu, my_block, 1);
+  const int before_off = __shfl_up_sync(0xffffffffu, my_off, 1), before_block = __shfl_up_sync(0xffffffffu, my_block, 1);
   bool begins = lane >= 1 && lane <= tile && my_block >= 0;
   if (begins && seen > 0) begins = before_block >= 0 ? before_block != my_block : begins_block(a, seen, my_block);
   const unsigned heads = __ballot_sync(0xffffffffu, begins) >> 1;  // bit i: token t0 + i
-  const unsigned goes_on = __ballot_sync(0xffffffffu, lane >= 1 && my_block >= 0 && my_block == before_block && my_slot == before_slot + 1);
+  const unsigned goes_on = __ballot_sync(0xffffffffu, lane >= 1 && my_block >= 0 && my_block == before_block && my_off == before_off + 1);
+  const int rank = __popc((heads << 1) & ((1u << lane) - 1));  // stretches that begin before this lane's token
   const int tasks = __popc(heads) * a.hkv;
   const int row_lanes = per_half, rows = 32 / row_lanes;  // lanes of a row, rows of a pass
   const int c = lane % row_lanes * V, sub = lane / row_lanes;
   const bool in = sub < rows;  // row_lanes need not divide 32
   const int64_t row = (int64_t)a.hkv * a.hd;
   for (int task = warp; task < tasks; task += 8) {
-    const int which = (int)__fns(heads, 0, task / a.hkv + 1);
+    const int nth = task / a.hkv;
+    const int which = __ffs(__ballot_sync(0xffffffffu, begins && rank == nth)) - 2;  // the lane behind it is token t0 + which
     const int64_t block = __shfl_sync(0xffffffffu, my_block, which + 1);
-    const int head = task % a.hkv;
+    const int head = task - nth * a.hkv;
     const bool rotate = kv == 0 && a.sin != nullptr;
     const T* src = reinterpret_cast<const T*>(kv ? a.v : a.k) + (int64_t)head * a.hd + c;
     const int64_t stride = kv ? a.v_stride : a.k_stride;
@@ -344,46 +355,52 @@ __global__ void __launch_bounds__(256, 4) append_kv8_vec_kernel(const __grid_con
     const unsigned stops = ~goes_on >> (which + 1) & ~1u;
     int n = stops ? __ffs(stops) - 1 : 32;
     const bool known = which + 1 + n < 32;
-    int off = (int)(__shfl_sync(0xffffffffu, my_slot, which + 1) - block * a.bs);
-    const int64_t behind = __shfl_sync(0xffffffffu, my_block, known ? which + 1 + n : 0);
-    const bool alone = known && (t0 + which + n >= a.tokens || (behind >= 0 && behind != block));
+    int off = __shfl_sync(0xffffffffu, my_off, which + 1);
+    const int behind = __shfl_sync(0xffffffffu, my_block, known ? which + 1 + n : 0);
+    const bool alone = known && (t0 + which + n >= tokens || (behind >= 0 && behind != (int)block));
     if (!known) n = run_length(a, t0 + which, block);
-    for (int64_t first = t0 + which; first >= 0;) {
+    for (int first = t0 + which; first >= 0;) {
+      bool strict = false;  // an infinite value is about: each value is looked at
       auto get = [&](int j, Piece<T>& lo, Piece<T>& hi) {
-        lo.load(src + (first + j) * stride);
-        hi.load(src + (first + j) * stride + half);
+        const T* x = src + (first + j) * stride;
+        const uint4 lo_raw = *reinterpret_cast<const uint4*>(x), hi_raw = *reinterpret_cast<const uint4*>(x + half);
         if (rotate) {
-          Piece<T> co, si;
-          co.load(cs + (first + j) * half + c);
-          si.load(sn + (first + j) * half + c);
-          rotate_pieces(lo, hi, co, si);
+          const int64_t at = (int64_t)(first + j) * half + c;
+          rotate_raw(lo_raw, hi_raw, *reinterpret_cast<const uint4*>(cs + at), *reinterpret_cast<const uint4*>(sn + at), lo, hi);
+        } else {
+          lo.expand(lo_raw);
+          hi.expand(hi_raw);
         }
+        if (strict) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          lo.f[i] = finite_or_nan(lo.f[i]);
-          hi.f[i] = finite_or_nan(hi.f[i]);
+          for (int i = 0; i < V; ++i) {
+            lo.f[i] = finite_or_nan(lo.f[i]);
+            hi.f[i] = finite_or_nan(hi.f[i]);
+          }
         }
       };
-      Piece<T> lo[KEEP], hi[KEEP];
-      float amax = 0.f;
-      auto largest = [&](const Piece<T>& p, const Piece<T>& q) {
+      Piece<T> lo, hi;  // the lane's first pair of pieces stays; further ones are read again
+      float amax;
+      for (;;) {
+        amax = 0.f;
+        auto largest = [&](const Piece<T>& p, const Piece<T>& q) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) amax = fmaxf(amax, fmaxf(fabsf(p.f[i]), fabsf(q.f[i])));  // skips NaN
-      };
-#pragma unroll
-      for (int u = 0; u < KEEP; ++u) {
-        const int j = u * rows + sub;
-        if (in && j < n) {
-          get(j, lo[u], hi[u]);
-          largest(lo[u], hi[u]);
+          for (int i = 0; i < V; ++i) amax = fmaxf(amax, fmaxf(fabsf(p.f[i]), fabsf(q.f[i])));  // skips NaN
+        };
+        if (in && sub < n) {
+          get(sub, lo, hi);
+          largest(lo, hi);
         }
+        for (int j = rows + sub; in && j < n; j += rows) {
+          Piece<T> p, q;
+          get(j, p, q);
+          largest(p, q);
+        }
+        amax = warp_max(amax);
+        if (strict || amax != INFINITY) break;
+        strict = true;
       }
-      for (int j = KEEP * rows + sub; in && j < n; j += rows) {
-        Piece<T> p, q;
-        get(j, p, q);
-        largest(p, q);
-      }
-      const float s = settle_scale_vec(a, kv, block, head, off, warp_max(amax), lane);
+      const float s = settle_scale_vec(a, kv, block, head, off, amax, lane);
       const uint32_t bits = __float_as_uint(s);
       const float inv = (bits & 0x7fffffu) == 0 ? __uint_as_float((254u << 23) - bits) : 0.f;
       uint8_t* dst = a.codes[kv] + (block * a.bs + off) * row + (int64_t)head * a.hd + c;
@@ -391,19 +408,15 @@ __global__ void __launch_bounds__(256, 4) append_kv8_vec_kernel(const __grid_con
         p.store_codes(dst + j * row, s, inv);
         q.store_codes(dst + j * row + half, s, inv);
       };
-#pragma unroll
-      for (int u = 0; u < KEEP; ++u) {
-        const int j = u * rows + sub;
-        if (in && j < n) put(j, lo[u], hi[u]);
-      }
-      for (int j = KEEP * rows + sub; in && j < n; j += rows) {
+      if (in && sub < n) put(sub, lo, hi);
+      for (int j = rows + sub; in && j < n; j += rows) {
         Piece<T> p, q;
         get(j, p, q);
         put(j, p, q);
       }
       if (alone) break;
       __syncwarp();
-      first = next_run(a, first + n, block);
+      first = (int)next_run(a, first + n, block);
       if (first >= 0) {
         n = run_length(a, first, block);
         off = (int)(a.slots[first] - block * a.bs);
@@ -486,13 +499,13 @@ static void launch_append(const AppendArgs& a, cudaStream_t s) {
   constexpr int V = Piece<T>::V;
   if (a.hd % 16 == 0 && a.hd / 2 % V == 0 && a.hd / 2 / V <= 32 && a.k_stride % V == 0 && a.v_stride % V == 0 &&
       (!a.q || a.q_stride % V == 0) && at16(a.q) && at16(a.k) && at16(a.v) && at16(a.sin) && at16(a.cos) && at16(a.q_out) &&
-      at16(a.codes[0]) && at16(a.codes[1])) {
+      at16(a.codes[0]) && at16(a.codes[1]) && a.tokens <= (1 << 30) && a.total_slots / a.bs < (int64_t(1) << 31)) {
     const int64_t threads = a.q ? a.tokens * (a.hd / 2 / V) * ((a.hq + kQHeads - 1) / kQHeads) : 0;
     const int64_t q_ctas = (threads + 255) / 256;
     // Tokens to a CTA.  Few are likely to be of as many requests and lie in as many blocks, which a CTA takes in
     // turn; many are of prompts, whose neighbours share blocks.  With 1, 8 and 16 to a CTA (8 kv heads of 64):
-    // 64 tokens of as many requests 4.0, 20 and 38 us, 512 12, 21 and 38, 2048 36, 34 and 56; of one prompt 512
-    // tokens 8.2, 6.5 and 5.1 us, 2048 16.7, 9.3 and 9.6, 16384 116, 60 and 56.
+    // 64 tokens of as many requests 3.6, 15 and 28 us, 512 9.4, 16 and 28, 4096 56, 46 and 57; of one prompt 512
+    // tokens 6.8, 5.4 and 4.5 us, 2048 14.8, 7.2 and 6.7, 16384 116, 49 and 44.
     const int tile = a.tokens <= 512 ? 1 : a.tokens <= 4096 ? 8 : 16;
     const int64_t kv_ctas = 2 * ((a.tokens + tile - 1) / tile);
     if (q_ctas + kv_ctas < (int64_t(1) << 31)) {
