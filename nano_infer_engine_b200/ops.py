@@ -914,7 +914,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
 
 # ------------------------------------------------------- 8-bit paged cache
 # Codes in e4m3, [layers, blocks, block_size, kv_heads, head_dim], and one fp32
-# scale per layer, block and kv head; the value of a code is code * scale.
+# scale per layer, block and kv head, in [2^-48, 2^48]; the value of a code is
+# code * scale.  The append writes powers of two; reading takes any scale in the range.
 KV8_DTYPE = torch.float8_e4m3fn
 
 
@@ -1147,8 +1148,9 @@ def _check_kv8_query(
     if out is not None and (out.shape != query.shape or out.dtype != query.dtype or out.stride(2) != 1
                             or out.stride(1) != d):
         raise ValueError("out must have the query's shape and dtype with contiguous rows")
-    if block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.stride(1) != 1:
-        raise ValueError("block_tables must be int32 [rows, stride] with contiguous rows")
+    if (block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.stride(1) != 1
+            or block_tables.stride(0) < block_tables.shape[1]):
+        raise ValueError("block_tables must be int32 [rows, stride] with contiguous rows that do not overlap")
     for name, t in (("seq_lens", seq_lens), ("table_rows", table_rows), ("req_list", req_list)):
         if t is not None and (t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous 1-D int32")

@@ -80,6 +80,7 @@ BAD_ATTENTION = [
     (dict(query=torch.zeros(2, 3, 64, dtype=BF16)), "multiple of kv_heads"),
     (dict(block_tables=torch.zeros(2, 3, dtype=torch.int64)), "block_tables"),
     (dict(block_tables=torch.zeros(1, 3, dtype=torch.int32)), "a row per request"),
+    (dict(block_tables=torch.zeros(1, 3, dtype=torch.int32).expand(2, 3)), "do not overlap"),
     (dict(seq_lens=torch.ones(2, dtype=torch.int64)), "seq_lens"),
     (dict(out=torch.zeros(2, 4, 64)), "out must"),
     (dict(out=torch.zeros(3, 4, 64, dtype=BF16)), "out must"),
