@@ -425,7 +425,8 @@ __global__ void __launch_bounds__(256, 3) append_kv8_vec_kernel(const __grid_con
   }
 }
 
-// Values of a table's first n tokens, 16 of K or V to a thread.
+// Values of a table's first n tokens, 16 of K or V to a thread: 16384 tokens of 8 heads of 64 as bf16 in 10.7 us (50
+// MB at 4.7 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(256) gather_kv8_vec_kernel(const uint8_t* __restrict__ kc, const uint8_t* __restrict__ vc,
                                                              const float* __restrict__ ks, const float* __restrict__ vs,

