@@ -33,7 +33,11 @@ __global__ void __launch_bounds__(kG8Warps * 32) kv8_generic_kernel(Kv8Args a) {
   __shared__ float sm_m[kG8Warps], sm_l[kG8Warps], sm_o[kG8Warps][kG8MaxHd];
 
   for (int64_t j = blockIdx.y; j < rows.count; j += gridDim.y) {
-    const int64_t keys = rows.keys + j + 1;  // this row sees the keys [0, keys)
+    int64_t keys = rows.keys + j + 1;  // this row sees the keys [0, keys)
+    if (keys > a.tstride * a.bs) {  // those past the end of the table have no block
+      if (threadIdx.x == 0) raise_flag(a.err, NIE_DEV_ERR_BLOCK_RANGE);
+      keys = a.tstride * a.bs;
+    }
     const T* qp = reinterpret_cast<const T*>(a.q) + (rows.first + j) * a.q_stride + (int64_t)h * a.hd;
     float q[kPer], o[kPer];
 #pragma unroll
@@ -44,8 +48,7 @@ __global__ void __launch_bounds__(kG8Warps * 32) kv8_generic_kernel(Kv8Args a) {
     }
     float m = -INFINITY, l = 0.f;
     for (int64_t p = warp; p < keys; p += kG8Warps) {
-      const int64_t lb = p / a.bs;
-      const int64_t block = lb < a.tstride ? (int64_t)table[lb] : -1;
+      const int64_t block = table[p / a.bs];
       if (block < 0 || block >= a.nb) {
         if (lane == 0) raise_flag(a.err, NIE_DEV_ERR_BLOCK_RANGE);
         continue;

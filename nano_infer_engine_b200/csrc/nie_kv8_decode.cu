@@ -135,19 +135,27 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
   int* len = cum + R + 1;
   int* trow = len + R;
   int* qrow = trow + R;
-  int* count = qrow + R;  // MULTI: query tokens
+  int* count = qrow + R;  // MULTI: query tokens,
+  int* behind = count + R;  // and the keys that the first of them does not see
   __shared__ int warp_sum[kD8Warps];
 
   pdl_trigger();  // the merging kernel may be staged now (it waits for this grid)
   // ---- lengths, tables and query rows of the requests; tiles before each
+  // Keys past the end of a table have no block.  (And no sum of tiles passes an int.)
+  const int64_t most = min(a.tstride * a.bs, (int64_t)((1 << 30) / R) * TOK);
   for (int i = threadIdx.x; i < R; i += kD8Warps * 32) {
     const int r = a.req_list ? a.req_list[i] : i;
-    int n = 0, tr = 0, qr = -1, c = 0;
+    int n = 0, tr = 0, qr = -1, c = 0, past = 0;
     if (r >= 0 && r < a.num_seqs) {
       tr = a.table_rows ? a.table_rows[r] : r;
       const Kv8Rows rows = kv8_rows(a, r, a.err);
       if (rows.count > 0 && tr >= 0 && tr < a.num_table_rows) {
         n = max(a.seq_lens[r], 0);
+        if (n > most) {
+          raise_flag(a.err, NIE_DEV_ERR_BLOCK_RANGE);
+          past = n - (int)most;
+          n = (int)most;
+        }
         qr = (int)rows.first;
         c = (int)rows.count;
         if (MULTI && rows.count * a.group > p.cols) n = 0, qr = -1, c = 0;  // longer than the call said
@@ -156,7 +164,10 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
       }
     }
     if (qr < 0) raise_flag(a.err, NIE_DEV_ERR_CAPACITY);
-    if constexpr (MULTI) count[i] = c;
+    if constexpr (MULTI) {
+      count[i] = c;
+      behind[i] = max(0, c - 1 - past);
+    }
     len[i] = n;
     trow[i] = tr;
     qrow[i] = qr;
@@ -286,7 +297,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
   auto begin = [&](int i) {
     if constexpr (MULTI) {
       nrows = min(min(p.rows, p.cols - col0), count[i] * a.group - col0);
-      back_max = count[i] - 1;
+      back_max = behind[i];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -661,7 +672,7 @@ template <int HD, int NT, bool MULTI, typename T>
 static int launch_decode(const Kv8Args& a, const D8Plan& p, dim3 grid, int sms, bool overlap, cudaStream_t s) {
   constexpr int SUBS = 2048 / HD / 16;
   const size_t smem = (size_t)kD8Warps * kD8Stages * (kD8Stage + SUBS * 16) +
-                      (size_t)kD8Warps * NT * 8 * (HD + 4 + 2) * sizeof(float) + (size_t)((4 + MULTI) * p.num_req + 1) * sizeof(int);
+                      (size_t)kD8Warps * NT * 8 * (HD + 4 + 2) * sizeof(float) + (size_t)((4 + 2 * MULTI) * p.num_req + 1) * sizeof(int);
   auto* kernel = kv8_decode_kernel<HD, NT, MULTI, T>;
   const int rc = opt_in_smem(kSmemKv8Decode + MULTI * 6 + (HD == 128 ? 4 : (NT == 2) * 2) + std::is_same<T, __half>::value,
                              (const void*)kernel, smem);

@@ -186,7 +186,10 @@ __device__ __noinline__ F8Req f8_request(const Kv8Args& a, int i, int32_t* err) 
   x.first = (int)rows.first;
   x.rows = (int)rows.count * a.group;
   x.ctx = (int)rows.keys;
-  x.n = max(a.seq_lens[r], 0);
+  // keys past the end of the table have no block
+  const int64_t most = min(a.tstride * a.bs, (int64_t)1 << 30), n = max(a.seq_lens[r], 0);
+  if (n > most) raise_flag(err, NIE_DEV_ERR_BLOCK_RANGE);
+  x.n = (int)min(n, most);
   x.trow = tr;
   return x;
 }
@@ -200,7 +203,7 @@ __device__ __forceinline__ int f8_tiles(const F8Req& x) {
 }
 template <class C>
 __device__ __forceinline__ int f8_keys(const F8Req& x, int group, int tile) {
-  return max(0, x.ctx + (min(x.rows, (tile + 1) * C::Rows) - 1) / group + 1);
+  return min(x.n, max(0, x.ctx + (min(x.rows, (tile + 1) * C::Rows) - 1) / group + 1));
 }
 template <class C>
 __device__ __forceinline__ int f8_key_tiles(int keys) {

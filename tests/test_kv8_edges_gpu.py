@@ -229,3 +229,29 @@ def test_a_request_longer_than_the_call_says(cuda):
     with pytest.raises(RuntimeError):
         ops().check_device_errors(cuda)
     assert (out[:6] == 3.0).all() and close(out[6:8], want[6:8], BF16)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("new", [None, [5, 9], [40, 70]])
+@pytest.mark.parametrize("length", [2**31 - 1, 2**31 - 70, 321])
+def test_a_length_past_the_table(cuda, new, length, dtype):
+    """Keys without a place in the table are flagged; those before them, and other requests, have their weight."""
+    lens = [320, 77]
+    q, (kc, vc, ks, vs), tables, sl, want = run_attention(cuda, dtype, lens, new, 8, 2, 64, 16, seed=700)
+    tables = tables[:, :20].contiguous()  # 320 keys
+    counts = new or [1, 1]
+    bad = torch.tensor([length, 77], dtype=torch.int32, device=cuda)
+    out = torch.zeros_like(q)
+    if new is None:
+        ops().paged_decode_kv8(q, kc, vc, ks, vs, 1, tables, bad, out=out)
+    else:
+        qsl = torch.tensor([0] + new).cumsum(0).to(cuda)
+        ops().varlen_attention_kv8(q, kc, vc, ks, vs, 1, tables, bad, qsl, max(new), out=out)
+    with pytest.raises(RuntimeError, match="block id outside the pool"):
+        ops().check_device_errors(cuda)
+    c, T = counts[0], sum(counts)
+    assert close(out[c:T], want[c:T], dtype)
+    seen = [min(320, length - c + 1 + j) for j in range(c)]
+    for j in {0, c // 2, c - 1}:
+        w, bound = plain.attention(q[j : j + 1], kc[1], vc[1], ks[1], vs[1], tables[0], seen[j], seen[j], 64**-0.5)
+        assert ((out[j].double() - w[0]).abs() <= step(dtype) * (w[0].abs() + bound[0]) + bound[0] + 1e-30).all()
