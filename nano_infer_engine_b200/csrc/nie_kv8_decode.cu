@@ -7,15 +7,17 @@
 // few enough to hide behind them.  Measured: 64 requests of up to 29600 keys, 8 kv
 // heads of 64, 171 us, 5.7 TB/s of codes; one of 131072 keys, 4 of 128, 36 us, 3.6
 // TB/s (27 us of it without any arithmetic, 6 in the merging kernel); 16 of up to
-// 4001 keys 16.5 us, mostly the two kernels' fixed parts.
+// 4001 keys 17 us, which the longest one's share of a cluster decides.
 //
 // Split.  The keys of all requests form one list of tiles (TOK tokens each, 4
 // KiB of codes per kv head); CTA c takes the c-th of equal stretches of it,
 // whatever the lengths, for HC kv heads, and deals the tiles of the stretch to
 // TS = 8 / HC warps in turn.  Warps merge per request through shared memory; a
 // request that lies in one CTA's stretch is finished there, one cut by a border
-// leaves (max, sum, unnormalised output) to a second kernel.  Every order of
-// summation follows from the lengths alone.
+// leaves (max, sum, unnormalised output) to a second kernel.  Where the tables are
+// short, a cluster of CTAs shares one request instead and merges in distributed
+// shared memory.  Every order of summation follows from the lengths and the
+// tables' width alone.
 //
 // One warp and tile.  cp.async brings the tile's codes to the warp's own ring of
 // two stages: no barrier between warps.  The products are transposed, so that
@@ -35,10 +37,14 @@
 // (11 bits, error 2^-12: below the output's own step) for the second product;
 // l takes it unrounded.  m is raised, and O and l rescaled, only when a tile
 // exceeds it by more than 2^8: p stays below 2^8, well inside f16.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <type_traits>
 
 #include "nie_kv8_attn.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace nie {
 
@@ -50,6 +56,7 @@ constexpr int kD8MaxReq = 512;     // requests of one launch (their lengths sit 
 // ragged kernel are filled well enough.  8 requests of 8 tokens behind 2000 keys, 32 heads on 8 of 64: 23.5 us here
 // and 49.2 there (of 16 tokens: 31.6 and 50.3); 16 on 4 of 128: 27.5 and 37.6 (38.3 and 38.9).
 constexpr int kD8ShortCols = 4096;
+constexpr int kD8MaxCluster = 8;
 constexpr float kD8Log2e = 1.4426950408889634f;
 constexpr float kD8Lazy = 8.f;
 
@@ -59,7 +66,7 @@ struct D8Plan {
   int cols;            // columns per kv head: its query heads, or (token, query head) pairs of the longest request
   int rows, subs;      // columns of one MMA column set; column sets per kv head
   int min_tiles;       // a CTA takes at least this many tiles
-  int whole;           // a CTA takes one request: nothing to merge
+  int whole, log2;     // a cluster of whole = 2^log2 CTAs takes one request, and no kernel has to merge (0: not so)
   float* partials;     // [ctas + num_req][hkv * cols][hd + 4]
   int32_t* cum_out;    // [num_req + 2]: tiles before each request, then tiles per CTA
 };
@@ -193,13 +200,18 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
   __syncthreads();
   const int total = cum[R];
   const int W = max((total + (int)gridDim.x - 1) / (int)gridDim.x, p.min_tiles);
-  const int lo = p.whole ? cum[blockIdx.x] : (int)min((int64_t)blockIdx.x * W, (int64_t)total);
-  const int hi = p.whole ? cum[blockIdx.x + 1] : min(total, lo + W);
+  int lo = (int)min((int64_t)blockIdx.x * W, (int64_t)total), hi = min(total, lo + W);
+  const int mine = blockIdx.x >> p.log2, rank = blockIdx.x & (p.whole - 1);  // of a cluster
+  if (p.whole) {
+    const int n = cum[mine + 1] - cum[mine];
+    lo = cum[mine] + (n * rank >> p.log2);
+    hi = cum[mine] + (n * (rank + 1) >> p.log2);
+  }
   // Everything above reads the step's metadata; the codes, scales and queries
   // may come from the kernel before, and the workspace may be in use by it.
   pdl_wait();
   if (p.whole) {
-    if (lo == hi && qrow[blockIdx.x] >= 0) {  // a request without keys: zeros
+    if (p.whole == 1 && lo == hi && qrow[blockIdx.x] >= 0) {  // a request without keys: zeros
       for (int c = 0; c < p.hc; ++c) {
         const int v = blockIdx.y * p.hc + c, first = v % p.subs * p.rows;
         const int n = min(p.rows, (MULTI ? count[blockIdx.x] * a.group : a.group) - first) * HD;
@@ -212,7 +224,12 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
     for (int i = threadIdx.x; i <= R; i += kD8Warps * 32) p.cum_out[i] = cum[i];
     if (threadIdx.x == 0) p.cum_out[R + 1] = W;
   }
-  if (lo >= hi) return;
+  float* shared_part = reinterpret_cast<float*>(sm);  // [hc * rows][hd + 4] for the cluster, over the ring
+  if (lo >= hi) {
+    if (p.whole <= 1) return;
+    for (int x = threadIdx.x; x < p.hc * p.rows; x += kD8Warps * 32)
+      *reinterpret_cast<float2*>(shared_part + x * (HD + 4) + HD) = make_float2(-INFINITY, 0.f);
+  }
 
   auto locate = [&](int x) {
     int l = 0, h = R;  // cum[l] <= x < cum[h]
@@ -534,7 +551,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
         L += merge_ml[w * 2 + 1] * f;
         O.x += y.x * f, O.y += y.y * f, O.z += y.z * f, O.w += y.w * f;
       }
-      if (whole) {
+      if (whole && p.whole <= 1) {
         const float inv = L == 0.f ? 0.f : 1.f / L;
         T* out = d8_row<MULTI>(reinterpret_cast<T*>(a.out), a.out_stride, a, qrow[i], kv, col) + d;
         out[0] = Num<T>::from_f(O.x * inv);
@@ -542,7 +559,8 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
         out[2] = Num<T>::from_f(O.z * inv);
         out[3] = Num<T>::from_f(O.w * inv);
       } else {
-        float* ps = p.partials + ((int64_t)(blockIdx.x + i) * a.hkv * p.cols + kv * p.cols + col) * (HD + 4);
+        float* ps = p.whole ? shared_part + (c * p.rows + h) * (HD + 4) :
+                    p.partials + ((int64_t)(blockIdx.x + i) * a.hkv * p.cols + kv * p.cols + col) * (HD + 4);
         *reinterpret_cast<float4*>(ps + d) = O;
         if (d == 0) *reinterpret_cast<float2*>(ps + HD) = make_float2(M, L);
       }
@@ -550,24 +568,61 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
     if (!last) __syncthreads();
   };
 
-  refill(0);
+  if (lo < hi) {
+    refill(0);
 #pragma unroll
-  for (int j = 0; j < kD8Stages - 1; ++j) issue(j);
-  int j = 0;
-  for (int i = locate(lo), at = lo; at < hi; ++i) {
-    if (cum[i + 1] == at) continue;  // a request without keys
-    const int end = min(hi, cum[i + 1]);
-    begin(i);
-    for (; j < items && first + j * p.ts < end; ++j) {
-      cp_wait<kD8Stages - 2>();
-      __syncwarp();  // the tile is there for every lane, and every lane is done with the stage that comes next
-      issue(j + kD8Stages - 1);
-      tile(j % kD8Stages);
+    for (int j = 0; j < kD8Stages - 1; ++j) issue(j);
+    int j = 0;
+    for (int i = locate(lo), at = lo; at < hi; ++i) {
+      if (cum[i + 1] == at) continue;  // a request without keys
+      const int end = min(hi, cum[i + 1]);
+      begin(i);
+      for (; j < items && first + j * p.ts < end; ++j) {
+        cp_wait<kD8Stages - 2>();
+        __syncwarp();  // the tile is there for every lane, and every lane is done with the stage that comes next
+        issue(j + kD8Stages - 1);
+        tile(j % kD8Stages);
+      }
+      finish(i, cum[i] >= lo && cum[i + 1] <= hi, end == hi);
+      at = end;
     }
-    finish(i, cum[i] >= lo && cum[i + 1] <= hi, end == hi);
-    at = end;
   }
   cp_wait<0>();
+  if (p.whole <= 1) return;
+  // ---- the cluster's CTAs to the output, each a share of it, in the order of their ranks
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  const int per_head = p.rows * (HD / 4);
+  for (int x = rank * (kD8Warps * 32) + threadIdx.x; x < p.hc * per_head; x += p.whole * (kD8Warps * 32)) {
+    const int c = x / per_head, h = x % per_head / (HD / 4), d = x % (HD / 4) * 4;
+    const int v = blockIdx.y * p.hc + c, col = v % p.subs * p.rows + h;
+    if (qrow[mine] < 0 || col >= (MULTI ? count[mine] * a.group : p.cols)) continue;
+    const float* at = shared_part + (c * p.rows + h) * (HD + 4);
+    float2 ml[kD8MaxCluster];
+    float M = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kD8MaxCluster; ++k) {
+      ml[k] = k < p.whole ? *reinterpret_cast<const float2*>(cluster.map_shared_rank(at, k) + HD) : make_float2(-INFINITY, 0.f);
+      M = fmaxf(M, ml[k].x);
+    }
+    float L = 0.f;
+    float4 O = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int k = 0; k < kD8MaxCluster; ++k) {
+      if (ml[k].x == -INFINITY && ml[k].y == 0.f) continue;  // no key; its output need not be there
+      const float f = merge_weight(ml[k].x, M);
+      const float4 y = *reinterpret_cast<const float4*>(cluster.map_shared_rank(at, k) + d);
+      L += ml[k].y * f;
+      O.x += y.x * f, O.y += y.y * f, O.z += y.z * f, O.w += y.w * f;
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    T* out = d8_row<MULTI>(reinterpret_cast<T*>(a.out), a.out_stride, a, qrow[mine], v / p.subs, col) + d;
+    out[0] = Num<T>::from_f(O.x * inv);
+    out[1] = Num<T>::from_f(O.y * inv);
+    out[2] = Num<T>::from_f(O.z * inv);
+    out[3] = Num<T>::from_f(O.w * inv);
+  }
+  cluster.sync();  // until the others have read
 }
 
 // Requests cut by a border: merge the CTAs' partials in order.  One CTA per
@@ -677,14 +732,25 @@ static int launch_decode(const Kv8Args& a, const D8Plan& p, dim3 grid, int sms, 
   const int rc = opt_in_smem(kSmemKv8Decode + MULTI * 6 + (HD == 128 ? 4 : (NT == 2) * 2) + std::is_same<T, __half>::value,
                              (const void*)kernel, smem);
   if (rc != NIE_OK) return rc;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kD8Warps * 32);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  cfg.attrs = attr;
   if (overlap) {
-    const cudaError_t e = launch_after_trigger(kernel, grid, dim3(kD8Warps * 32), smem, s, a, p);
-    if (e != cudaSuccess) return fail(NIE_ERR_CUDA, "kv8_decode_kernel launch: %s", cudaGetErrorString(e));
-  } else {
-    kernel<<<grid, kD8Warps * 32, smem, s>>>(a, p);
-    const int st = check_launch("kv8_decode_kernel");
-    if (st != NIE_OK) return st;
+    attr[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
   }
+  if (p.whole > 1) {
+    attr[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    attr[cfg.numAttrs].val.clusterDim.x = (unsigned)p.whole;
+    attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
+    ++cfg.numAttrs;
+  }
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, p);
+  if (e != cudaSuccess) return fail(NIE_ERR_CUDA, "kv8_decode_kernel launch: %s", cudaGetErrorString(e));
   if (p.whole) return NIE_OK;
   // A request is cut into 1 + grid.x / requests parts on average, so a large batch's requests into few: four groups
   // take them in one round of loads, and more of the small CTAs are on the GPU at once.  In all, 64 requests of
@@ -712,6 +778,17 @@ static void d8_columns(D8Plan& p, const Kv8Args& a, int max_query_len) {
   p.hc = sets % 2 == 0 ? 2 : 1;
   p.ts = kD8Warps / p.hc;
   p.min_tiles = p.ts;
+}
+
+// Where the tables hold few keys, a cluster of CTAs takes a request and needs no second launch: one CTA, more while
+// there are SMs for them and 256 keys to each.  With at most 1024 keys to a CTA one request of 100 keys takes 5.6 us
+// against 7.2 in two launches, 8 of 2000 11.8 and 12.3, 32 of 2000 19.3 and 23.0, 8 x 5 drafts behind up to 2000 16.1
+// and 19.1; requests of very uneven length lose by it (16 of 1 to 4001 keys 17.3 and 16.5, one launch less).
+static int d8_cluster_log2(int64_t keys, int num_req, int sets, int sms) {
+  const int64_t room = 2 * sms / ((int64_t)num_req * sets);
+  int log2 = 0;
+  while ((1 << log2) < kD8MaxCluster && (2 << log2) <= room && keys > (256 << log2)) ++log2;
+  return keys > (1024 << log2) ? -1 : log2;
 }
 
 template <bool MULTI>
@@ -743,11 +820,11 @@ static int run_decode(int dtype, const Kv8Args& args, int num_requests, int max_
       overlap = false;  // the kernel before is this function's own, which reads the same workspace
     }
     d8_columns(p, a, max_query_len);
-    // Where the tables hold 1024 keys at most, a CTA takes a request (at most 8 tiles to a warp) and no second
-    // launch is needed: 100 keys take 5.6 us and one launch, against 7.2 us and two.
-    p.whole = a.tstride * a.bs <= 1024;
     const int sets = a.hkv * p.subs / p.hc;
-    const int ctas = p.whole ? p.num_req : std::max(1, 2 * sms / sets);
+    p.log2 = d8_cluster_log2(a.tstride * a.bs, p.num_req, sets, sms);
+    p.whole = p.log2 < 0 ? 0 : 1 << p.log2;
+    p.log2 = std::max(p.log2, 0);
+    const int ctas = p.whole ? p.num_req * p.whole : std::max(1, 2 * sms / sets);
     p.cum_out = (int32_t*)workspace;
     p.partials = (float*)((char*)workspace + d8_header(std::min(num_requests, kD8MaxReq)));
     const dim3 grid((unsigned)ctas, (unsigned)sets);

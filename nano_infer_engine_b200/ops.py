@@ -1239,7 +1239,7 @@ def paged_decode_kv8(
         int(overlap),
     )
     check(status, "nie_paged_decode_kv8")
-    _count(kv8_launch_count(query.dtype, bs, d, R, block_tables.stride(0) * bs))
+    _count(kv8_launch_count(query.dtype, bs, d, R, block_tables.stride(0) * bs, h, query.shape[1] // h, False, index))
     return out
 
 
@@ -1275,6 +1275,7 @@ def varlen_attention_kv8(
         raise ValueError("query_start_loc must be contiguous int64 with one boundary more than requests")
     if int(max_query_len) < 1:
         raise ValueError("max_query_len must be positive")
+    max_query_len = min(int(max_query_len), max(1, query.shape[0]))
     code = dtype_code(query.dtype)
     index = _cuda_device(query, key_cache, value_cache, key_scales, value_scales, block_tables, seq_lens, query_start_loc,
                          out, table_rows, req_list)
@@ -1314,13 +1315,13 @@ def varlen_attention_kv8(
         query_start_loc.data_ptr(),
         _ptr(req_list),
         R,
-        int(max_query_len),
+        max_query_len,
         float(d**-0.5 if scale is None else scale),
         ws.data_ptr(),
         need,
     )
     check(status, "nie_varlen_attention_kv8")
-    _count(kv8_launch_count(query.dtype, bs, d, R, block_tables.stride(0) * bs, int(max_query_len) * (query.shape[1] // h)))
+    _count(kv8_launch_count(query.dtype, bs, d, R, block_tables.stride(0) * bs, h, max_query_len * (query.shape[1] // h), True, index))
     return out
 
 
@@ -1353,14 +1354,28 @@ def decode_launch_count(dtype: torch.dtype, block_size: int, kv_heads: int, head
     return 2 if fast else 1
 
 
+@functools.lru_cache(maxsize=1024)
 def kv8_launch_count(
-    dtype: torch.dtype, block_size: int, head_dim: int, num_requests: int, max_keys: int, columns: int | None = None
+    dtype: torch.dtype, block_size: int, head_dim: int, num_requests: int, max_keys: int, kv_heads: int, columns: int,
+    ragged: bool, index: int,
 ) -> int:
-    """Kernels of one :func:`paged_decode_kv8` call whose tables hold ``max_keys`` keys, or of one
-    :func:`varlen_attention_kv8` call with ``columns`` (tokens x query heads) to a kv head: one, and its
-    merging kernel where a request is split, per 512 or 256 requests, or the generic one."""
+    """Kernels of one :func:`paged_decode_kv8` or (``ragged``) :func:`varlen_attention_kv8` call on a device.
+
+    ``max_keys``: that the tables hold; ``columns``: (tokens x) query heads to a kv head.  One kernel and its
+    merging kernel per 256 requests of any length, or per 512 of a few tokens, where the tables are too long
+    for a cluster to a request; the generic kernel for what the others do not take."""
     if dtype == torch.float32 or head_dim not in (64, 128) or block_size % 16:
         return 1
-    if columns is not None and columns * head_dim > 4096:
+    if ragged and columns * head_dim > 4096:
         return 2 * -(-num_requests // 256)
-    return (1 if max_keys <= 1024 else 2) * -(-num_requests // 512)
+    sets = kv_heads * -(-columns // (16 if head_dim == 64 else 8))
+    sets = sets // 2 if sets % 2 == 0 else sets
+    places = 2 * int(lib.nie_device_sm_count(index))
+    total = 0
+    for at in range(0, num_requests, 512):
+        room = places // (min(512, num_requests - at) * sets)
+        ctas = 1
+        while ctas < 8 and 2 * ctas <= room and max_keys > 256 * ctas:
+            ctas *= 2
+        total += 1 if max_keys <= 1024 * ctas else 2
+    return total
