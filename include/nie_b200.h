@@ -478,12 +478,20 @@ int nie_gather_kv8(const void* key_cache, const void* value_cache,
  * (NIE_DEV_ERR_CAPACITY) and skipped.
  * head_dim <= 256.  The workspace (nie_paged_decode_kv8_workspace_size,
  * nie_varlen_kv8_workspace_size bytes, 256-byte aligned) holds partial sums of
- * one call; calls that share it must not overlap on the GPU.  overlap != 0: the kernel may start before the
+ * one call; it may be null where that is 0 (short tables).  Calls that share
+ * it must not overlap on the GPU.  overlap != 0: the kernel may start before the
  * previous kernel on the stream ends, as nie_paged_decode_overlapped, with its
  * precondition. */
 size_t nie_paged_decode_kv8_workspace_size(int device, int32_t num_requests,
-                                           int32_t q_heads, int32_t head_dim);
-size_t nie_varlen_kv8_workspace_size(int device, int32_t head_dim);
+                                           int32_t q_heads, int32_t kv_heads,
+                                           int32_t head_dim,
+                                           int32_t block_size,
+                                           int64_t table_stride);
+size_t nie_varlen_kv8_workspace_size(int device, int32_t num_requests,
+                                     int32_t q_heads, int32_t kv_heads,
+                                     int32_t head_dim, int32_t block_size,
+                                     int64_t table_stride,
+                                     int32_t max_query_len);
 
 int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* out,
                          int64_t out_row_stride, int64_t num_q_rows,

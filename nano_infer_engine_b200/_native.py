@@ -120,7 +120,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p]
         + [c_int64, c_void_p, c_void_p, c_int32, c_void_p, c_void_p],
     ),
-    "nie_paged_decode_kv8_workspace_size": (c_size_t, [c_int, c_int32, c_int32, c_int32]),
+    "nie_paged_decode_kv8_workspace_size": (c_size_t, [c_int, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64]),
     "nie_paged_decode_kv8": (
         c_int,
         [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32]
@@ -133,7 +133,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         + [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32]
         + [c_void_p, c_void_p, c_int32, c_int32, c_float, c_void_p, c_size_t, c_void_p, c_void_p],
     ),
-    "nie_varlen_kv8_workspace_size": (c_size_t, [c_int, c_int32]),
+    "nie_varlen_kv8_workspace_size": (
+        c_size_t,
+        [c_int, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32],
+    ),
     "nie_token_logprobs": (
         c_int,
         [c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]

@@ -133,6 +133,25 @@ static void to_layer(Kv8Args& a, int32_t layer) {
   a.group = a.hq / a.hkv;
 }
 
+// What the choice of a kernel and its workspace depend on, into a.
+static bool geometry(Kv8Args& a, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t block_size,
+                     int64_t table_stride) {
+  if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || block_size <= 0 || table_stride < 0)
+    return false;
+  a.hq = q_heads, a.hkv = kv_heads, a.hd = head_dim, a.bs = block_size, a.tstride = table_stride;
+  a.group = q_heads / kv_heads;
+  return true;
+}
+
+static size_t varlen_workspace(int sms, const Kv8Args& a, int num_requests, int max_query_len) {
+  return kv8_short_takes(sms, a, num_requests, max_query_len) ? kv8_decode_workspace(sms, a, num_requests, max_query_len)
+                                                              : kv8_prefill_workspace(sms, a.hd);
+}
+
+static bool holds(const void* workspace, size_t bytes, size_t need) {
+  return need == 0 || (workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 && bytes >= need);
+}
+
 }  // namespace nie
 
 using namespace nie;
@@ -162,8 +181,7 @@ extern "C" int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* o
   if (kv8_decode_takes(dtype, a)) {
     const int sms = sm_count(stream_device(s));
     NIE_REQUIRE(sms > 0, "cannot query the SM count");
-    NIE_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
-                    workspace_bytes >= kv8_decode_workspace(sms, num_requests, q_heads, head_dim),
+    NIE_REQUIRE(holds(workspace, workspace_bytes, kv8_decode_workspace(sms, a, num_requests, 1)),
                 "workspace too small or not 256-byte aligned");
     return launch_kv8_decode(dtype, a, num_requests, sms, workspace, overlap != 0, s);
   }
@@ -171,10 +189,12 @@ extern "C" int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* o
 }
 
 extern "C" size_t nie_paged_decode_kv8_workspace_size(int device, int32_t num_requests, int32_t q_heads,
-                                                      int32_t head_dim) {
+                                                      int32_t kv_heads, int32_t head_dim, int32_t block_size,
+                                                      int64_t table_stride) {
+  Kv8Args a{};
   const int sms = sm_count(device);
-  if (sms <= 0 || num_requests <= 0 || q_heads <= 0 || head_dim <= 0) return 0;
-  return kv8_decode_workspace(sms, num_requests, q_heads, head_dim);
+  if (sms <= 0 || num_requests <= 0 || !geometry(a, q_heads, kv_heads, head_dim, block_size, table_stride)) return 0;
+  return kv8_decode_workspace(sms, a, num_requests, 1);
 }
 
 extern "C" int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, void* out, int64_t out_row_stride,
@@ -198,23 +218,29 @@ extern "C" int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, voi
   const int rc = check_args(a, dtype, layer, num_layers, num_requests);
   if (rc != NIE_OK) return rc;
   NIE_REQUIRE(query_start_loc, "null pointer argument");
+  NIE_REQUIRE(max_query_len > 0, "max_query_len must be positive");
   if (num_requests == 0) return NIE_OK;
   to_layer(a, layer);
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   if (kv8_prefill_takes(dtype, a)) {
     const int sms = sm_count(stream_device(s));
     NIE_REQUIRE(sms > 0, "cannot query the SM count");
-    NIE_REQUIRE(workspace && (reinterpret_cast<uintptr_t>(workspace) & 255) == 0 &&
-                    workspace_bytes >= kv8_prefill_workspace(sms, head_dim),
+    NIE_REQUIRE(holds(workspace, workspace_bytes, varlen_workspace(sms, a, num_requests, max_query_len)),
                 "workspace too small or not 256-byte aligned");
-    if (kv8_short_takes(dtype, a, num_requests, max_query_len, sms, workspace_bytes))
+    if (kv8_short_takes(sms, a, num_requests, max_query_len))
       return launch_kv8_short(dtype, a, num_requests, max_query_len, sms, workspace, s);
     return launch_kv8_prefill(dtype, a, num_requests, sms, workspace, s);
   }
   return launch_kv8_generic(dtype, a, num_requests, max_query_len, s);
 }
 
-extern "C" size_t nie_varlen_kv8_workspace_size(int device, int32_t head_dim) {
+extern "C" size_t nie_varlen_kv8_workspace_size(int device, int32_t num_requests, int32_t q_heads, int32_t kv_heads,
+                                                int32_t head_dim, int32_t block_size, int64_t table_stride,
+                                                int32_t max_query_len) {
+  Kv8Args a{};
   const int sms = sm_count(device);
-  return sms <= 0 || head_dim <= 0 ? 0 : kv8_prefill_workspace(sms, head_dim);
+  if (sms <= 0 || num_requests <= 0 || max_query_len <= 0 ||
+      !geometry(a, q_heads, kv_heads, head_dim, block_size, table_stride))
+    return 0;
+  return varlen_workspace(sms, a, num_requests, max_query_len);
 }

@@ -56,14 +56,14 @@ __device__ __forceinline__ Kv8Rows kv8_rows(const Kv8Args& a, int r, int32_t* er
 }
 
 // The kernel of single tokens (nie_kv8_decode.cu), where kv8_decode_takes() says
-// so; workspace of kv8_decode_workspace() bytes, 256-byte aligned.
+// so; workspace of kv8_decode_workspace() bytes, 256-byte aligned (none where it is 0).
 bool kv8_decode_takes(int dtype, const Kv8Args& a);
-size_t kv8_decode_workspace(int sms, int num_requests, int q_heads, int head_dim);
+size_t kv8_decode_workspace(int sms, const Kv8Args& a, int num_requests, int max_query_len);
 int launch_kv8_decode(int dtype, const Kv8Args& a, int num_requests, int sms, void* workspace, bool overlap,
                       cudaStream_t s);
 
-// The same for requests of a few query tokens each (max_query_len at most), where kv8_short_takes().
-bool kv8_short_takes(int dtype, const Kv8Args& a, int num_requests, int max_query_len, int sms, size_t workspace_bytes);
+// The same for requests of a few query tokens each, max_query_len at most, where kv8_short_takes() them, too.
+bool kv8_short_takes(int sms, const Kv8Args& a, int num_requests, int max_query_len);
 int launch_kv8_short(int dtype, const Kv8Args& a, int num_requests, int max_query_len, int sms, void* workspace,
                      cudaStream_t s);
 

@@ -711,11 +711,6 @@ __global__ void __launch_bounds__(HD / 4 * GROUPS) kv8_decode_merge_kernel(const
 
 static size_t d8_header(int R) { return (((size_t)(R + 2) * sizeof(int32_t)) + 255) & ~size_t(255); }
 
-size_t kv8_decode_workspace(int sms, int num_requests, int q_heads, int head_dim) {
-  const int R = std::min(num_requests, kD8MaxReq);
-  return d8_header(R) + (size_t)(2 * sms + R) * q_heads * (head_dim + 4) * sizeof(float);
-}
-
 bool kv8_decode_takes(int dtype, const Kv8Args& a) {
   auto aligned = [](const void* p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
   return (dtype == NIE_DTYPE_BF16 || dtype == NIE_DTYPE_F16) && (a.hd == 64 || a.hd == 128) && a.bs % 16 == 0 &&
@@ -791,6 +786,16 @@ static int d8_cluster_log2(int64_t keys, int num_req, int sets, int sms) {
   return keys > (1024 << log2) ? -1 : log2;
 }
 
+// The split of p.num_req requests; CTAs to a column set.
+static int d8_split(D8Plan& p, const Kv8Args& a, int max_query_len, int sms) {
+  d8_columns(p, a, max_query_len);
+  const int sets = a.hkv * p.subs / p.hc;
+  p.log2 = d8_cluster_log2(a.tstride * a.bs, p.num_req, sets, sms);
+  p.whole = p.log2 < 0 ? 0 : 1 << p.log2;
+  p.log2 = std::max(p.log2, 0);
+  return p.whole ? p.num_req * p.whole : std::max(1, 2 * sms / sets);
+}
+
 template <bool MULTI>
 static int run_decode(int dtype, const Kv8Args& args, int num_requests, int max_query_len, int sms, void* workspace,
                       bool overlap, cudaStream_t s) {
@@ -819,12 +824,7 @@ static int run_decode(int dtype, const Kv8Args& args, int num_requests, int max_
       }
       overlap = false;  // the kernel before is this function's own, which reads the same workspace
     }
-    d8_columns(p, a, max_query_len);
-    const int sets = a.hkv * p.subs / p.hc;
-    p.log2 = d8_cluster_log2(a.tstride * a.bs, p.num_req, sets, sms);
-    p.whole = p.log2 < 0 ? 0 : 1 << p.log2;
-    p.log2 = std::max(p.log2, 0);
-    const int ctas = p.whole ? p.num_req * p.whole : std::max(1, 2 * sms / sets);
+    const int ctas = d8_split(p, a, max_query_len, sms), sets = a.hkv * p.subs / p.hc;
     p.cum_out = (int32_t*)workspace;
     p.partials = (float*)((char*)workspace + d8_header(std::min(num_requests, kD8MaxReq)));
     const dim3 grid((unsigned)ctas, (unsigned)sets);
@@ -846,13 +846,19 @@ int launch_kv8_decode(int dtype, const Kv8Args& a, int num_requests, int sms, vo
   return run_decode<false>(dtype, a, num_requests, 1, sms, workspace, overlap, s);
 }
 
-bool kv8_short_takes(int dtype, const Kv8Args& a, int num_requests, int max_query_len, int sms, size_t workspace_bytes) {
-  if (!kv8_decode_takes(dtype, a) || (int64_t)max_query_len * a.group * a.hd > kD8ShortCols) return false;
+size_t kv8_decode_workspace(int sms, const Kv8Args& a, int num_requests, int max_query_len) {
+  // of the first launch: the last one has fewer requests, and more CTAs to each
   D8Plan p{};
-  d8_columns(p, a, max_query_len);
-  const int R = std::min(num_requests, kD8MaxReq), ctas = std::max(1, 2 * sms / (a.hkv * p.subs / p.hc));
-  return a.hkv * p.cols <= 65535 &&
-         d8_header(R) + (size_t)(ctas + R) * a.hkv * p.cols * (a.hd + 4) * sizeof(float) <= workspace_bytes;
+  p.num_req = std::min(num_requests, kD8MaxReq);
+  const int ctas = d8_split(p, a, max_query_len, sms);
+  if (p.whole) return 0;
+  return d8_header(p.num_req) + (size_t)(ctas + p.num_req) * a.hkv * p.cols * (a.hd + 4) * sizeof(float);
+}
+
+bool kv8_short_takes(int sms, const Kv8Args& a, int num_requests, int max_query_len) {
+  return (a.hd == 64 || a.hd == 128) && (int64_t)max_query_len * a.group * a.hd <= kD8ShortCols &&
+         (int64_t)a.hq * max_query_len <= 65535 &&
+         kv8_decode_workspace(sms, a, num_requests, max_query_len) <= kv8_prefill_workspace(sms, a.hd);
 }
 
 int launch_kv8_short(int dtype, const Kv8Args& a, int num_requests, int max_query_len, int sms, void* workspace,

@@ -940,14 +940,8 @@ def _launch(index: int, entry, *args) -> int:
         return entry(*args, flag.data_ptr(), _stream(flag))
 
 
-@functools.lru_cache(maxsize=None)
-def _kv8_decode_workspace_bytes(index: int, num_requests: int, q_heads: int, head_dim: int) -> int:
-    return int(lib.nie_paged_decode_kv8_workspace_size(index, num_requests, q_heads, head_dim))
-
-
-@functools.lru_cache(maxsize=None)
-def _kv8_varlen_workspace_bytes(index: int, head_dim: int) -> int:
-    return int(lib.nie_varlen_kv8_workspace_size(index, head_dim))
+_kv8_decode_workspace_bytes = functools.lru_cache(maxsize=1024)(lib.nie_paged_decode_kv8_workspace_size)
+_kv8_varlen_workspace_bytes = functools.lru_cache(maxsize=1024)(lib.nie_varlen_kv8_workspace_size)
 
 
 def _kv8_geometry(
@@ -1201,9 +1195,10 @@ def paged_decode_kv8(
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if R == 0:
         return out
+    stride = block_tables.stride(0)
     # of this call alone: calls on other streams and captured graphs have their own
-    need = _kv8_decode_workspace_bytes(index, R, query.shape[1], d)
-    ws = torch.empty(need, dtype=torch.uint8, device=query.device)
+    need = _kv8_decode_workspace_bytes(index, R, query.shape[1], h, d, bs, stride)
+    ws = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     status = _launch(
         index,
         lib.nie_paged_decode_kv8,
@@ -1225,7 +1220,7 @@ def paged_decode_kv8(
         d,
         query.shape[1],
         block_tables.data_ptr(),
-        block_tables.stride(0),
+        stride,
         block_tables.shape[0],
         _ptr(table_rows),
         seq_lens.data_ptr(),
@@ -1234,12 +1229,12 @@ def paged_decode_kv8(
         _ptr(req_list),
         R,
         float(d**-0.5 if scale is None else scale),
-        ws.data_ptr(),
+        _ptr(ws),
         need,
         int(overlap),
     )
     check(status, "nie_paged_decode_kv8")
-    _count(kv8_launch_count(query.dtype, bs, d, R, block_tables.stride(0) * bs, h, query.shape[1] // h, False, index))
+    _count(kv8_launch_count(query.dtype, bs, d, R, stride * bs, h, query.shape[1] // h, False, index))
     return out
 
 
@@ -1283,9 +1278,10 @@ def varlen_attention_kv8(
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if R == 0:
         return out
+    stride = block_tables.stride(0)
     # of this call alone: calls on other streams and captured graphs have their own
-    need = _kv8_varlen_workspace_bytes(index, d)
-    ws = torch.empty(need, dtype=torch.uint8, device=query.device)
+    need = _kv8_varlen_workspace_bytes(index, R, query.shape[1], h, d, bs, stride, max_query_len)
+    ws = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     status = _launch(
         index,
         lib.nie_varlen_attention_kv8,
@@ -1307,7 +1303,7 @@ def varlen_attention_kv8(
         d,
         query.shape[1],
         block_tables.data_ptr(),
-        block_tables.stride(0),
+        stride,
         block_tables.shape[0],
         _ptr(table_rows),
         seq_lens.data_ptr(),
@@ -1317,11 +1313,12 @@ def varlen_attention_kv8(
         R,
         max_query_len,
         float(d**-0.5 if scale is None else scale),
-        ws.data_ptr(),
+        _ptr(ws),
         need,
     )
     check(status, "nie_varlen_attention_kv8")
-    _count(kv8_launch_count(query.dtype, bs, d, R, block_tables.stride(0) * bs, h, max_query_len * (query.shape[1] // h), True, index))
+    long = need == _kv8_varlen_workspace_bytes(index, R, query.shape[1], h, d, bs, stride, 2**31 - 1)
+    _count(kv8_launch_count(query.dtype, bs, d, R, stride * bs, h, max_query_len * (query.shape[1] // h), long, index))
     return out
 
 
@@ -1357,16 +1354,17 @@ def decode_launch_count(dtype: torch.dtype, block_size: int, kv_heads: int, head
 @functools.lru_cache(maxsize=1024)
 def kv8_launch_count(
     dtype: torch.dtype, block_size: int, head_dim: int, num_requests: int, max_keys: int, kv_heads: int, columns: int,
-    ragged: bool, index: int,
+    long: bool, index: int,
 ) -> int:
-    """Kernels of one :func:`paged_decode_kv8` or (``ragged``) :func:`varlen_attention_kv8` call on a device.
+    """Kernels of one :func:`paged_decode_kv8` or :func:`varlen_attention_kv8` (``long``: not the form of few
+    tokens) call on a device.
 
     ``max_keys``: that the tables hold; ``columns``: (tokens x) query heads to a kv head.  One kernel and its
     merging kernel per 256 requests of any length, or per 512 of a few tokens, where the tables are too long
     for a cluster to a request; the generic kernel for what the others do not take."""
     if dtype == torch.float32 or head_dim not in (64, 128) or block_size % 16:
         return 1
-    if ragged and columns * head_dim > 4096:
+    if long:
         return 2 * -(-num_requests // 256)
     sets = kv_heads * -(-columns // (16 if head_dim == 64 else 8))
     sets = sets // 2 if sets % 2 == 0 else sets

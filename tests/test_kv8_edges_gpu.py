@@ -255,3 +255,33 @@ def test_a_length_past_the_table(cuda, new, length, dtype):
     for j in {0, c // 2, c - 1}:
         w, bound = plain.attention(q[j : j + 1], kc[1], vc[1], ks[1], vs[1], tables[0], seen[j], seen[j], 64**-0.5)
         assert ((out[j].double() - w[0]).abs() <= step(dtype) * (w[0].abs() + bound[0]) + bound[0] + 1e-30).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_launches_are_counted(cuda, dtype):
+    """The count that the package keeps, against the profiler's."""
+    from nano_infer_engine_b200 import ops as module
+
+    cases = [([100], None, 64), ([1500] * 3, None, 64), ([5000] * 40, None, 64), ([30] * 600, None, 128),
+             ([2000] * 8, [5] * 8, 64), ([5000] * 40, [3] * 40, 64), ([300] * 3, [100] * 3, 128), ([40] * 300, [33] * 300, 64)]
+    for lens, new, hd in cases:
+        q, (kc, vc, ks, vs), tables, sl, _ = run_attention(cuda, dtype, lens, new, 8, 2, hd, 16, seed=800)
+        qsl = torch.tensor([0] + (new or [])).cumsum(0).to(cuda)
+
+        def call():
+            if new is None:
+                module.paged_decode_kv8(q, kc, vc, ks, vs, 1, tables, sl)
+            else:
+                module.varlen_attention_kv8(q, kc, vc, ks, vs, 1, tables, sl, qsl, max(new))
+
+        before = module.LAUNCHES
+        call()
+        counted = module.LAUNCHES - before
+        torch.cuda.synchronize()
+        with torch.profiler.profile(activities=[torch.profiler.ProfilerActivity.CUDA]) as prof:
+            call()
+            torch.cuda.synchronize()
+        if not prof.key_averages():
+            pytest.skip("the profiler sees no kernels here")
+        seen = sum(e.count for e in prof.key_averages() if "kv8" in e.key)
+        assert counted == seen, (lens[0], len(lens), new and new[0], hd)
