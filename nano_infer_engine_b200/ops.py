@@ -887,11 +887,12 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
     index = _cuda_device(logits, tokens)
     tokens = tokens.contiguous()
     device = logits.device
-    out = torch.empty((2, rows), dtype=torch.float32, device=device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+    entropy = torch.empty(rows, dtype=torch.float32, device=device)
     top_logprobs = torch.empty((rows, top), dtype=torch.float32, device=device)
     top_ids = torch.empty((rows, top), dtype=torch.int64, device=device)
     if rows == 0:
-        return TokenLogprobs(out[0], out[1], top_logprobs, top_ids)
+        return TokenLogprobs(logprobs, entropy, top_logprobs, top_ids)
     status = _launch(
         index,
         lib.nie_token_logprobs,
@@ -902,14 +903,14 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor, *, top: int = 0) 
         code,
         tokens.data_ptr(),
         top,
-        out.data_ptr(),
-        out.data_ptr() + 4 * rows,
+        logprobs.data_ptr(),
+        entropy.data_ptr(),
         top_logprobs.data_ptr(),
         top_ids.data_ptr(),
     )
     check(status, "nie_token_logprobs")
     _count()
-    return TokenLogprobs(out[0], out[1], top_logprobs, top_ids)
+    return TokenLogprobs(logprobs, entropy, top_logprobs, top_ids)
 
 
 # ------------------------------------------------------- 8-bit paged cache
