@@ -626,17 +626,17 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
 }
 
 // Requests cut by a border: merge the CTAs' partials in order.  One CTA per
-// (request, column); GROUPS groups of its threads take every GROUPS-th partial,
-// all of a thread's loads go out together.  Requests without keys get zeros.
-template <int HD, int GROUPS, bool MULTI, typename T>
-__global__ void __launch_bounds__(HD / 4 * GROUPS) kv8_decode_merge_kernel(const __grid_constant__ Kv8Args a,
+// (request, column, 4 LANES dims); GROUPS groups of its threads take every
+// GROUPS-th partial, all of a thread's loads go out together.  Requests without
+// keys get zeros.
+template <int HD, int GROUPS, int LANES, bool MULTI, typename T>
+__global__ void __launch_bounds__(LANES * GROUPS) kv8_decode_merge_kernel(const __grid_constant__ Kv8Args a,
                                                                            const __grid_constant__ D8Plan p) {
-  constexpr int LANES = HD / 4;
   __shared__ float4 so[GROUPS][LANES];
   __shared__ float sm_m[GROUPS], sm_l[GROUPS];
   pdl_wait();
   const int i = blockIdx.x, h = blockIdx.y;
-  const int group = threadIdx.x / LANES, d = threadIdx.x % LANES;
+  const int group = threadIdx.x / LANES, lane = threadIdx.x % LANES, d = blockIdx.z * LANES + lane;
   const int lo = p.cum_out[i], hi = p.cum_out[i + 1], W = p.cum_out[p.num_req + 1];
   const int r = a.req_list ? a.req_list[i] : i;
   if (r < 0 || r >= a.num_seqs) return;  // flagged by the first kernel
@@ -683,8 +683,8 @@ __global__ void __launch_bounds__(HD / 4 * GROUPS) kv8_decode_merge_kernel(const
     }
     M = mn;
   }
-  so[group][d] = O;
-  if (d == 0) {
+  so[group][lane] = O;
+  if (lane == 0) {
     sm_m[group] = M;
     sm_l[group] = L;
   }
@@ -698,7 +698,7 @@ __global__ void __launch_bounds__(HD / 4 * GROUPS) kv8_decode_merge_kernel(const
 #pragma unroll
   for (int k = 0; k < GROUPS; ++k) {
     const float f = merge_weight(sm_m[k], mn);
-    const float4 y = so[k][d];
+    const float4 y = so[k][lane];
     L += sm_l[k] * f;
     O.x += y.x * f, O.y += y.y * f, O.z += y.z * f, O.w += y.w * f;
   }
@@ -748,14 +748,14 @@ static int launch_decode(const Kv8Args& a, const D8Plan& p, dim3 grid, int sms, 
   if (e != cudaSuccess) return fail(NIE_ERR_CUDA, "kv8_decode_kernel launch: %s", cudaGetErrorString(e));
   if (p.whole) return NIE_OK;
   // A request is cut into 1 + grid.x / requests parts on average, so a large batch's requests into few: four groups
-  // take them in one round of loads, and more of the small CTAs are on the GPU at once.  In all, 64 requests of
-  // 29600 keys x 32 heads take 169.2 us with 4 groups and 173.2 with 16; 16 of 4001 keys 16.9 and 16.35; one of
-  // 131072 keys 46.1 and 35.9 (34.7 with 32, which costs the other two 2 and 7 us).
+  // take them in one round of loads, and more of the small CTAs are on the GPU at once.  64 requests of up to 29600
+  // keys x 32 heads take 169.2 us in all with 4 groups of a whole row and 173.2 with 16.  Few requests have many
+  // parts: one of 131072 keys takes 46.1 us with 4 groups, 36.4 with 16, 35.5 with 32 groups of 32 dims each.
   const dim3 merge_grid((unsigned)p.num_req, (unsigned)(a.hkv * p.cols));
   if ((int64_t)p.num_req * a.hkv * p.cols > 4 * sms)
-    pdl_launch(kv8_decode_merge_kernel<HD, 4, MULTI, T>, merge_grid, dim3(HD), s, a, p);
+    pdl_launch(kv8_decode_merge_kernel<HD, 4, HD / 4, MULTI, T>, merge_grid, dim3(HD), s, a, p);
   else
-    pdl_launch(kv8_decode_merge_kernel<HD, 16, MULTI, T>, merge_grid, dim3(HD * 4), s, a, p);
+    pdl_launch(kv8_decode_merge_kernel<HD, 32, 8, MULTI, T>, dim3(merge_grid.x, merge_grid.y, HD / 32), dim3(256), s, a, p);
   return check_launch("kv8_decode_merge_kernel");
 }
 
