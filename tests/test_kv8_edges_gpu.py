@@ -6,14 +6,16 @@ from __future__ import annotations
 import kv8_plain as plain
 import pytest
 import torch
-from test_kv8_gpu import BF16, F16, ops, run_attention, step
+from test_kv8_gpu import BF16, F16, ops, run_append, run_attention, step
+from test_logprobs_gpu import check as check_logprobs
 
 pytestmark = pytest.mark.gpu
 
 
 def close(got, want, dtype, slack=0.0):
-    """Two kernels' results of one formula: each is within a step of it, and within 2^-10 of the mean weight's
-    rounding (see kv8_plain.attention)."""
+    """Two results of one formula: each is off by half a step of the type and by 2^-11 of the weights' mass
+    sum p |v| (kv8_plain.attention), which is 1.3 on average here and below 4 where a few keys share the weight
+    (a single key's is exact): 2 * 2^-11 * 4 = 2^-8."""
     err = (got.double() - want.double()).abs()
     return bool((err <= 2 * step(dtype) * want.double().abs() + 2.0**-8 + slack).all())
 
@@ -285,3 +287,32 @@ def test_launches_are_counted(cuda, dtype):
             pytest.skip("the profiler sees no kernels here")
         seen = sum(e.count for e in prof.key_averages() if "kv8" in e.key)
         assert counted == seen, (lens[0], len(lens), new and new[0], hd)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_append_of_thousands_of_tokens(cuda, dtype):
+    """More than 4096: prompts that begin anywhere in a block, one of a single token, an infinite value in between."""
+    run_append(cuda, dtype, [3000, 1, 1203, 77], [5, 16, 31, 0], 4, 1, 64, 16, seed=900)
+
+    def poke(qkv, slots, total):
+        qkv[2000, ::7] = float("inf")
+        qkv[4100, ::5] = float("nan")
+        slots[700:703] = -1
+
+    run_append(cuda, dtype, [4000, 300], [5, 3], 2, 2, 64, 32, seed=901, poke=poke)
+
+
+def test_append_of_thousands_of_requests(cuda):
+    """A token each, 600 and 4200 of them: every one in a block of its own, some where the block begins."""
+    for n in (600, 4200):
+        run_append(cuda, BF16, [1] * n, [i % 19 for i in range(n)], 2, 1, 64, 16, seed=910)
+
+
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+def test_logprobs_of_rows_split_in_two_and_four(cuda, dtype):
+    for rows, vocab in ((100, 40001), (60, 40001), (149, 40001)):
+        g = torch.Generator(device=cuda).manual_seed(rows)
+        x = (torch.randn(rows, vocab, device=cuda, generator=g) * 4).to(dtype)
+        x[3] = float("-inf")
+        x[3, 39000] = 1.0
+        check_logprobs(x, torch.randint(0, vocab, (rows,), device=cuda, generator=g), 7)
