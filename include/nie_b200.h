@@ -467,7 +467,12 @@ int nie_gather_kv8(const void* key_cache, const void* value_cache,
 /* nie_paged_decode_kv8 / nie_varlen_attention_kv8: nie_paged_decode /
  * nie_varlen_attention over an 8-bit cache; q and out have `dtype` and
  * num_q_rows rows.  Scores, softmax and sums are fp32 and the output is
- * rounded once (the scores are not rounded to the activation's type).  A row
+ * rounded once (the scores are not rounded to the activation's type); but where
+ * tensor cores take them (bf16 / f16 queries, head_dim 64 or 128, block_size a
+ * multiple of 16) the softmax weights that multiply V are rounded to 11 bits, and
+ * a weight w of a block with scale vs loses bits below w vs = 2^-23 of the row's
+ * largest, all of them below 2^-34 (the sum that they are divided by is not
+ * rounded).  A row
  * that sees no key (seq_len 0) is zeros.  A request with a query row outside
  * [0, num_q_rows) raises NIE_DEV_ERR_CAPACITY and is skipped; a key whose block
  * is outside the pool raises NIE_DEV_ERR_BLOCK_RANGE.  seq_lens, table_rows and

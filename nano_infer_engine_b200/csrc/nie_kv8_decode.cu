@@ -33,10 +33,15 @@
 // Softmax with scales.  With c = ks scale log2(e) of a block, each key's weight
 // on the codes of V is 2^(S c + log2 vs): the running maximum is kept over
 // y = S c + log2 vs, p = 2^(y - m), O = sum p vcode and l = sum p / vs, so that
-// p keeps its bits where scales of blocks lie far apart.  p is rounded to f16
-// (11 bits, error 2^-12: below the output's own step) for the second product;
-// l takes it unrounded.  m is raised, and O and l rescaled, only when a tile
-// exceeds it by more than 2^8: p stays below 2^8, well inside f16.
+// what a block adds to O does not depend on how its scale and its codes share it.
+// p is rounded to f16 for the second product, an error of 2^-12 of it; l takes it
+// unrounded.  Next to a bf16 output's half step of 2^-9 that is nothing (1.6e-3 of the
+// output's size from 64 bits either way); next to f16's 2^-12 it is as much again (2.8e-4 from
+// 64 bits where an fp32 p leaves 2.1e-4).  What the rounding leaves, taken along in a second
+// product, costs 8 % of the time at 64 requests and 3 % at one of 131072 keys.
+// m is raised, and O and l rescaled, only when a p would pass 2^15 (the largest
+// is 2^9 then): f16 ends at 2^16, and so has the most room below.  Weights (times vs)
+// under 2^-23 of the largest lose bits, those under 2^-34 are in l alone.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -58,7 +63,7 @@ constexpr int kD8MaxReq = 512;     // requests of one launch (their lengths sit 
 constexpr int kD8ShortCols = 4096;
 constexpr int kD8MaxCluster = 8;
 constexpr float kD8Log2e = 1.4426950408889634f;
-constexpr float kD8Lazy = 8.f;
+constexpr float kD8Most = 15.f, kD8Up = 9.f;  // log2 of p: its most, and that of the key that raised m
 
 struct D8Plan {
   int num_req;
@@ -414,7 +419,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
     }
     bool raise = false;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) raise |= mx[nt][0] > m[nt][0] + kD8Lazy || mx[nt][1] > m[nt][1] + kD8Lazy;
+    for (int nt = 0; nt < NT; ++nt) raise |= mx[nt][0] > m[nt][0] + kD8Most || mx[nt][1] > m[nt][1] + kD8Most;
     if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -424,7 +429,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          x = fmaxf(x, m[nt][e]);
+          x = fmaxf(x - kD8Up, m[nt][e]);
           const float keep = x == m[nt][e] ? 1.f : fast_exp2(m[nt][e] - x);
           m[nt][e] = x;
           l[nt][e] *= keep;

@@ -1181,6 +1181,11 @@ def paged_decode_kv8(
 ) -> torch.Tensor:
     """:func:`paged_decode` over an 8-bit cache: fp32 scores, softmax and sums, the output rounded once.
 
+    bf16 and f16 queries with head_dim 64 or 128 and blocks of a multiple of 16 tokens go to tensor
+    cores: there the softmax weights are rounded to 11 bits before they multiply V (not in the sum
+    that they are divided by), and lose bits below 2^-23 of the largest (weight times its block's
+    scale of V), all of them below 2^-34.
+
     A request of length 0 gives zeros; rows of ``out`` that no request has are left as they were.
     ``overlap``: as in :func:`paged_decode`.
     """
@@ -1257,7 +1262,8 @@ def varlen_attention_kv8(
     num_requests: int | None = None,
     scale: float | None = None,
 ) -> torch.Tensor:
-    """:func:`varlen_attention` over an 8-bit cache: fp32 scores, softmax and sums, the output rounded once.
+    """:func:`varlen_attention` over an 8-bit cache: fp32 scores, softmax and sums, the output rounded once;
+    softmax weights as in :func:`paged_decode_kv8`.
 
     No request has more than ``max_query_len`` tokens; a short one is worth stating, since requests of a few
     tokens (drafts to verify) have a form of their own.  Requests that have more raise the device error flag
