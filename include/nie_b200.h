@@ -476,7 +476,9 @@ int nie_gather_kv8(const void* key_cache, const void* value_cache,
  * that sees no key (seq_len 0) is zeros.  A request with a query row outside
  * [0, num_q_rows) raises NIE_DEV_ERR_CAPACITY and is skipped; a key whose block
  * is outside the pool raises NIE_DEV_ERR_BLOCK_RANGE.  seq_lens, table_rows and
- * q_rows have num_seqs entries, block_tables num_table_rows rows; a request of
+ * q_rows have num_seqs entries, block_tables num_table_rows rows of table_width
+ * entries, table_stride >= table_width from one to the next; keys past a row's
+ * end raise NIE_DEV_ERR_BLOCK_RANGE and are left out.  A request of
  * req_list or a row of table_rows outside them is flagged and skipped likewise.
  * No request has more than max_query_len tokens: where that times the query
  * heads of a kv head times head_dim is 4096 at most, longer ones are flagged
@@ -491,11 +493,11 @@ size_t nie_paged_decode_kv8_workspace_size(int device, int32_t num_requests,
                                            int32_t q_heads, int32_t kv_heads,
                                            int32_t head_dim,
                                            int32_t block_size,
-                                           int64_t table_stride);
+                                           int64_t table_width);
 size_t nie_varlen_kv8_workspace_size(int device, int32_t num_requests,
                                      int32_t q_heads, int32_t kv_heads,
                                      int32_t head_dim, int32_t block_size,
-                                     int64_t table_stride,
+                                     int64_t table_width,
                                      int32_t max_query_len);
 
 int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* out,
@@ -506,9 +508,9 @@ int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* out,
                          int64_t num_blocks, int32_t block_size,
                          int32_t kv_heads, int32_t head_dim, int32_t q_heads,
                          const int32_t* block_tables, int64_t table_stride,
-                         int64_t num_table_rows, const int32_t* table_rows,
-                         const int32_t* seq_lens, int32_t num_seqs,
-                         const int64_t* q_rows, const int32_t* req_list,
+                         int64_t table_width, int64_t num_table_rows,
+                         const int32_t* table_rows, const int32_t* seq_lens,
+                         int32_t num_seqs, const int64_t* q_rows, const int32_t* req_list,
                          int32_t num_requests, float scale, void* workspace,
                          size_t workspace_bytes, int32_t overlap,
                          int32_t* err_flag, void* stream);
@@ -521,9 +523,10 @@ int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, void* out,
                              int64_t num_blocks, int32_t block_size,
                              int32_t kv_heads, int32_t head_dim,
                              int32_t q_heads, const int32_t* block_tables,
-                             int64_t table_stride, int64_t num_table_rows,
-                             const int32_t* table_rows, const int32_t* seq_lens,
-                             int32_t num_seqs, const int64_t* query_start_loc,
+                             int64_t table_stride, int64_t table_width,
+                             int64_t num_table_rows, const int32_t* table_rows,
+                             const int32_t* seq_lens, int32_t num_seqs,
+                             const int64_t* query_start_loc,
                              const int32_t* req_list, int32_t num_requests,
                              int32_t max_query_len, float scale,
                              void* workspace, size_t workspace_bytes,

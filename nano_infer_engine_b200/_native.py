@@ -124,14 +124,14 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "nie_paged_decode_kv8": (
         c_int,
         [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32]
-        + [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32]
-        + [c_void_p, c_void_p, c_int32, c_float, c_void_p, c_size_t, c_int32, c_void_p, c_void_p],
+        + [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p]
+        + [c_int32, c_void_p, c_void_p, c_int32, c_float, c_void_p, c_size_t, c_int32, c_void_p, c_void_p],
     ),
     "nie_varlen_attention_kv8": (
         c_int,
         [c_void_p, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32]
-        + [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int32]
-        + [c_void_p, c_void_p, c_int32, c_int32, c_float, c_void_p, c_size_t, c_void_p, c_void_p],
+        + [c_int64, c_int64, c_int32, c_int32, c_int32, c_int32, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p]
+        + [c_int32, c_void_p, c_void_p, c_int32, c_int32, c_float, c_void_p, c_size_t, c_void_p, c_void_p],
     ),
     "nie_varlen_kv8_workspace_size": (
         c_size_t,

@@ -34,9 +34,9 @@ __global__ void __launch_bounds__(kG8Warps * 32) kv8_generic_kernel(Kv8Args a) {
 
   for (int64_t j = blockIdx.y; j < rows.count; j += gridDim.y) {
     int64_t keys = rows.keys + j + 1;  // this row sees the keys [0, keys)
-    if (keys > a.tstride * a.bs) {  // those past the end of the table have no block
+    if (keys > a.twidth * a.bs) {  // those past the end of the table have no block
       if (threadIdx.x == 0) raise_flag(a.err, NIE_DEV_ERR_BLOCK_RANGE);
-      keys = a.tstride * a.bs;
+      keys = a.twidth * a.bs;
     }
     const T* qp = reinterpret_cast<const T*>(a.q) + (rows.first + j) * a.q_stride + (int64_t)h * a.hd;
     float q[kPer], o[kPer];
@@ -119,7 +119,7 @@ static int check_args(const Kv8Args& a, int32_t dtype, int32_t layer, int64_t nu
   NIE_REQUIRE(a.nb > 0 && a.bs > 0 && a.hkv > 0 && a.hd > 0 && a.hq > 0, "bad geometry");
   NIE_REQUIRE(a.hq % a.hkv == 0, "q_heads must be divisible by kv_heads");
   NIE_REQUIRE(num_requests >= 0, "num_requests must be non-negative");
-  NIE_REQUIRE(a.tstride > 0, "table_stride must be positive");
+  NIE_REQUIRE(a.twidth > 0 && a.tstride >= a.twidth, "table_width must be positive and at most table_stride");
   NIE_REQUIRE(a.num_q_rows >= 0 && a.num_table_rows >= 0 && a.num_seqs >= 0, "row counts must be non-negative");
   return NIE_OK;
 }
@@ -135,10 +135,10 @@ static void to_layer(Kv8Args& a, int32_t layer) {
 
 // What the choice of a kernel and its workspace depend on, into a.
 static bool geometry(Kv8Args& a, int32_t q_heads, int32_t kv_heads, int32_t head_dim, int32_t block_size,
-                     int64_t table_stride) {
-  if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || block_size <= 0 || table_stride < 0)
+                     int64_t table_width) {
+  if (q_heads <= 0 || kv_heads <= 0 || q_heads % kv_heads || head_dim <= 0 || block_size <= 0 || table_width < 0)
     return false;
-  a.hq = q_heads, a.hkv = kv_heads, a.hd = head_dim, a.bs = block_size, a.tstride = table_stride;
+  a.hq = q_heads, a.hkv = kv_heads, a.hd = head_dim, a.bs = block_size, a.twidth = table_width;
   a.group = q_heads / kv_heads;
   return true;
 }
@@ -161,8 +161,9 @@ extern "C" int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* o
                                     const float* key_scales, const float* value_scales, int32_t dtype, int32_t layer,
                                     int64_t num_layers, int64_t num_blocks, int32_t block_size, int32_t kv_heads,
                                     int32_t head_dim, int32_t q_heads, const int32_t* block_tables,
-                                    int64_t table_stride, int64_t num_table_rows, const int32_t* table_rows,
-                                    const int32_t* seq_lens, int32_t num_seqs, const int64_t* q_rows,
+                                    int64_t table_stride, int64_t table_width, int64_t num_table_rows,
+                                    const int32_t* table_rows, const int32_t* seq_lens, int32_t num_seqs,
+                                    const int64_t* q_rows,
                                     const int32_t* req_list, int32_t num_requests, float scale,
                                     void* workspace, size_t workspace_bytes, int32_t overlap, int32_t* err_flag,
                                     void* stream) {
@@ -170,7 +171,7 @@ extern "C" int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* o
   a.q = q, a.out = out, a.q_stride = q_row_stride, a.out_stride = out_row_stride, a.num_q_rows = num_q_rows;
   a.kc = (const uint8_t*)key_cache, a.vc = (const uint8_t*)value_cache, a.ks = key_scales, a.vs = value_scales;
   a.nb = num_blocks, a.bs = block_size, a.hkv = kv_heads, a.hd = head_dim, a.hq = q_heads;
-  a.tables = block_tables, a.tstride = table_stride, a.num_table_rows = num_table_rows, a.table_rows = table_rows;
+  a.tables = block_tables, a.tstride = table_stride, a.twidth = table_width, a.num_table_rows = num_table_rows, a.table_rows = table_rows;
   a.seq_lens = seq_lens, a.num_seqs = num_seqs, a.q_rows = q_rows, a.req_list = req_list;
   a.scale = scale, a.err = err_flag;
   const int rc = check_args(a, dtype, layer, num_layers, num_requests);
@@ -190,10 +191,10 @@ extern "C" int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* o
 
 extern "C" size_t nie_paged_decode_kv8_workspace_size(int device, int32_t num_requests, int32_t q_heads,
                                                       int32_t kv_heads, int32_t head_dim, int32_t block_size,
-                                                      int64_t table_stride) {
+                                                      int64_t table_width) {
   Kv8Args a{};
   const int sms = sm_count(device);
-  if (sms <= 0 || num_requests <= 0 || !geometry(a, q_heads, kv_heads, head_dim, block_size, table_stride)) return 0;
+  if (sms <= 0 || num_requests <= 0 || !geometry(a, q_heads, kv_heads, head_dim, block_size, table_width)) return 0;
   return kv8_decode_workspace(sms, a, num_requests, 1);
 }
 
@@ -202,9 +203,9 @@ extern "C" int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, voi
                                         const float* key_scales, const float* value_scales, int32_t dtype,
                                         int32_t layer, int64_t num_layers, int64_t num_blocks, int32_t block_size,
                                         int32_t kv_heads, int32_t head_dim, int32_t q_heads,
-                                        const int32_t* block_tables, int64_t table_stride, int64_t num_table_rows,
-                                        const int32_t* table_rows, const int32_t* seq_lens, int32_t num_seqs,
-                                        const int64_t* query_start_loc,
+                                        const int32_t* block_tables, int64_t table_stride, int64_t table_width,
+                                        int64_t num_table_rows, const int32_t* table_rows, const int32_t* seq_lens,
+                                        int32_t num_seqs, const int64_t* query_start_loc,
                                         const int32_t* req_list, int32_t num_requests, int32_t max_query_len,
                                         float scale, void* workspace, size_t workspace_bytes, int32_t* err_flag,
                                         void* stream) {
@@ -212,7 +213,7 @@ extern "C" int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, voi
   a.q = q, a.out = out, a.q_stride = q_row_stride, a.out_stride = out_row_stride, a.num_q_rows = num_q_rows;
   a.kc = (const uint8_t*)key_cache, a.vc = (const uint8_t*)value_cache, a.ks = key_scales, a.vs = value_scales;
   a.nb = num_blocks, a.bs = block_size, a.hkv = kv_heads, a.hd = head_dim, a.hq = q_heads;
-  a.tables = block_tables, a.tstride = table_stride, a.num_table_rows = num_table_rows, a.table_rows = table_rows;
+  a.tables = block_tables, a.tstride = table_stride, a.twidth = table_width, a.num_table_rows = num_table_rows, a.table_rows = table_rows;
   a.seq_lens = seq_lens, a.num_seqs = num_seqs, a.qsl = query_start_loc, a.req_list = req_list;
   a.scale = scale, a.err = err_flag;
   const int rc = check_args(a, dtype, layer, num_layers, num_requests);
@@ -235,12 +236,12 @@ extern "C" int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, voi
 }
 
 extern "C" size_t nie_varlen_kv8_workspace_size(int device, int32_t num_requests, int32_t q_heads, int32_t kv_heads,
-                                                int32_t head_dim, int32_t block_size, int64_t table_stride,
+                                                int32_t head_dim, int32_t block_size, int64_t table_width,
                                                 int32_t max_query_len) {
   Kv8Args a{};
   const int sms = sm_count(device);
   if (sms <= 0 || num_requests <= 0 || max_query_len <= 0 ||
-      !geometry(a, q_heads, kv_heads, head_dim, block_size, table_stride))
+      !geometry(a, q_heads, kv_heads, head_dim, block_size, table_width))
     return 0;
   return varlen_workspace(sms, a, num_requests, max_query_len);
 }

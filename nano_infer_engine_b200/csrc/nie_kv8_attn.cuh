@@ -19,7 +19,7 @@ struct Kv8Args {
   int64_t nb;
   int bs, hkv, hd, hq, group;
   const int32_t* tables;
-  int64_t tstride;
+  int64_t tstride, twidth;       // entries from one row to the next, entries of a row
   const int32_t* table_rows;
   const int32_t* seq_lens;
   const int64_t* q_rows;  // single-token calls: a request's query row (null: its index)

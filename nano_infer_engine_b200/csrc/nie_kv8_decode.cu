@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
   pdl_trigger();  // the merging kernel may be staged now (it waits for this grid)
   // ---- lengths, tables and query rows of the requests; tiles before each
   // Keys past the end of a table have no block.  (And no sum of tiles passes an int.)
-  const int64_t most = min(a.tstride * a.bs, (int64_t)((1 << 30) / R) * TOK);
+  const int64_t most = min(a.twidth * a.bs, (int64_t)((1 << 30) / R) * TOK);
   for (int i = threadIdx.x; i < R; i += kD8Warps * 32) {
     const int r = a.req_list ? a.req_list[i] : i;
     int n = 0, tr = 0, qr = -1, c = 0, past = 0;
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
       const int n = min(16, len[i] - tok);
       if (n > 0) {
         const int lb = tok / a.bs;
-        const int64_t block = lb < a.tstride ? (int64_t)a.tables[(int64_t)trow[i] * a.tstride + lb] : -1;
+        const int64_t block = lb < a.twidth ? (int64_t)a.tables[(int64_t)trow[i] * a.tstride + lb] : -1;
         if (block < 0 || block >= a.nb) {
           raise_flag(a.err, NIE_DEV_ERR_BLOCK_RANGE);
         } else {
@@ -795,7 +795,7 @@ static int d8_cluster_log2(int64_t keys, int num_req, int sets, int sms) {
 static int d8_split(D8Plan& p, const Kv8Args& a, int max_query_len, int sms) {
   d8_columns(p, a, max_query_len);
   const int sets = a.hkv * p.subs / p.hc;
-  p.log2 = d8_cluster_log2(a.tstride * a.bs, p.num_req, sets, sms);
+  p.log2 = d8_cluster_log2(a.twidth * a.bs, p.num_req, sets, sms);
   p.whole = p.log2 < 0 ? 0 : 1 << p.log2;
   p.log2 = std::max(p.log2, 0);
   return p.whole ? p.num_req * p.whole : std::max(1, 2 * sms / sets);

@@ -190,7 +190,7 @@ __device__ __noinline__ F8Req f8_request(const Kv8Args& a, int i, int32_t* err) 
   x.rows = (int)rows.count * a.group;
   x.ctx = (int)rows.keys;
   // keys past the end of the table have no block
-  const int64_t most = min(a.tstride * a.bs, (int64_t)1 << 30), n = max(a.seq_lens[r], 0);
+  const int64_t most = min(a.twidth * a.bs, (int64_t)1 << 30), n = max(a.seq_lens[r], 0);
   if (n > most) raise_flag(err, NIE_DEV_ERR_BLOCK_RANGE);
   x.n = (int)min(n, most);
   x.trow = tr;
@@ -290,7 +290,7 @@ template <typename T>
 __device__ __noinline__ void f8_put_nan(const Kv8Args& a, int trow, int h, int from, int to, T* out, int step) {
   for (int key = from; key < to; ++key) {
     const int lb = key / a.bs;
-    const int64_t block = lb < a.tstride ? (int64_t)a.tables[(int64_t)trow * a.tstride + lb] : -1;
+    const int64_t block = lb < a.twidth ? (int64_t)a.tables[(int64_t)trow * a.tstride + lb] : -1;
     if (block < 0 || block >= a.nb) continue;
     const uint8_t* codes = a.vc + ((block * a.bs + key % a.bs) * a.hkv + h) * a.hd;
     for (int d = 0; d < a.hd; ++d)
@@ -427,7 +427,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
         if (lane < C::Subs) count = min(16, min(ahead.keys, ahead.x.n) - key);
         const int lb = key / a.bs;
         offset = key - lb * a.bs;
-        entry = count > 0 && lb < a.tstride ? a.tables[(int64_t)ahead.x.trow * a.tstride + lb] : -1;
+        entry = count > 0 && lb < a.twidth ? a.tables[(int64_t)ahead.x.trow * a.tstride + lb] : -1;
       }
     };
     // scales of the next tile and of the one after it (first warp, lane s: the s-th 16 keys)

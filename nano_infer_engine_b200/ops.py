@@ -1145,7 +1145,7 @@ def _check_kv8_query(
         raise ValueError("out must have the query's shape and dtype with contiguous rows")
     if (block_tables.dtype != torch.int32 or block_tables.ndim != 2 or block_tables.stride(1) != 1
             or block_tables.stride(0) < block_tables.shape[1]):
-        raise ValueError("block_tables must be int32 [rows, stride] with contiguous rows that do not overlap")
+        raise ValueError("block_tables must be int32 [rows, columns] with contiguous rows that do not overlap")
     for name, t in (("seq_lens", seq_lens), ("table_rows", table_rows), ("req_list", req_list)):
         if t is not None and (t.dtype != torch.int32 or t.ndim != 1 or not t.is_contiguous()):
             raise ValueError(f"{name} must be contiguous 1-D int32")
@@ -1201,9 +1201,9 @@ def paged_decode_kv8(
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if R == 0:
         return out
-    stride = block_tables.stride(0)
+    width = block_tables.shape[1]
     # of this call alone: calls on other streams and captured graphs have their own
-    need = _kv8_decode_workspace_bytes(index, R, query.shape[1], h, d, bs, stride)
+    need = _kv8_decode_workspace_bytes(index, R, query.shape[1], h, d, bs, width)
     ws = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     status = _launch(
         index,
@@ -1226,7 +1226,8 @@ def paged_decode_kv8(
         d,
         query.shape[1],
         block_tables.data_ptr(),
-        stride,
+        block_tables.stride(0),
+        width,
         block_tables.shape[0],
         _ptr(table_rows),
         seq_lens.data_ptr(),
@@ -1240,7 +1241,7 @@ def paged_decode_kv8(
         int(overlap),
     )
     check(status, "nie_paged_decode_kv8")
-    _count(kv8_launch_count(query.dtype, bs, d, R, stride * bs, h, query.shape[1] // h, False, index))
+    _count(kv8_launch_count(query.dtype, bs, d, R, width * bs, h, query.shape[1] // h, False, index))
     return out
 
 
@@ -1285,9 +1286,9 @@ def varlen_attention_kv8(
         out = torch.empty_like(query, memory_format=torch.contiguous_format)
     if R == 0:
         return out
-    stride = block_tables.stride(0)
+    width = block_tables.shape[1]
     # of this call alone: calls on other streams and captured graphs have their own
-    need = _kv8_varlen_workspace_bytes(index, R, query.shape[1], h, d, bs, stride, max_query_len)
+    need = _kv8_varlen_workspace_bytes(index, R, query.shape[1], h, d, bs, width, max_query_len)
     ws = torch.empty(need, dtype=torch.uint8, device=query.device) if need else None
     status = _launch(
         index,
@@ -1310,7 +1311,8 @@ def varlen_attention_kv8(
         d,
         query.shape[1],
         block_tables.data_ptr(),
-        stride,
+        block_tables.stride(0),
+        width,
         block_tables.shape[0],
         _ptr(table_rows),
         seq_lens.data_ptr(),
@@ -1324,8 +1326,8 @@ def varlen_attention_kv8(
         need,
     )
     check(status, "nie_varlen_attention_kv8")
-    long = need == _kv8_varlen_workspace_bytes(index, R, query.shape[1], h, d, bs, stride, 2**31 - 1)
-    _count(kv8_launch_count(query.dtype, bs, d, R, stride * bs, h, max_query_len * (query.shape[1] // h), long, index))
+    long = need == _kv8_varlen_workspace_bytes(index, R, query.shape[1], h, d, bs, width, 2**31 - 1)
+    _count(kv8_launch_count(query.dtype, bs, d, R, width * bs, h, max_query_len * (query.shape[1] // h), long, index))
     return out
 
 
