@@ -430,7 +430,9 @@ int nie_linear_timeout_test(const void* x, int64_t ldx, const void* w, int64_t n
  * The scale s of a run is the least power of two with max|x| <= 448 s.  Where
  * the run continues a block (its first slot is not the block's first), s is not
  * below the block's scale, and if it is above, the codes in front of the run
- * are brought to s.  Non-finite values are stored as NaN and do not count for the scale;
+ * are brought to s.  Appending is all that this does: what a block holds behind
+ * a run is not kept, neither by a run that begins the block (whatever its scale
+ * was before) nor by one that raises its scale.  Non-finite values are stored as NaN and do not count for the scale;
  * magnitudes above 448 * 2^48 saturate.  Slots below 0 are skipped; slots at or
  * past num_blocks * block_size are skipped and raise NIE_DEV_ERR_SLOT_RANGE.
  */

@@ -13,7 +13,8 @@
 // and have slots that follow one another ("a run") share s = 2^e, the least power of
 // two with max|x| <= 448 s.  A run that continues a block (its first slot is
 // not the block's first) never lowers the block's scale; where it raises it,
-// the codes before the run are brought to the new scale.  A power of two
+// the codes before the run are brought to the new scale; those behind it are not
+// looked at, and a run that begins a block replaces the scale: a block is appended to.  A power of two
 // costs no precision in a floating format and makes that step exact except
 // for codes that become subnormal.  Scales stay in [2^-48, 2^48]; values
 // beyond 448 * 2^48 saturate.  Non-finite values are stored as NaN and do not

@@ -986,7 +986,8 @@ def rope_write_kv8(
     The rotation is fp32, rounded once.  The tokens of the call that lie in one block (neighbours,
     as :func:`pack_ragged` gives them; a block may not occur in two places of a call) share per kv
     head the least power-of-two scale that holds them; where they continue a block its scale never
-    falls, and where it grows the block's earlier codes are brought to it.  Non-finite values are
+    falls, and where it grows the block's earlier codes are brought to it.  What a block holds behind
+    the call's tokens is not kept (:meth:`PagedKVCache.write` writes anywhere).  Non-finite values are
     stored as NaN.  Returns the rotated queries as ``[T, q_heads, D]``.
     """
     L, nb, bs, h, d = _kv8_geometry(key_cache, value_cache, key_scales, value_scales, layer)

@@ -97,6 +97,7 @@ class PagedKVCache:
         self.head_dim = head_dim
         self._block_tables: dict[str, list[int]] = {}
         self._sequence_lengths: dict[str, int] = {}
+        self._written: dict[str, list[int]] = {}  # 8-bit caches: per layer, the end of what write() stored
 
         self.quantized = dtype == ops.KV8_DTYPE
         if self.quantized and head_dim % 2:
@@ -184,6 +185,7 @@ class PagedKVCache:
         self.allocator.free(ids)
         del self._block_tables[sequence_id]
         del self._sequence_lengths[sequence_id]
+        self._written.pop(sequence_id, None)
         self._release_row(sequence_id)
 
     # ------------------------------------------------- device table mirror
@@ -277,7 +279,10 @@ class PagedKVCache:
 
     # ------------------------------------------------------------ data ops
     def write(self, layer_index: int, sequence_id: str, start_position: int, keys, values) -> None:
-        """Store K/V rows at consecutive positions (reference paged_cache.py:264-322)."""
+        """Store K/V rows at consecutive positions (reference paged_cache.py:264-322).
+
+        In an 8-bit cache the stored rows of a block share a scale: those around the new ones keep
+        their values, with another rounding where the block's scale grows."""
         if not _is_int(layer_index):
             raise TypeError("layer_index must be an integer")
         if layer_index < 0 or layer_index >= self.num_layers:
@@ -307,12 +312,39 @@ class PagedKVCache:
         if keys.device != self.keys.device or values.device != self.values.device:
             raise ValueError("keys and values must be on the cache device")
         self._resolve_position(sequence_id, start_position + token_count - 1)
-        meta = self.pack((sequence_id,), (start_position,), (token_count,))
         if self.quantized:
-            ops.write_kv8(keys, values, self.keys, self.values, self.key_scales, self.value_scales, layer_index,
-                          meta.slot_mapping)
+            self._write_kv8(layer_index, sequence_id, start_position, keys, values)
             return
+        meta = self.pack((sequence_id,), (start_position,), (token_count,))
         ops.write_kv(keys, values, self.keys, self.values, layer_index, meta.slot_mapping)
+
+    def _write_kv8(self, layer_index: int, sequence_id: str, start: int, keys, values) -> None:
+        """:meth:`write` of an 8-bit cache.
+
+        The kernel appends: a run from a block's first slot begins the block anew, one from a later
+        slot goes by the block's scale, and neither looks at the rows behind it.  So rows that are
+        stored behind the run in its last block are read and written with it, and a block that holds
+        nothing yet forgets the scale of its owner before."""
+        bs = self.block_size
+        end = start + keys.shape[0]
+        written = self._written.setdefault(sequence_id, [0] * self.num_layers)
+        stored = max(self._sequence_lengths[sequence_id], written[layer_index])
+        table = self._block_tables[sequence_id]
+        if start % bs and stored <= start - start % bs:
+            with torch.inference_mode():  # whichever mode the cache was made in
+                for scales in (self.key_scales, self.value_scales):
+                    scales[layer_index, table[start // bs]].zero_()
+        last = (end - 1) // bs  # the run's last block
+        behind = min(stored, (last + 1) * bs)
+        if behind > end:
+            row = self.device_block_tables()[self._rows[sequence_id]]
+            k, v = ops.gather_kv8(self.keys, self.values, self.key_scales, self.value_scales, layer_index,
+                                  row[last : last + 1], behind - last * bs, dtype=torch.float32)
+            keys, values = (torch.cat([new.float(), old[end - last * bs :]]) for new, old in ((keys, k), (values, v)))
+        meta = self.pack((sequence_id,), (start,), (keys.shape[0],))
+        ops.write_kv8(keys, values, self.keys, self.values, self.key_scales, self.value_scales, layer_index,
+                      meta.slot_mapping)
+        written[layer_index] = max(written[layer_index], end)
 
     def gather(
         self, layer_index: int, sequence_id: str, token_count: int, *, dtype: torch.dtype | None = None
