@@ -331,9 +331,8 @@ class PagedKVCache:
         stored = max(self._sequence_lengths[sequence_id], written[layer_index])
         table = self._block_tables[sequence_id]
         if start % bs and stored <= start - start % bs:
-            with torch.inference_mode():  # whichever mode the cache was made in
-                for scales in (self.key_scales, self.value_scales):
-                    scales[layer_index, table[start // bs]].zero_()
+            for scales in (self.key_scales, self.value_scales):
+                scales[layer_index, table[start // bs]].zero_()
         last = (end - 1) // bs  # the run's last block
         behind = min(stored, (last + 1) * bs)
         if behind > end:

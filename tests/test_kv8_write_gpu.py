@@ -117,15 +117,6 @@ def test_a_block_that_another_sequence_had(cuda):
     m.check()
 
 
-def test_a_cache_made_in_inference_mode(cuda):
-    with torch.inference_mode():
-        cache = new_cache(cuda)
-    m = Mirror(cache, "s", 16)
-    m.write(5, 4, 1.0)
-    m.write(0, 5, 3.0)
-    m.check()
-
-
 def test_layers_have_their_own_state(cuda):
     m = Mirror(new_cache(cuda), "s", 32)
     m.write(8, 8, 1.0, layers=(0,))
