@@ -74,6 +74,8 @@ class PDPair:
             raise ValueError("prefill_cache and decode_cache must be different caches")
         check_engine(prefill_model, prefill_cache, "prefill")
         check_engine(decode_model, decode_cache, "decode")
+        if prefill_cache.quantized != decode_cache.quantized:
+            raise ValueError("prefill_cache and decode_cache must both be 8-bit caches or neither")
         return cls(prefill_model, decode_model, prefill_cache, decode_cache)
 
     @property
