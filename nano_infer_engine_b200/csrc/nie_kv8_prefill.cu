@@ -123,6 +123,11 @@ __device__ __forceinline__ bool f8_wait(F8Bars* b, uint64_t* bar, uint32_t parit
   return false;
 }
 
+// The same out of line, for a wait outside the loops: their code fills the instruction caches as it is.
+__device__ __noinline__ bool f8_wait_call(F8Bars* b, uint64_t* bar, uint32_t parity, int32_t* err) {
+  return f8_wait(b, bar, parity, err);
+}
+
 // The same for warps that run ahead: they sleep between probes, since every probe
 // goes through the queue that the exponentials of the softmax warps use.
 __device__ __forceinline__ bool f8_wait_idle(F8Bars* b, uint64_t* bar, uint32_t parity, int32_t* err) {
@@ -765,6 +770,11 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
         tmem_wait_st();
         return true;
       };
+      // Before a segment's first tile, its scores.  A part without rows passes tiles over without a wait, and its warps
+      // may be two of a stage's phases ahead here, where kv_full's parity would take the older phase for theirs.
+      // Behind s_full the tile's phase is over, and the next one waits for this warp's weights; the stages after it
+      // are one phase behind at most, since the loaders fill them in turn.
+      if (!f8_wait_call(b, &b->s_full[x][used % C::SBufs], (uint32_t)(used / C::SBufs) & 1u, a.err)) break;
       for (int kt = tlo; kt < thi; ++kt, ++used) {
         // the loaders' factors are there before the scores: waited for while there is time
         if (!f8_wait(b, &b->kv_full[st], kv_par, a.err) ||
