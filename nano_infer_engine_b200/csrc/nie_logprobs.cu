@@ -21,8 +21,10 @@
 // passes it goes to a buffer of (value, index) keys, whose k-th best, found by
 // counting, is the bound of the next rounds.  It is raised behind rounds 1, 2, 4, 8,
 // ..., so that about k values of each doubling pass it and most rounds need no
-// barrier.  Rows that overflow the buffer (values that rise all the way) are gone
-// through again, with the bound raised after every load.
+// barrier.  Loads of nothing but forbidden tokens bring no key: a mask may leave fewer
+// values than a bound takes.  Rows that overflow the buffer (values that rise all the way), or
+// have fewer than k values above the lowest that the maxima know and some below, are
+// gone through again, with the bound raised after every load.
 //
 // Few rows are split over a cluster of up to 4 CTAs; the first one merges the
 // others' sums and keys through distributed shared memory.
@@ -105,6 +107,7 @@ struct LpPair;
 template <>
 struct LpPair<__nv_bfloat16> {
   static constexpr float kLowest = -1.2959972171045839e38f;  // 0xfec3
+  static constexpr uint32_t kNone = 0xff80ff80u;  // -inf, -inf
   static __device__ __forceinline__ uint32_t finite(uint32_t a) { return larger(a, 0xfec3fec3u); }
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
     uint32_t d;
@@ -118,6 +121,7 @@ struct LpPair<__nv_bfloat16> {
 template <>
 struct LpPair<__half> {
   static constexpr float kLowest = -65504.f;
+  static constexpr uint32_t kNone = 0xfc00fc00u;
   static __device__ __forceinline__ uint32_t finite(uint32_t a) { return larger(a, 0xfbfffbffu); }
   static __device__ __forceinline__ uint32_t larger(uint32_t a, uint32_t b) {
     uint32_t d;
@@ -129,6 +133,7 @@ struct LpPair<__half> {
 template <>
 struct LpPair<float> {
   static constexpr float kLowest = -kLpRange;
+  static constexpr uint32_t kNone = 0xff800000u;
 };
 __device__ __forceinline__ float lp_max_nan(float a, float b) {
   float d;
@@ -201,6 +206,7 @@ struct __align__(16) LpShared {
   uint4 queue[kLpQueue];
   int queue_at[kLpQueue];       // their places in the row, in loads
   int queued;
+  int low;                      // a load of nothing but values up to kLowest, not all of them -inf, was left out
   float groups[32];
   LpSums sums[kLpWarps];
   int count;                    // keys offered; those past kLpCap are lost
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_co
   const int v0 = min(nvec, part * share), v1 = min(nvec, v0 + share);
   const uint4* vec = reinterpret_cast<const uint4*>(row + head);
 
-  if (tid == 0) sh.count = sh.queued = 0;
+  if (tid == 0) sh.count = sh.queued = sh.low = 0;
   __syncthreads();
 
   LpSums mine{-1.5f * kLpRange, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
@@ -350,12 +356,16 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_co
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int v = from + u * kLpThreads + tid;
-          if (v < v1 && top[u] >= floor_v) {
+          if (v >= v1 || top[u] < floor_v) continue;
+          if (top[u] > LpPair<T>::kLowest) {
             const int at = atomicAdd(&sh.queued, 1);
             if (at < kLpQueue) {
               sh.queue[at] = raw[u];
               sh.queue_at[at] = v;
             }
+          } else if (raw[u].x != LpPair<T>::kNone || raw[u].y != LpPair<T>::kNone || raw[u].z != LpPair<T>::kNone ||
+                     raw[u].w != LpPair<T>::kNone) {
+            sh.low = 1;
           }
         }
       }
@@ -395,8 +405,14 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_co
   }
   if constexpr (TOP) {
     __syncthreads();
-    if (sh.count > kLpCap || sh.queued > kLpQueue) {
-      // some were lost: all again, the bound raised on the way; a round's 256 values and 512 keys fit
+    bool again = sh.count > kLpCap || sh.queued > kLpQueue;  // some were lost
+    if (!again && sh.low) {  // some were left out: needed if one of their kind is among the k best
+      const int n = sh.count;
+      if (n >= k) lp_rank(sh, n, k);
+      again = n < k || !(lp_value(sh.best[k - 1]) > LpPair<T>::kLowest);
+    }
+    if (again) {
+      // all again, the bound raised on the way; a round's 256 values and 512 keys fit
       __syncthreads();
       if (tid == 0) sh.count = 0;
       set_bound(0);
