@@ -534,6 +534,10 @@ int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, void* out,
                              void* workspace, size_t workspace_bytes,
                              int32_t* err_flag, void* stream);
 
+/* Kernels that the calling thread's last nie_paged_decode_kv8 or
+ * nie_varlen_attention_kv8 launched. */
+int nie_kv8_launch_count(void);
+
 /*
  * nie_token_logprobs: for each row of logits (`cols` elements at row_stride)
  *   logprobs[r]  log softmax(logits[r])[tokens[r]]

@@ -137,6 +137,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_size_t,
         [c_int, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32],
     ),
+    "nie_kv8_launch_count": (c_int, []),
     "nie_token_logprobs": (
         c_int,
         [c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p]

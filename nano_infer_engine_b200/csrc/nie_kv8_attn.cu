@@ -12,6 +12,11 @@
 
 namespace nie {
 
+int& kv8_launches() {
+  static thread_local int n = 0;
+  return n;
+}
+
 constexpr int kG8Warps = 4;
 constexpr int kG8MaxHd = 256;
 
@@ -103,6 +108,7 @@ __global__ void __launch_bounds__(kG8Warps * 32) kv8_generic_kernel(Kv8Args a) {
 static int launch_kv8_generic(int dtype, const Kv8Args& a, int num_req, int max_q, cudaStream_t s) {
   if (a.hd > kG8MaxHd) return fail(NIE_ERR_UNSUPPORTED, "head_dim %d > %d", a.hd, kG8MaxHd);
   if (a.hq > 65535) return fail(NIE_ERR_UNSUPPORTED, "too many query heads: %d", a.hq);
+  ++kv8_launches();
   const dim3 grid((unsigned)num_req, (unsigned)std::min(std::max(max_q, 1), 65535), (unsigned)a.hq);
   switch (dtype) {
     case NIE_DTYPE_F32: kv8_generic_kernel<float><<<grid, kG8Warps * 32, 0, s>>>(a); break;
@@ -167,6 +173,7 @@ extern "C" int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* o
                                     const int32_t* req_list, int32_t num_requests, float scale,
                                     void* workspace, size_t workspace_bytes, int32_t overlap, int32_t* err_flag,
                                     void* stream) {
+  kv8_launches() = 0;
   Kv8Args a{};
   a.q = q, a.out = out, a.q_stride = q_row_stride, a.out_stride = out_row_stride, a.num_q_rows = num_q_rows;
   a.kc = (const uint8_t*)key_cache, a.vc = (const uint8_t*)value_cache, a.ks = key_scales, a.vs = value_scales;
@@ -189,6 +196,8 @@ extern "C" int nie_paged_decode_kv8(const void* q, int64_t q_row_stride, void* o
   return launch_kv8_generic(dtype, a, num_requests, 1, s);
 }
 
+extern "C" int nie_kv8_launch_count(void) { return kv8_launches(); }
+
 extern "C" size_t nie_paged_decode_kv8_workspace_size(int device, int32_t num_requests, int32_t q_heads,
                                                       int32_t kv_heads, int32_t head_dim, int32_t block_size,
                                                       int64_t table_width) {
@@ -209,6 +218,7 @@ extern "C" int nie_varlen_attention_kv8(const void* q, int64_t q_row_stride, voi
                                         const int32_t* req_list, int32_t num_requests, int32_t max_query_len,
                                         float scale, void* workspace, size_t workspace_bytes, int32_t* err_flag,
                                         void* stream) {
+  kv8_launches() = 0;
   Kv8Args a{};
   a.q = q, a.out = out, a.q_stride = q_row_stride, a.out_stride = out_row_stride, a.num_q_rows = num_q_rows;
   a.kc = (const uint8_t*)key_cache, a.vc = (const uint8_t*)value_cache, a.ks = key_scales, a.vs = value_scales;

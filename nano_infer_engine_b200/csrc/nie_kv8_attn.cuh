@@ -55,6 +55,9 @@ __device__ __forceinline__ Kv8Rows kv8_rows(const Kv8Args& a, int r, int32_t* er
   return x;
 }
 
+// Kernels that the calling thread's last attention call launched; each launch adds itself.
+int& kv8_launches();
+
 // The kernel of single tokens (nie_kv8_decode.cu), where kv8_decode_takes() says
 // so; workspace of kv8_decode_workspace() bytes, 256-byte aligned (none where it is 0).
 bool kv8_decode_takes(int dtype, const Kv8Args& a);

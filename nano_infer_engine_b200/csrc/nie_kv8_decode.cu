@@ -749,9 +749,11 @@ static int launch_decode(const Kv8Args& a, const D8Plan& p, dim3 grid, int sms, 
     attr[cfg.numAttrs].val.clusterDim.y = attr[cfg.numAttrs].val.clusterDim.z = 1;
     ++cfg.numAttrs;
   }
+  ++kv8_launches();
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a, p);
   if (e != cudaSuccess) return fail(NIE_ERR_CUDA, "kv8_decode_kernel launch: %s", cudaGetErrorString(e));
   if (p.whole) return NIE_OK;
+  ++kv8_launches();
   // A request is cut into 1 + grid.x / requests parts on average, so a large batch's requests into few: four groups
   // take them in one round of loads, and more of the small CTAs are on the GPU at once.  64 requests of up to 29600
   // keys x 32 heads take 169.2 us in all with 4 groups of a whole row and 173.2 with 16.  Few requests have many

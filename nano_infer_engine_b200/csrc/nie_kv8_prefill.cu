@@ -921,6 +921,7 @@ static int launch_prefill(const Kv8Args& a, const F8Plan& p, int sms, cudaStream
   auto* kernel = kv8_prefill_kernel<HD, T>;
   const int rc = opt_in_smem(kSmemKv8Prefill + (HD == 128) * 2 + std::is_same<T, __half>::value, (const void*)kernel, smem);
   if (rc != NIE_OK) return rc;
+  kv8_launches() += 2;
   kernel<<<sms, C::Threads, smem, s>>>(a, p);
   const int st = check_launch("kv8_prefill_kernel");
   if (st != NIE_OK) return st;

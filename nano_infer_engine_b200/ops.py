@@ -1242,7 +1242,7 @@ def paged_decode_kv8(
         int(overlap),
     )
     check(status, "nie_paged_decode_kv8")
-    _count(kv8_launch_count(query.dtype, bs, d, R, width * bs, h, query.shape[1] // h, False, index))
+    _count(lib.nie_kv8_launch_count())
     return out
 
 
@@ -1327,8 +1327,7 @@ def varlen_attention_kv8(
         need,
     )
     check(status, "nie_varlen_attention_kv8")
-    long = need == _kv8_varlen_workspace_bytes(index, R, query.shape[1], h, d, bs, width, 2**31 - 1)
-    _count(kv8_launch_count(query.dtype, bs, d, R, width * bs, h, max_query_len * (query.shape[1] // h), long, index))
+    _count(lib.nie_kv8_launch_count())
     return out
 
 
@@ -1359,31 +1358,3 @@ def decode_launch_count(dtype: torch.dtype, block_size: int, kv_heads: int, head
     """Kernels one :func:`paged_decode` call launches (split-K kernel + combine, or the generic one)."""
     fast = dtype == torch.bfloat16 and head_dim == 64 and block_size == 16 and q_heads // kv_heads <= 16 and kv_heads <= 16
     return 2 if fast else 1
-
-
-@functools.lru_cache(maxsize=1024)
-def kv8_launch_count(
-    dtype: torch.dtype, block_size: int, head_dim: int, num_requests: int, max_keys: int, kv_heads: int, columns: int,
-    long: bool, index: int,
-) -> int:
-    """Kernels of one :func:`paged_decode_kv8` or :func:`varlen_attention_kv8` (``long``: not the form of few
-    tokens) call on a device.
-
-    ``max_keys``: that the tables hold; ``columns``: (tokens x) query heads to a kv head.  One kernel and its
-    merging kernel per 256 requests of any length, or per 512 of a few tokens, where the tables are too long
-    for a cluster to a request; the generic kernel for what the others do not take."""
-    if dtype == torch.float32 or head_dim not in (64, 128) or block_size % 16:
-        return 1
-    if long:
-        return 2 * -(-num_requests // 256)
-    sets = kv_heads * -(-columns // (16 if head_dim == 64 else 8))
-    sets = sets // 2 if sets % 2 == 0 else sets
-    places = 2 * int(lib.nie_device_sm_count(index))
-    total = 0
-    for at in range(0, num_requests, 512):
-        room = places // (min(512, num_requests - at) * sets)
-        ctas = 1
-        while ctas < 8 and 2 * ctas <= room and max_keys > 256 * ctas:
-            ctas *= 2
-        total += 1 if max_keys <= 1024 * ctas else 2
-    return total
