@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(kD8Warps * 32, 2) kv8_decode_kernel(const __gr
       const int n = min(16, len[i] - tok);
       if (n > 0) {
         const int lb = tok / a.bs;
-        const int64_t block = lb < a.twidth ? (int64_t)a.tables[(int64_t)trow[i] * a.tstride + lb] : -1;
+        const int64_t block = a.tables[(int64_t)trow[i] * a.tstride + lb];  // lb is in the table: no length passes it
         if (block < 0 || block >= a.nb) {
           raise_flag(a.err, NIE_DEV_ERR_BLOCK_RANGE);
         } else {
