@@ -757,10 +757,15 @@ static int launch_decode(const Kv8Args& a, const D8Plan& p, dim3 grid, int sms, 
   // A request is cut into 1 + grid.x / requests parts on average, so a large batch's requests into few: four groups
   // take them in one round of loads, and more of the small CTAs are on the GPU at once.  64 requests of up to 29600
   // keys x 32 heads take 169.2 us in all with 4 groups of a whole row and 173.2 with 16.  Few requests have many
-  // parts: one of 131072 keys takes 46.1 us with 4 groups, 36.4 with 16, 35.5 with 32 groups of 32 dims each.
+  // parts.  With 4 groups, 16, and 32 of 32 dims each, on wide tables: one of 131072 keys x 32 heads 45.6, 36.4 and
+  // 35.5 us, one of 29600 18.5, 14.1 and 14.3, 4 of 4001 12.3, 11.9 and 11.8, 8 14.4, 13.8 and 14.0, 16 of 1 to 4001
+  // 17.7, 17.3 and 19.4, 18 of 1 to 2000 14.4, 13.9 and 16.4, 16 of 1 to 29600 55.2, 54.8 and 57.1.
   const dim3 merge_grid((unsigned)p.num_req, (unsigned)(a.hkv * p.cols));
-  if ((int64_t)p.num_req * a.hkv * p.cols > 4 * sms)
+  const int64_t rows = (int64_t)p.num_req * a.hkv * p.cols;
+  if (rows > 4 * sms)
     pdl_launch(kv8_decode_merge_kernel<HD, 4, HD / 4, MULTI, T>, merge_grid, dim3(HD), s, a, p);
+  else if (rows > sms)
+    pdl_launch(kv8_decode_merge_kernel<HD, 16, HD / 4, MULTI, T>, merge_grid, dim3(4 * HD), s, a, p);
   else
     pdl_launch(kv8_decode_merge_kernel<HD, 32, 8, MULTI, T>, dim3(merge_grid.x, merge_grid.y, HD / 32), dim3(256), s, a, p);
   return check_launch("kv8_decode_merge_kernel");
