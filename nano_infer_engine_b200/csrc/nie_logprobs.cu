@@ -352,21 +352,28 @@ __global__ void __launch_bounds__(kLpThreads, 4) logprobs_kernel(const __grid_co
         const float b = __shfl_sync(0xffffffffu, g, __ffs(at) - 1);
         if (b > LpPair<T>::kLowest) set_bound((lp_key(b, 0) >> 32) << 32);  // that value at any index
       }
-      if (most >= floor_v) {
+      // loads that hold something above kLowest, and above the bound where there is one
+      const float gate = fmaxf(floor_v, __uint_as_float(__float_as_uint(LpPair<T>::kLowest) - 1u));
+      if (most >= gate) {
 #pragma unroll
         for (int u = 0; u < U; ++u) {
           const int v = from + u * kLpThreads + tid;
-          if (v >= v1 || top[u] < floor_v) continue;
-          if (top[u] > LpPair<T>::kLowest) {
+          if (v < v1 && top[u] >= gate) {
             const int at = atomicAdd(&sh.queued, 1);
             if (at < kLpQueue) {
               sh.queue[at] = raw[u];
               sh.queue_at[at] = v;
             }
-          } else if (raw[u].x != LpPair<T>::kNone || raw[u].y != LpPair<T>::kNone || raw[u].z != LpPair<T>::kNone ||
-                     raw[u].w != LpPair<T>::kNone) {
-            sh.low = 1;
           }
+        }
+      }
+      if (floor_v == -INFINITY) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          if (from + u * kLpThreads + tid < v1 && top[u] < gate &&
+              (raw[u].x != LpPair<T>::kNone || raw[u].y != LpPair<T>::kNone || raw[u].z != LpPair<T>::kNone ||
+               raw[u].w != LpPair<T>::kNone))
+            sh.low = 1;
         }
       }
       // behind rounds 1, 2, 4, 8, ...: about k values of each doubling pass the bound
