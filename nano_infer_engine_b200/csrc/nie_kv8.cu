@@ -26,7 +26,9 @@
 // first pair of them stays in registers between the run's maximum and its codes.
 // Registers decide: with two pairs and four CTAs to an SM the loops' state went to
 // memory and 16384 tokens (32 + 2 x 8 heads of 64, bf16) took 55 us; with one and
-// three CTAs 44 us, 185 MB at 4.2 TB/s, of which the queries' 134 MB take 24.
+// three CTAs 43 us, 185 MB at 4.3 TB/s, of which the queries' 134 MB take 24.  fp32
+// rows 68 us.  Other sizes and alignments take the plain kernel: 2048 tokens of heads of
+// 72 62 us, where those of 64 take 7.
 //
 // One warp owns a (block, kv head, K or V) and takes the block's runs in turn,
 // as calls of their own would be, so no two warps write one scale or one code

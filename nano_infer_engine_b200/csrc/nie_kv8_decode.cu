@@ -5,7 +5,7 @@
 // multiply-adds per query head of its group, far below the tensor rate, so the
 // work is to keep the loads of all SMs in flight and the instructions per code
 // few enough to hide behind them.  Measured: 64 requests of up to 29600 keys, 8 kv
-// heads of 64, 171 us, 5.7 TB/s of codes; one of 131072 keys, 4 of 128, 36 us, 3.6
+// heads of 64, 171 us, 5.7 TB/s of codes; one of 131072 keys, 4 of 128, 35 us, 3.8
 // TB/s (27 us of it without any arithmetic, 6 in the merging kernel); 16 of up to
 // 4001 keys 17 us, which the longest one's share of a cluster decides.
 //
@@ -756,7 +756,7 @@ static int launch_decode(const Kv8Args& a, const D8Plan& p, dim3 grid, int sms, 
   ++kv8_launches();
   // A request is cut into 1 + grid.x / requests parts on average, so a large batch's requests into few: four groups
   // take them in one round of loads, and more of the small CTAs are on the GPU at once.  64 requests of up to 29600
-  // keys x 32 heads take 169.2 us in all with 4 groups of a whole row and 173.2 with 16.  Few requests have many
+  // keys x 32 heads take 171.1 us in all with 4 groups of a whole row and 175.9 with 16.  Few requests have many
   // parts.  With 4 groups, 16, and 32 of 32 dims each, on wide tables: one of 131072 keys x 32 heads 45.6, 36.4 and
   // 35.5 us, one of 29600 18.5, 14.1 and 14.3, 4 of 4001 12.3, 11.9 and 11.8, 8 14.4, 13.8 and 14.0, 16 of 1 to 4001
   // 17.7, 17.3 and 19.4, 18 of 1 to 2000 14.4, 13.9 and 16.4, 16 of 1 to 29600 55.2, 54.8 and 57.1.
@@ -780,8 +780,9 @@ static void d8_columns(D8Plan& p, const Kv8Args& a, int max_query_len) {
   p.subs = (p.cols + most - 1) / most;
   p.rows = (p.cols + p.subs - 1) / p.subs;
   const int sets = a.hkv * p.subs;
-  // Two column sets to a CTA halve the warps that are merged per set.  64 requests of 29600 keys, 8 sets: 178.7 us
-  // with one, 173.1 with two, 174.2 and 176 with four and eight; one of 131072 keys: 33.9, 35.9, 40.2, 40.1.
+  // Two column sets to a CTA halve the warps that are merged per set.  With one, two, four and eight: 64 requests of up
+  // to 29600 keys, 8 sets, 175.2, 171.1, 171.9 and 174.0 us; 16 of 1 to 4001 on wide tables 18.1, 16.5, 16.5 and 17.5;
+  // 8 x 5 drafts, 16 sets, 15.9, 16.3, 18.1 and 21.7; one of 131072 keys, 4 sets, 34.3, 35.8 and 39.5.
   p.hc = sets % 2 == 0 ? 2 : 1;
   p.ts = kD8Warps / p.hc;
   p.min_tiles = p.ts;

@@ -5,9 +5,9 @@
 // clock and SM against 8192 flops of f16 MMA, head_dim 64 spends twice the MMA's
 // time in exp2 and head_dim 128 the same.  So the MMAs run behind the softmax, and
 // all else (loads, 8 bit to f16) is done by warps of its own.  Measured: 8192 tokens
-// of one prompt, 32 heads on 8 of 64, bf16: 585 us, 470 TFLOP/s of causal work, of
+// of one prompt, 32 heads on 8 of 64, bf16: 586 us, 470 TFLOP/s of causal work, of
 // which exp2 alone is 240 us and the MMAs 185; 6 x 513 tokens behind up to 4000, 16
-// on 4 of 128, f16: 88 us, 448 TFLOP/s.  What is left is the latency of a row's chain.
+// on 4 of 128, f16: 87 us, 453 TFLOP/s.  What is left is the latency of a row's chain.
 //
 // Rows.  The query heads of a kv head share its codes, so the rows of a tile are
 // (token, head of the group) pairs in that order, of one kv head, in MMA tiles of
@@ -55,7 +55,8 @@ constexpr int kF8MaxReq = 256;     // requests of one launch
 constexpr int kF8MaxStages = 4;
 constexpr uint32_t kF8OCol = 256;
 // A segment's fixed part (its queries, its first and last waits, its output), in key tiles.  With 2, 5 and 10: 6 x
-// 513 tokens behind up to 4000 take 90.1, 86.5 and 93.4 us, 8192 of one prompt 604, 585 and 600.
+// 513 tokens behind up to 4000 take 93.7, 88.5 and 95.2 us, 8192 of one prompt 597, 589 and 602; less even loads
+// differ: 513 tokens behind 487 35, 37 and 40, 16 x 128 behind 2872 133, 136 and 141, 90 x 65 behind 5 43, 48 and 43.
 constexpr int kF8SegCost = 5;
 constexpr uint32_t kF8Wait = 1u << 22;
 constexpr float kF8Log2e = 1.4426950408889634f;

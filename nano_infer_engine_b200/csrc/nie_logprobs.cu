@@ -8,8 +8,9 @@
 // What bounds it: the row is read once, 16 bytes a load; at 12 bf16 values a clock
 // and SM the exponentials (16 a clock) and the instructions around them (5 to a
 // value) are close behind.  So everything comes from one pass, in pairs of values.
-// Measured: 4096 rows of 128256 bf16 values with 20 alternatives 242 us (4.3 TB/s), 333 of
-// 50257 fp32 values with 3 20 us (3.3 TB/s), one row with 5 11.5 us.
+// Measured: 4096 rows of 128256 bf16 values with 20 alternatives 244 us (4.3 TB/s), without
+// any 164 (6.4 TB/s), 333 of 50257 fp32 values with 3 20 us (3.3 TB/s), one row with 5 11.7
+// us, without any 6.6.
 //
 // Sums: every thread keeps (reference, Z, S) of its own values in fp32; the
 // reference is raised only when exceeded by 8 (e^8 leaves fp32 room enough), and the
