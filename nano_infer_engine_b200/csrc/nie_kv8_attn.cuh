@@ -58,6 +58,16 @@ __device__ __forceinline__ Kv8Rows kv8_rows(const Kv8Args& a, int r, int32_t* er
 // Kernels that the calling thread's last attention call launched; each launch adds itself.
 int& kv8_launches();
 
+// 16 bytes to shared memory, those past `bytes` zeros.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
 // The kernel of single tokens (nie_kv8_decode.cu), where kv8_decode_takes() says
 // so; workspace of kv8_decode_workspace() bytes, 256-byte aligned (none where it is 0).
 bool kv8_decode_takes(int dtype, const Kv8Args& a);

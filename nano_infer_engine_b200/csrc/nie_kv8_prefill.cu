@@ -160,13 +160,6 @@ __device__ __forceinline__ void f8_add2(float& d0, float& d1, float b0, float b1
       : "=f"(d0), "=f"(d1)
       : "f"(d0), "f"(d1), "f"(b0), "f"(b1));
 }
-__device__ __forceinline__ uint32_t f8_pack(float lo, float hi) {
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-__device__ __forceinline__ void f8_cp16(uint32_t dst, const void* src, int bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
 
 // kind::f16 with f16 (or bf16) A and B, f32 D.
 constexpr uint32_t f8_idesc(int m, int n, bool b_mn_major, bool bf16) {
@@ -460,8 +453,8 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
           const bool there = row < __shfl_sync(0xffffffffu, here, s);
           const int64_t off =
               there ? (int64_t)(from + row) * row_bytes + (int64_t)ahead.h * HD + half * 64 + (tid & 3) * 16 : 0;
-          f8_cp16(base + j * (C::Loaders * 16), a.kc + off, there ? 16 : 0);
-          f8_cp16(base + (Copies + j) * (C::Loaders * 16), a.vc + off, there ? 16 : 0);
+          cp_async16(base + j * (C::Loaders * 16), a.kc + off, there ? 16 : 0);
+          cp_async16(base + (Copies + j) * (C::Loaders * 16), a.vc + off, there ? 16 : 0);
         }
         if (++a_kt >= ahead.t_hi()) {
           ahead.next(a, R);
@@ -654,7 +647,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
       const uint32_t dst = smem_u32(sq) + x * C::PartBytes + t * 128;
 #pragma unroll
       for (int c = 0; c < HD / 8; ++c)
-        f8_cp16(dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (t & 7)) << 4), q + c * 8, there ? 16 : 0);
+        cp_async16(dst + (c >> 3) * (128 * 128) + (((c & 7) ^ (t & 7)) << 4), q + c * 8, there ? 16 : 0);
     };
     auto queries_there = [&]() {
       asm volatile("cp.async.wait_all;" ::: "memory");
@@ -762,7 +755,7 @@ __global__ void __launch_bounds__(F8Cfg<HD>::Threads, 1)
               }
               const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
               f8_add2(r0, r1, p0, p1);
-              pk[e / 2] = f8_pack(p0, p1);
+              pk[e / 2] = pack_f16x2(p0, p1);
             }
             l = fmaf(r0 + r1, h ? f1.z : f0.z, l);
           }
